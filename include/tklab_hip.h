@@ -407,6 +407,23 @@ int tk_gqa_decode(int dtype, const void* q, const void* k, const void* v, void* 
                   const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                   const int64_t* o_strides, float scale, void* stream);
 
+/* Rotary positions of one call's queries and (when `k` is non-null) keys:
+ *   y1 = m (x1 cos a - x2 sin a),  y2 = m (x2 cos a + x1 sin a),  a = position * frequencies[pair]
+ * over the pairs of the first rotary_dim features, (i, i + rotary_dim / 2) or, with
+ * `interleaved`, (2i, 2i + 1); later features are copied. `inverse` turns by -a (the gradient).
+ * Row (b, h, n) of a tensor starts at b strides[0] + h strides[1] + n strides[2] and has
+ * head_dim <= 1024 unit-stride features; its position is positions[b position_strides[0] +
+ * n position_strides[1]], int32, or int64 with `wide_positions`. `frequencies` is
+ * float64[rotary_dim / 2] in radians per position. Any alignment the dtype allows; outputs may
+ * not overlap inputs. No counterpart in the reference (its tables are per row and its pairs
+ * halves of the whole feature dimension, src/tklab/kernels/rope.py:26-73). */
+int tk_rotary(int dtype, const void* q, void* q_out, const void* k, void* k_out,
+              const void* positions, const double* frequencies, int64_t batch, int64_t tokens,
+              int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim,
+              const int64_t* q_strides, const int64_t* q_out_strides, const int64_t* k_strides,
+              const int64_t* k_out_strides, const int64_t* position_strides, float magnitude,
+              int interleaved, int wide_positions, int inverse, void* stream);
+
 /* ---- Calibration kernels (no counterpart in the reference). They measure the
  * roofs this GPU sustains, so that the kernels above can be priced against
  * measured ceilings beside the published peaks. */

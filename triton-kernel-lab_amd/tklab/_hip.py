@@ -105,6 +105,10 @@ _SIGNATURES: dict[str, list[object]] = {
         _I32, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
         _I64P, _F32, _P,
     ],
+    "tk_rotary": [
+        _I32, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
+        _I64P, _I64P, _F32, _I32, _I32, _I32, _P,
+    ],
     "tk_roof_copy": [_P, _P, _I64, _P],
     "tk_roof_stream": [_P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _P],
     "tk_roof_mfma": [_I32, _P, _I64, _I64, _P],
@@ -206,6 +210,15 @@ def call(name: str, *args: object) -> None:
     if status != 0:
         message = load_library().tk_last_error().decode(errors="replace")
         raise HipLibraryError(f"{name} failed: {message}")
+
+
+def call_on(tensor: torch.Tensor, name: str, *args: object) -> None:
+    """:func:`call` with ``tensor``'s device current, whichever device the caller has selected."""
+    if tensor.get_device() == torch.cuda.current_device():
+        call(name, *args)
+        return
+    with torch.cuda.device(tensor.device):
+        call(name, *args)
 
 
 def query(name: str, *args: int | None) -> int:

@@ -1,0 +1,263 @@
+"""Rotary positions from token positions: both pair layouts, part of the head, scaled contexts.
+
+``rope`` takes per-row tables and turns halves of the whole feature dimension, as the reference
+does (``rope.py:26-73``). :func:`rotary_embedding` is the form a model's attention layer needs: it
+turns the queries and keys of a call in one launch, at positions given per token, over the first
+``2 * len(frequencies)`` features of each head, and forms the angles itself in float64, so no
+table bounds the context. :func:`rotary_frequencies` makes the frequencies, plain or scaled for
+contexts longer than a model was trained on. The gradient is the rotation by the negative angle.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Any
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from tklab import _hip
+
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_POSITION_DTYPES = (torch.int32, torch.int64)
+_MAX_HEAD_DIM = 1024
+_SCALINGS = ("none", "linear", "ntk", "yarn")
+
+
+def rotary_frequencies(
+    rotary_dim: int,
+    *,
+    base: float = 10000.0,
+    scaling: str = "none",
+    factor: float = 1.0,
+    original_length: int | None = None,
+    fast_turns: float = 32.0,
+    slow_turns: float = 1.0,
+    device: torch.device | str | None = None,
+) -> tuple[torch.Tensor, float]:
+    """Frequencies (float64 ``[rotary_dim // 2]``, radians per position) and magnitude.
+
+    Pair ``i`` turns by ``base ** (-2 i / rotary_dim)`` radians per position. ``scaling`` stretches
+    that for contexts ``factor`` times the original:
+
+    - ``"linear"``: every frequency divided by ``factor``;
+    - ``"ntk"``: ``base`` multiplied by ``factor ** (d / (d - 2))``, which divides the slowest
+      pair's frequency by ``factor`` and leaves the fastest pair's;
+    - ``"yarn"``: pairs that turn more than ``fast_turns`` times over ``original_length`` keep
+      their frequency, those below ``slow_turns`` have it divided by ``factor``, with a linear
+      ramp over the pairs between; the magnitude is ``0.1 ln(factor) + 1``.
+
+    The magnitude is 1 for the others. Made once for a model and kept.
+
+    Raises:
+        ValueError: on an odd or empty ``rotary_dim``, an unknown scaling, a factor below 1, or
+            ``"yarn"`` without ``original_length``.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and positive")
+    if scaling not in _SCALINGS:
+        raise ValueError(f"scaling must be one of {', '.join(_SCALINGS)}")
+    if not base > 1.0:
+        raise ValueError("base must be greater than 1")
+    if not factor >= 1.0:
+        raise ValueError("factor must be at least 1")
+    half = rotary_dim // 2
+    if scaling == "ntk":
+        if rotary_dim <= 2:
+            raise ValueError("ntk scaling needs a rotary_dim above 2")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    index = torch.arange(half, dtype=torch.float64, device=device)
+    plain = torch.pow(torch.tensor(base, dtype=torch.float64, device=device), -index / half)
+    if scaling == "linear":
+        return plain / factor, 1.0
+    if scaling != "yarn":
+        return plain, 1.0
+    if original_length is None or original_length <= 0:
+        raise ValueError("yarn scaling needs a positive original_length")
+    if not fast_turns > slow_turns > 0:
+        raise ValueError("yarn scaling needs fast_turns > slow_turns > 0")
+
+    def pair_turning(turns: float) -> float:
+        """The (fractional) pair that makes ``turns`` turns over the original length."""
+        return half * math.log(original_length / (turns * 2 * math.pi)) / math.log(base)
+
+    low = max(math.floor(pair_turning(fast_turns)), 0)
+    high = min(math.ceil(pair_turning(slow_turns)), half - 1)
+    ramp = ((index - low) / max(high - low, 1e-3)).clamp(0, 1)
+    return plain * (1 - ramp) + plain / factor * ramp, 0.1 * math.log(factor) + 1.0
+
+
+def rotary_embedding(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    magnitude: float = 1.0,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Turn ``q`` (and ``k``) by their tokens' positions.
+
+    Args:
+        q, k: ``[batch, heads, tokens, head_dim]``, or packed ``[tokens, heads, head_dim]``;
+            float16, bfloat16 or float32, any strides with a contiguous last dimension, head
+            counts of their own. ``k`` may be ``None``. head_dim at most 1024.
+        positions: int32 or int64, ``[batch, tokens]`` or ``[tokens]`` (shared by the batch);
+            ``[tokens]`` for packed tensors. Any value, negative ones included.
+        frequencies: float64 ``[rotary_dim // 2]`` on the same device
+            (:func:`rotary_frequencies`); features past ``rotary_dim`` are copied.
+        interleaved: pairs are ``(2i, 2i + 1)``; otherwise ``(i, i + rotary_dim // 2)``.
+        magnitude: multiplies cosine and sine (rounded to float32).
+
+    Returns:
+        The turned ``q``, or ``(q, k)``, with the inputs' shape and memory order. Angles are
+        float64, the rotation float32, rounded once to the dtype. Differentiable in ``q`` and
+        ``k``.
+
+    Raises:
+        ValueError: on an unsupported shape, dtype, layout or device.
+    """
+    _validate(q, k, positions, frequencies)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _RotaryFunction.apply(q, k, positions, frequencies, interleaved, float(magnitude))
+        return out if k is not None else out[0]
+    turned_q, turned_k = _launch(q, k, positions, frequencies, interleaved, float(magnitude))
+    return turned_q if k is None else (turned_q, turned_k)
+
+
+class _RotaryFunction(torch.autograd.Function):
+    """Autograd bridge: the gradient is the inverse rotation with the same magnitude."""
+
+    @staticmethod
+    def forward(ctx: Any, q, k, positions, frequencies, interleaved, magnitude):
+        """Turn and keep the positions and frequencies."""
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = (interleaved, magnitude)
+        return _launch(q, k, positions, frequencies, interleaved, magnitude)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, dq, dk):
+        """Gradients of the tensors that were given one and need one."""
+        positions, frequencies = ctx.saved_tensors
+        wanted = [g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad)]
+        given = [_unit_stride(g) for g in wanted if g is not None]
+        if not given:
+            return (None,) * 6
+        first, second = given[0], given[1] if len(given) == 2 else None
+        turned = list(_launch(first, second, positions, frequencies, *ctx.how, inverse=True))
+        grads = [None if g is None else turned.pop(0) for g in wanted]
+        return (*grads, None, None, None, None)
+
+
+def _unit_stride(grad: torch.Tensor) -> torch.Tensor:
+    """The gradient with a contiguous last dimension (a broadcast one has stride 0)."""
+    return grad if grad.stride(-1) == 1 else grad.contiguous()
+
+
+def _launch(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+    interleaved: bool,
+    magnitude: float,
+    *,
+    inverse: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Allocate the outputs and enqueue the rotation of tensors already checked."""
+    q_out = _output(q)
+    k_out = None if k is None else _output(k)
+    packed = q.ndim == 3
+    tokens = q.shape[0] if packed else q.shape[2]
+    position_strides = positions.stride() if positions.ndim == 2 else (0, positions.stride(0))
+    _hip.call_on(
+        q,
+        "tk_rotary",
+        _hip.dtype_code(q.dtype),
+        q.data_ptr(),
+        q_out.data_ptr(),
+        _hip.ptr(k),
+        _hip.ptr(k_out),
+        positions.data_ptr(),
+        frequencies.data_ptr(),
+        1 if packed else q.shape[0],
+        tokens,
+        q.shape[1],
+        0 if k is None else k.shape[1],
+        q.shape[-1],
+        2 * frequencies.shape[0],
+        _strides(q),
+        _strides(q_out),
+        None if k is None else _strides(k),
+        None if k_out is None else _strides(k_out),
+        _hip.int64_array(position_strides),
+        magnitude,
+        int(interleaved),
+        int(positions.dtype == torch.int64),
+        int(inverse),
+        _hip.stream_of(q),
+    )
+    return q_out, k_out
+
+
+def _output(x: torch.Tensor) -> torch.Tensor:
+    """A tensor like ``x`` in its memory order, rows unit-stride and no element shared."""
+    out = torch.empty_like(x, requires_grad=False)
+    if out.stride(-1) != 1:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return out
+
+
+def _strides(x: torch.Tensor) -> Any:
+    """``{batch, head, token}`` strides."""
+    s = x.stride()
+    return _hip.int64_array((0, s[1], s[0]) if x.ndim == 3 else s[:3])
+
+
+def _validate(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+) -> None:
+    """Check the rotation's contract."""
+    if q.ndim not in (3, 4):
+        raise ValueError("rotary_embedding expects q [batch, heads, tokens, head_dim] or packed "
+                         "[tokens, heads, head_dim]")
+    if q.numel() == 0:
+        raise ValueError("rotary_embedding does not support empty dimensions")
+    if k is not None:
+        if k.ndim != q.ndim:
+            raise ValueError("q and k must both be packed or both be batched")
+        if k.numel() == 0:
+            raise ValueError("rotary_embedding does not support empty dimensions")
+        other = [d for d in range(q.ndim) if d != 1]
+        if any(k.shape[d] != q.shape[d] for d in other):
+            raise ValueError("q and k may differ only in their head counts")
+        if k.dtype != q.dtype or k.device != q.device:
+            raise ValueError("q and k must share a dtype and a device")
+    if q.dtype not in _DTYPES:
+        raise ValueError("rotary_embedding supports float16, bfloat16 and float32 tensors")
+    tokens = q.shape[0] if q.ndim == 3 else q.shape[2]
+    shapes = [(tokens,)] if q.ndim == 3 else [(tokens,), (q.shape[0], tokens)]
+    if tuple(positions.shape) not in shapes:
+        raise ValueError("positions must be [tokens]" + (" or [batch, tokens]" * (q.ndim == 4)))
+    if positions.dtype not in _POSITION_DTYPES:
+        raise ValueError("positions must be int32 or int64")
+    if frequencies.ndim != 1 or frequencies.dtype != torch.float64:
+        raise ValueError("frequencies must be a float64 [rotary_dim // 2] tensor")
+    if frequencies.numel() == 0 or 2 * frequencies.numel() > q.shape[-1]:
+        raise ValueError("frequencies must cover at least one pair and at most head_dim features")
+    if frequencies.stride(0) != 1:
+        raise ValueError("frequencies must be contiguous")
+    if q.shape[-1] > _MAX_HEAD_DIM:
+        raise ValueError(f"rotary_embedding supports head_dim up to {_MAX_HEAD_DIM}")
+    if q.device.type != "cuda":
+        raise ValueError("rotary_embedding requires CUDA (ROCm/HIP) tensors")
+    if positions.device != q.device or frequencies.device != q.device:
+        raise ValueError("q, positions and frequencies must be on one device")
+    for name, tensor in (("q", q), ("k", k)):
+        if tensor is not None and tensor.stride(-1) != 1:
+            raise ValueError(f"{name} requires a contiguous final dimension")
