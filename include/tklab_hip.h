@@ -424,6 +424,39 @@ int tk_rotary(int dtype, const void* q, void* q_out, const void* k, void* k_out,
               const int64_t* k_out_strides, const int64_t* position_strides, float magnitude,
               int interleaved, int wide_positions, int inverse, void* stream);
 
+/* Verification of drafted tokens. Per sequence, `nodes` <= 256 nodes, node 0 the last token;
+ * target[b][i] (strides {batch, node}, unit-stride entries) is the target's distribution behind
+ * node i, tokens[b][i] node i's token (int64 with `wide_tokens`, else int32), parents[b][i] its
+ * parent (NULL: i - 1), uniforms[b][i] its random number; node_strides are the batch strides of
+ * tokens, parents and uniforms. From node 0 on, the current node's children are tried in order:
+ * child i with token x becomes the current node if u_i q(x) < p(x) with `draft` (row i - 1 is
+ * what node i was drawn from; not with parents), else if u_i (1 - rejected siblings' p) < p(x).
+ * The next token is drawn with u_0 from max(p - q, 0) after a rejection with `draft`, else from
+ * p without the rejected tokens (p itself where that has no mass, -1 where p has none): the first
+ * v with cumulative weight > u_0 * total, in float64. path int32[batch][nodes] gets the accepted
+ * nodes, then -1; count int32[batch]; next_token int64[batch]. A node whose parent is not in
+ * [0, i) or whose token is not in [0, vocabulary) is skipped. `chunk`, a multiple of 8 giving
+ * splits = ceil(vocabulary / chunk) <= 64, is a workgroup's share of a row; `workspace` holds
+ * batch * (16 * splits + 4 * (4 + nodes)) bytes, 8-byte aligned, overwritten. Two launches. */
+int tk_verify_draft(int dtype, const void* target, const void* draft, const void* tokens,
+                    const int32_t* parents, const float* uniforms, int32_t* path, int32_t* count,
+                    int64_t* next_token, void* workspace, int64_t batch, int64_t nodes,
+                    int64_t vocabulary, int64_t chunk, const int64_t* target_strides,
+                    const int64_t* draft_strides, const int64_t* node_strides, int wide_tokens,
+                    void* stream);
+
+/* Append accepted nodes to the caches: row seqlens[b] + i of every KV head takes row path[b][i]
+ * of the tree, i < count[b] (rows past max_len and path entries outside [0, nodes) are not
+ * written); new_seqlens[b] = min(seqlens[b] + count[b], max_len), seqlens and count clamped to
+ * [0, max_len] and [0, nodes]. Strides {batch, head, position}, multiples of 8 elements, bases
+ * 16-byte aligned; dtype F16 or BF16, head_dim a multiple of 8; path is contiguous. */
+int tk_commit_draft(int dtype, void* k_cache, void* v_cache, const void* k_tree,
+                    const void* v_tree, const int32_t* seqlens, const int32_t* path,
+                    const int32_t* count, int32_t* new_seqlens, int64_t batch, int64_t kv_heads,
+                    int64_t max_len, int64_t nodes, int64_t head_dim,
+                    const int64_t* k_cache_strides, const int64_t* v_cache_strides,
+                    const int64_t* k_tree_strides, const int64_t* v_tree_strides, void* stream);
+
 /* ---- Calibration kernels (no counterpart in the reference). They measure the
  * roofs this GPU sustains, so that the kernels above can be priced against
  * measured ceilings beside the published peaks. */
