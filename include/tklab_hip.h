@@ -424,6 +424,30 @@ int tk_rotary(int dtype, const void* q, void* q_out, const void* k, void* k_out,
               const int64_t* k_out_strides, const int64_t* position_strides, float magnitude,
               int interleaved, int wide_positions, int inverse, void* stream);
 
+/* Attention of drafted tokens over a KV cache and each other: query row (b, h, t) sees the first
+ * clamp(seqlens[b], 0, max_len) cache keys of KV head h / (q_heads / kv_heads) (all max_len when
+ * `seqlens` is NULL) and the drafted keys j < nodes with mask[b][t][j] != 0 (bytes; strides
+ * {batch, row}, unit-stride entries). o in the storage dtype, lse float32 [batch][q_heads][nodes],
+ * base 2; a row that sees nothing gets 0 and -inf. A key that a row does not see does not reach
+ * it, infinities and NaN included. Strides {batch, head, position} in elements, multiples of 8,
+ * key strides below 2^24, bases 16-byte aligned; dtype F16 or BF16, head_dim 64 or 128, nodes <=
+ * 256. `workspace`: tk_tree_decode_slots(...) * nodes * (q_heads / kv_heads) * (head_dim + 2)
+ * floats, 16-byte aligned, overwritten (NULL when that is 0). At most two launches. The workload
+ * and head mapping are tk_gqa_decode's with several query tokens per sequence. */
+int tk_tree_decode(int dtype, const void* q, const void* k_cache, const void* v_cache,
+                   const void* k_tree, const void* v_tree, const void* mask,
+                   const int32_t* seqlens, void* o, float* lse, float* workspace, int64_t batch,
+                   int64_t q_heads, int64_t kv_heads, int64_t max_len, int64_t nodes,
+                   int64_t head_dim, const int64_t* q_strides, const int64_t* k_strides,
+                   const int64_t* v_strides, const int64_t* k_tree_strides,
+                   const int64_t* v_tree_strides, const int64_t* mask_strides,
+                   const int64_t* o_strides, float scale, void* stream);
+
+/* Partial results that tk_tree_decode keeps per query row of a KV head for these sizes (group =
+ * q_heads / kv_heads); -1 for sizes it does not take. No launch, no GPU. */
+int tk_tree_decode_slots(int64_t batch, int64_t kv_heads, int64_t group, int64_t max_len,
+                         int64_t nodes);
+
 /* Verification of drafted tokens. Per sequence, `nodes` <= 256 nodes, node 0 the last token;
  * target[b][i] (strides {batch, node}, unit-stride entries) is the target's distribution behind
  * node i, tokens[b][i] node i's token (int64 with `wide_tokens`, else int32), parents[b][i] its

@@ -1,0 +1,748 @@
+// Attention of drafted tokens over a KV cache and over each other: sequence b has `nodes` query
+// tokens, each of which sees the first clamp(seqlens[b], 0, max_len) cache keys and the drafted
+// keys that its row of the mask names. Query head h reads KV head h / (q_heads / kv_heads).
+//
+// The nodes x group query rows of one KV head form one matrix (row r = node r / group, head
+// r % group), so each key is read once for all of them. Split kernel: a workgroup of W waves
+// takes 16 W MT rows (MT row tiles per wave) over a run of 32-key tiles; the drafted keys are
+// the tiles behind the context's. Both products run on v_mfma_f32_16x16x32 with the keys as the
+// first operand's rows, as in the one-token decode:
+//   S^T (16 keys x 16 rows) = K . Q^T, Q^T in registers; a row's maximum and sum are over a
+//     lane's values and lanes ^ 16, ^ 32.
+//   O^T (16 dims x 16 rows) += V^T . P^T, P^T from the score registers, V^T by transposing LDS
+//     reads.
+// K and V tiles reach LDS by non-temporal buffer->LDS DMA into one ring per workgroup (each wave
+// fetches its share; one barrier per tile), so LDS holds a key once for all waves. Rows outside
+// the context or the tree lie outside the tile's buffer range and arrive as zeros.
+//
+// Softmax statistics and sums are float32, P is rounded to the storage dtype for the second
+// product (as in every attention of this library), O once at the end.
+//
+// Masked keys must not reach a row by way of 0 * inf or 0 * NaN in the second product. Past the
+// context's end V is zero; a drafted tile's V is checked, and if it holds an infinity or a NaN
+// the tile is added key by key, and only to the rows that see the key.
+//
+// Splits: the tiles of all sequences are shared out in equal runs of `chunk` tiles, found by
+// every workgroup from the lengths (which only the device knows), so a ragged batch fills the
+// chip evenly whatever max_len is. A sequence that is one run is normalized and written by its
+// workgroup; longer ones are joined by the combine kernel in a fixed order.
+#include "attention_dma.hpp"
+#include "tk_common.hpp"
+
+namespace {
+
+using tk_attn::f32x4;
+using tk_attn::i32x2;
+using tk_attn::i32x4;
+
+constexpr int kTileKeys = 32;
+constexpr int kMaxNodes = 256;
+constexpr int kMaskWords = kMaxNodes / 32;
+constexpr int kNonTemporal = 2;
+constexpr float kLog2e = 1.4426950408889634f;
+// The running maximum before any key: finite, so that a masked score (-inf) minus it stays
+// -inf, and below every score that carries weight.
+constexpr float kNoMax = -3.0e38f;
+
+struct TreeArgs {
+  const void *q, *k, *v, *k_tree, *v_tree;
+  const uint8_t* mask;
+  const int32_t* seqlens;
+  void* o;
+  float* lse;
+  float* part_o;   // [slot][row][D], slot = (flat split, KV head)
+  float2* part_ml; // [slot][row]
+  int64_t qb, qh, qt, ob, oh, ot;
+  int64_t kb, kh, kl, vb, vh, vl;
+  int64_t ktb, kth, ktl, vtb, vth, vtl;
+  int64_t mb, mt;
+  int batch, q_heads, kv_heads, group, nodes, rows, max_len;
+  int tree_tiles, min_chunk, runs, row_blocks, flat;  // flat: upper bound on the flat splits
+  float scale_log2;
+};
+
+// ---- Runs of tiles
+
+// 32-key tiles of sequence b: the context's and the tree's.
+__device__ __forceinline__ int context_length(const TreeArgs& a, int b) {
+  const int n = a.seqlens != nullptr ? a.seqlens[b] : a.max_len;
+  return min(max(n, 0), a.max_len);
+}
+
+// Sum over lane and prefix of it, by one wave.
+__device__ __forceinline__ int wave_prefix(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(v, d);
+    if (lane >= d) v += up;
+  }
+  return v;
+}
+
+struct Lengths {
+  int first;  // this lane's sequence's length (sequence = lane)
+  int chunk;  // tiles per run
+};
+
+__device__ __forceinline__ int tiles_of(const TreeArgs& a, int length) {
+  return (length + kTileKeys - 1) / kTileKeys + a.tree_tiles;
+}
+
+__device__ __forceinline__ Lengths read_lengths(const TreeArgs& a, int lane) {
+  Lengths r;
+  r.first = lane < a.batch ? context_length(a, lane) : 0;
+  int sum = lane < a.batch ? tiles_of(a, r.first) : 0;
+  for (int b = lane + 64; b < a.batch; b += 64) sum += tiles_of(a, context_length(a, b));
+  const int total = __builtin_amdgcn_readlane(wave_prefix(sum, lane), 63);
+  r.chunk = max(a.min_chunk, (total + a.runs - 1) / a.runs);
+  return r;
+}
+
+struct Run {
+  int b, length, split, splits, flat0;  // flat0: the sequence's first flat split
+};
+
+// Sequence and split of flat split f (all wave-uniform); false past the last.
+__device__ __forceinline__ bool find_run(const TreeArgs& a, const Lengths& n, int f, int lane,
+                                         Run& out) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    const int len = b0 == 0 ? n.first : (b < a.batch ? context_length(a, b) : 0);
+    const int mine = b < a.batch ? (tiles_of(a, len) + n.chunk - 1) / n.chunk : 0;
+    const int upto = before + wave_prefix(mine, lane);
+    const uint64_t hit = __ballot(upto > f);
+    if (hit != 0) {
+      const int at = __builtin_ctzll(hit);
+      out.b = b0 + at;
+      out.length = __builtin_amdgcn_readlane(len, at);
+      out.splits = __builtin_amdgcn_readlane(mine, at);
+      out.flat0 = __builtin_amdgcn_readlane(upto, at) - out.splits;
+      out.split = f - out.flat0;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// Splits and first flat split of sequence b (wave-uniform).
+__device__ __forceinline__ void sequence_runs(const TreeArgs& a, const Lengths& n, int b, int lane,
+                                              Run& out) {
+  int before = 0;
+  for (int b0 = 0; b0 <= b; b0 += 64) {
+    const int i = b0 + lane;
+    const int len = b0 == 0 ? n.first : (i < a.batch ? context_length(a, i) : 0);
+    const int mine = i < a.batch ? (tiles_of(a, len) + n.chunk - 1) / n.chunk : 0;
+    const int upto = before + wave_prefix(mine, lane);
+    if (b < b0 + 64) {
+      out.splits = __builtin_amdgcn_readlane(mine, b - b0);
+      out.flat0 = __builtin_amdgcn_readlane(upto, b - b0) - out.splits;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+
+// ---- LDS ring (rows stored whole, chunks swizzled, as the DMA writes contiguous LDS)
+
+template <int D>
+struct Ring {
+  static constexpr int RB = D * 2;             // bytes per row
+  static constexpr int TILE = kTileKeys * RB;  // bytes per tensor tile
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int NS = D == 128 ? 4 : 8;  // 64 KiB: two workgroups share a CU
+  static constexpr int IPT = TILE / 1024;      // DMA instructions per tensor tile
+  static constexpr int RPI = 1024 / RB;        // rows per DMA instruction
+  static constexpr int CPR = RB / 16;          // 16-byte chunks per row
+  // K: chunk c of row r at slot c ^ kswz(r): a ds_read_b128 phase (16 lanes, one chunk of 16
+  // rows) touches 16 distinct bank groups. V: 32-byte granule g of row r at g ^ vswz(r): a
+  // transposing read's phase takes one granule of 8 rows, on distinct positions.
+  static __device__ __forceinline__ int kswz(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
+  static __device__ __forceinline__ int vswz(int r) { return D == 128 ? (r & 7) : ((r >> 1) & 3); }
+};
+
+__device__ __forceinline__ void* uniform_ptr(const void* p) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(x >> 32));
+  return reinterpret_cast<void*>((uint64_t(hi) << 32) | lo);
+}
+
+// Where a run's tiles come from: context rows, then the tree's.
+template <typename T>
+struct Source {
+  const T *k, *v, *k_tree, *v_tree;
+  int64_t kl, vl, ktl, vtl;
+  int length, context_tiles, nodes, end;  // end: first tile past the run
+};
+
+// This wave's share of tile `tile` into ring stage `stage`. Tiles past the run's end (issued to
+// keep the wait counts static) have no rows: nothing is read, LDS gets zeros.
+template <typename T, int D, int W>
+__device__ __forceinline__ void fetch(char* ring, const Source<T>& s, int tile, int stage, int wave,
+                                      const int* row, const int* kchunk, const int* vchunk) {
+  using R = Ring<D>;
+  constexpr int PER = R::IPT / W;
+  const bool tree = tile >= s.context_tiles;
+  const int key0 = (tree ? tile - s.context_tiles : tile) * kTileKeys;
+  int rows = min((tree ? s.nodes : s.length) - key0, kTileKeys);
+  if (tile >= s.end) rows = 0;
+  const int64_t kl = tree ? s.ktl : s.kl, vl = tree ? s.vtl : s.vl;
+  const T* kp = (tree ? s.k_tree : s.k) + (rows > 0 ? key0 * kl : 0);
+  const T* vp = (tree ? s.v_tree : s.v) + (rows > 0 ? key0 * vl : 0);
+  // The last row ends D elements in: bytes past it are outside the range.
+  const uint32_t krange = rows > 0 ? uint32_t((rows - 1) * kl + D) * 2 : 0;
+  const uint32_t vrange = rows > 0 ? uint32_t((rows - 1) * vl + D) * 2 : 0;
+  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+      uniform_ptr(kp), (short)0, __builtin_amdgcn_readfirstlane(krange), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+      uniform_ptr(vp), (short)0, __builtin_amdgcn_readfirstlane(vrange), 0x00020000);
+  const uint32_t k2 = __builtin_amdgcn_readfirstlane(uint32_t(kl * 2));
+  const uint32_t v2 = __builtin_amdgcn_readfirstlane(uint32_t(vl * 2));
+  char* dst = ring + stage * R::STAGE + wave * PER * 1024;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (tk_attn::lds_void*)(dst + i * 1024), 16,
+                                             row[i] * k2 + kchunk[i], 0, 0, kNonTemporal);
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (tk_attn::lds_void*)(dst + R::TILE + i * 1024), 16,
+                                             row[i] * v2 + vchunk[i], 0, 0, kNonTemporal);
+}
+
+template <typename T>
+__device__ __forceinline__ i32x4 pack_probabilities(const float (&p)[2][4]) {
+  return i32x4{int(tk_attn::pack2<T>(p[0][0], p[0][1])), int(tk_attn::pack2<T>(p[0][2], p[0][3])),
+               int(tk_attn::pack2<T>(p[1][0], p[1][1])), int(tk_attn::pack2<T>(p[1][2], p[1][3]))};
+}
+
+// Largest |x| bit pattern of packed 16-bit values, kept per half.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 max_magnitude(u16x2 m, int x) {
+  return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x & 0x7FFF7FFF));
+}
+
+// The elements of a fragment that belong to key j of the tile (element e of this lane is key
+// 16 (e / 4) + 4 quad + e % 4), the others zero.
+__device__ __forceinline__ i32x4 only_key(i32x4 f, int j, int quad) {
+  i32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = 16 * (i / 2) + 4 * quad + 2 * (i % 2);
+    r[i] = key == j ? (f[i] & 0xFFFF) : key + 1 == j ? int(uint32_t(f[i]) & 0xFFFF0000u) : 0;
+  }
+  return r;
+}
+
+template <typename T, int D, int W, int MT>
+__global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(TreeArgs a) {
+  using R = Ring<D>;
+  constexpr int DC = D / 32, OC = D / 16, NS = R::NS, RB = R::RB, PER = R::IPT / W;
+  constexpr int ROWS = 16 * W * MT;
+  constexpr int NONFINITE = __is_same(T, __bf16) ? 0x7F80 : 0x7C00;
+  __shared__ __attribute__((aligned(1024))) char ring[NS * R::STAGE];
+  __shared__ uint32_t seen[ROWS * kMaskWords];  // drafted keys by the block's nodes
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroup -> (flat split, KV head, row block): the row blocks of a run are dealt to one XCD
+  // (workgroup index modulo 8), one after the other, so that they share its L2.
+  const int pair = (blockIdx.x / (8 * a.row_blocks)) * 8 + blockIdx.x % 8;
+  const int rb = (blockIdx.x / 8) % a.row_blocks;
+  const int f = pair / a.kv_heads;
+  const int kvh = pair - f * a.kv_heads;
+  const Lengths lengths = read_lengths(a, lane);
+  Run run;
+  if (f >= a.flat || !find_run(a, lengths, f, lane, run)) return;
+
+  const int b = run.b;
+  Source<T> src;
+  src.k = static_cast<const T*>(a.k) + b * a.kb + kvh * a.kh;
+  src.v = static_cast<const T*>(a.v) + b * a.vb + kvh * a.vh;
+  src.k_tree = static_cast<const T*>(a.k_tree) + b * a.ktb + kvh * a.kth;
+  src.v_tree = static_cast<const T*>(a.v_tree) + b * a.vtb + kvh * a.vth;
+  src.kl = a.kl;
+  src.vl = a.vl;
+  src.ktl = a.ktl;
+  src.vtl = a.vtl;
+  src.length = run.length;
+  src.nodes = a.nodes;
+  src.context_tiles = (run.length + kTileKeys - 1) / kTileKeys;
+  const int tiles = src.context_tiles + a.tree_tiles;
+  const int t0 = run.split * lengths.chunk;
+  const int t1 = min(t0 + lengths.chunk, tiles);
+  src.end = t1;
+
+  const int row16 = lane & 15;
+  const int quad = lane >> 4;
+  const int r0 = rb * ROWS;
+  const int w0 = r0 + wave * 16 * MT;   // this wave's first row
+  const bool busy = w0 < a.rows;        // waves past the last row only fetch
+
+  // Q^T fragments: row w0 + 16 mt + row16 (zero past the last), dims 32 c + 8 quad .. +7.
+  i32x4 qf[MT][DC];
+  int node[MT];  // the lane's rows' nodes
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = w0 + 16 * m + row16;
+    node[m] = r / a.group;
+    const int h = kvh * a.group + (r - node[m] * a.group);
+    const T* p = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + node[m] * a.qt + 8 * quad;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+      qf[m][c] = r < a.rows ? *reinterpret_cast<const i32x4*>(p + 32 * c) : i32x4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int c = 0; c < DC; ++c) tk_attn::pin(qf[m][c]);
+
+  // DMA sources: instruction i of this wave's share covers rows RPI (wave PER + i) .. +RPI-1;
+  // the lane fetches the chunk that belongs at its LDS slot.
+  int drow[PER], kchunk[PER], vchunk[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = (wave * PER + i) * R::RPI + lane / R::CPR;
+    const int slot = lane % R::CPR;
+    drow[i] = r;
+    kchunk[i] = (slot ^ R::kswz(r)) * 16;
+    vchunk[i] = ((((slot >> 1) ^ R::vswz(r)) << 1) | (slot & 1)) * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    fetch<T, D, W>(ring, src, t0 + i, i, wave, drow, kchunk, vchunk);
+
+  // The block's nodes' mask rows as bits, if the run holds drafted tiles.
+  const int node0 = r0 / a.group;
+  if (t1 > src.context_tiles) {
+    const int last = min((min(r0 + ROWS, a.rows) - 1) / a.group, a.nodes - 1);
+    const uint8_t* mask = a.mask + b * a.mb;
+    for (int n = node0 + wave; n <= last; n += W)
+      for (int j0 = 0; j0 < a.nodes; j0 += 64) {
+        const int j = j0 + lane;
+        const uint64_t bits = __ballot(j < a.nodes && mask[n * a.mt + j] != 0);
+        if (lane < 2 && j0 / 32 + lane < kMaskWords)
+          seen[(n - node0) * kMaskWords + j0 / 32 + lane] = uint32_t(bits >> (32 * lane));
+      }
+  }
+
+  const uint32_t ring_base = (uint32_t)(uintptr_t)(tk_attn::lds_void*)ring;
+  uint32_t ka[DC], va[OC];
+#pragma unroll
+  for (int c = 0; c < DC; ++c) ka[c] = row16 * RB + (((4 * c + quad) ^ R::kswz(row16)) * 16);
+  {
+    const int trow = 4 * quad + (row16 >> 2);
+#pragma unroll
+    for (int c = 0; c < OC; ++c)
+      va[c] = R::TILE + trow * RB + ((c ^ R::vswz(trow)) * 32) + 8 * (row16 & 3);
+  }
+
+  f32x4 o[MT][OC];
+  float top[MT], sum[MT];  // reference maximum of row row16, this lane's share of its sum
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    top[m] = kNoMax;
+    sum[m] = 0.f;
+#pragma unroll
+    for (int c = 0; c < OC; ++c) o[m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int t = t0; t < t1; ++t) {
+    const int it = t - t0;
+    // Tile t has landed (this wave's share) once only the NS - 2 younger tiles' loads are
+    // outstanding; behind the barrier every wave's share has, and every wave has read the stage
+    // that tile t + NS - 1 takes.
+    tk_attn::wait_vmcnt<(NS - 2) * 2 * PER>();
+    if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    fetch<T, D, W>(ring, src, t + NS - 1, (it + NS - 1) % NS, wave, drow, kchunk, vchunk);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!busy) continue;
+    const uint32_t sb = ring_base + (it % NS) * R::STAGE;
+
+    i32x4 kc[2][DC];
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      kc[0][c] = tk_attn::lds_read_b128<0>(sb + ka[c]);
+      kc[1][c] = tk_attn::lds_read_b128<16 * RB>(sb + ka[c]);
+    }
+    tk_attn::wait_lgkm<0>();
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      tk_attn::pin(kc[0][c]);
+      tk_attn::pin(kc[1][c]);
+    }
+    // sc[m][i][r]: row row16 of tile m, key 16 i + 4 quad + r.
+    float sc[MT][2][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < DC; ++c) acc = tk_attn::Mma16<T>::run(kc[i][c], qf[m][c], acc);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[m][i][r] = acc[r] * a.scale_log2;
+      }
+    // V^T fragments, read while the softmax runs, in batches of four output chunks (8 reads:
+    // lgkmcnt counts at most 15).
+    constexpr int HB = 4;
+    i32x2 lo[OC], hi[OC];
+    const bool drafted = t >= src.context_tiles;
+    const int live = drafted ? kTileKeys : src.length - t * kTileKeys;
+    if (drafted) {
+      const int word = t - src.context_tiles;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const bool real = w0 + 16 * m + row16 < a.rows;
+        const uint32_t bits = real ? seen[(node[m] - node0) * kMaskWords + word] >> (4 * quad) : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!((bits >> (16 * i + r)) & 1)) sc[m][i][r] = -INFINITY;
+      }
+    } else if (live < kTileKeys) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * i + 4 * quad + r >= live) sc[m][i][r] = -INFINITY;
+    }
+#pragma unroll
+    for (int c = 0; c < HB; ++c) {
+      lo[c] = tk_attn::lds_read_tr16<0>(sb + va[c]);
+      hi[c] = tk_attn::lds_read_tr16<16 * RB>(sb + va[c]);
+    }
+    // Lazy rescale: the reference maximum moves only when the tile's exceeds it by more than 8
+    // (base 2), so p <= 2^8 and o and sum are rescaled in few tiles.
+    i32x4 pf[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float high = sc[m][0][0];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) high = fmaxf(high, sc[m][i][r]);
+      high = tk_attn::max_over_column(high);
+      const bool grow = high > top[m] + 8.f;
+      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+        const float next = grow ? high : top[m];
+        float alpha = __builtin_amdgcn_exp2f(top[m] - next);
+        asm volatile("" : "+v"(alpha));  // keeps the multiplies inside the branch
+        top[m] = next;
+        sum[m] *= alpha;
+#pragma unroll
+        for (int c = 0; c < OC; ++c) o[m][c] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          sc[m][i][r] = __builtin_amdgcn_exp2f(sc[m][i][r] - top[m]);
+          sum[m] += sc[m][i][r];
+        }
+      pf[m] = pack_probabilities<T>(sc[m]);
+    }
+    bool by_key = false;
+    if (drafted) {
+      u16x2 most = {0, 0};
+#pragma unroll
+      for (int c0 = 0; c0 < OC; c0 += HB) {
+        i32x4 vf[HB];
+#pragma unroll
+        for (int c = 0; c < HB; ++c) vf[c] = tk_attn::read_v16<0, RB>(sb + va[c0 + c]);
+        tk_attn::wait_lgkm<0>();
+#pragma unroll
+        for (int c = 0; c < HB; ++c) {
+          tk_attn::pin(vf[c]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most = max_magnitude(most, vf[c][i]);
+        }
+      }
+      by_key = __ballot(most[0] >= NONFINITE || most[1] >= NONFINITE) != 0;
+    }
+    if (by_key) {
+      const int word = t - src.context_tiles;
+      for (int c0 = 0; c0 < OC; ++c0) {
+        // Selects a register by a loop index through unrolled comparisons.
+        i32x4 vf = tk_attn::read_v16<0, RB>(sb + R::TILE + (4 * quad + (row16 >> 2)) * RB +
+                                            ((c0 ^ R::vswz(4 * quad + (row16 >> 2))) * 32) +
+                                            8 * (row16 & 3));
+        tk_attn::wait_lgkm<0>();
+        tk_attn::pin(vf);
+        for (int j = 0; j < kTileKeys; ++j) {
+          const i32x4 vj = only_key(vf, j, quad);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const f32x4 one = tk_attn::Mma16<T>::run(vj, only_key(pf[m], j, quad),
+                                                     f32x4{0.f, 0.f, 0.f, 0.f});
+            const bool real = w0 + 16 * m + row16 < a.rows;
+            const bool sees =
+                real && ((seen[(node[m] - node0) * kMaskWords + word] >> j) & 1) != 0;
+#pragma unroll
+            for (int c = 0; c < OC; ++c)
+              if (c == c0 && sees) o[m][c] += one;
+          }
+        }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int c0 = 0; c0 < OC; c0 += HB) {
+      tk_attn::wait_lgkm<0>();
+#pragma unroll
+      for (int c = c0; c < c0 + HB; ++c) asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
+      if (c0 + HB < OC) {
+#pragma unroll
+        for (int c = c0 + HB; c < c0 + 2 * HB; ++c) {
+          lo[c] = tk_attn::lds_read_tr16<0>(sb + va[c]);
+          hi[c] = tk_attn::lds_read_tr16<16 * RB>(sb + va[c]);
+        }
+      }
+#pragma unroll
+      for (int c = c0; c < c0 + HB; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          o[m][c] = tk_attn::Mma16<T>::run(i32x4{lo[c][0], lo[c][1], hi[c][0], hi[c][1]}, pf[m],
+                                           o[m][c]);
+    }
+  }
+  // The tiles issued past the end still write (zeros) into the ring.
+  tk_attn::wait_vmcnt<0>();
+  if (!busy) return;
+
+  const int slot = f * a.kv_heads + kvh;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const float l = tk_attn::sum_over_column(sum[m]);
+    const int r = w0 + 16 * m + row16;
+    if (r >= a.rows) continue;
+    if (run.splits == 1) {
+      const int h = kvh * a.group + (r - node[m] * a.group);
+      T* dst = static_cast<T*>(a.o) + b * a.ob + h * a.oh + node[m] * a.ot + 4 * quad;
+#pragma unroll
+      for (int c = 0; c < OC; ++c) {
+        float out[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = l == 0.f ? 0.f : o[m][c][i] / l;
+        tk::store_vec<T, 4>(dst + 16 * c, out);
+      }
+      if (quad == 0)
+        a.lse[(int64_t(b) * a.q_heads + h) * a.nodes + node[m]] =
+            l == 0.f ? -INFINITY : top[m] + log2f(l);
+    } else {
+      const int64_t at = int64_t(slot) * a.rows + r;
+#pragma unroll
+      for (int c = 0; c < OC; ++c)
+        *reinterpret_cast<f32x4*>(a.part_o + at * D + 16 * c + 4 * quad) = o[m][c];
+      if (quad == 0) a.part_ml[at] = float2{top[m], l};
+    }
+  }
+}
+
+// One wave per (sequence, KV head, row): L = D / 4 lanes hold a row of O as float4, 64 / L splits
+// at a time, folded in a fixed order.
+constexpr int kCombineWaves = 4;
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kCombineWaves) void tree_combine_kernel(TreeArgs a) {
+  constexpr int L = D / 4, S = 64 / L;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = blockIdx.x * kCombineWaves + wave;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const Lengths lengths = read_lengths(a, lane);
+  Run run;
+  sequence_runs(a, lengths, b, lane, run);
+  if (run.splits == 1 || r >= a.rows) return;
+  const int64_t step = int64_t(a.kv_heads) * a.rows;  // rows between a row's splits
+  const int64_t at0 = (int64_t(run.flat0) * a.kv_heads + kvh) * a.rows + r;
+  float high = kNoMax;
+  for (int i = lane; i < run.splits; i += 64) high = fmaxf(high, a.part_ml[at0 + i * step].x);
+  high = tk::wave_allreduce(high, tk::MaxOp{});
+  float total = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int part = lane / L, d = (lane % L) * 4;
+#pragma unroll 4
+  for (int i = part; i < run.splits; i += S) {
+    const float2 ml = a.part_ml[at0 + i * step];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + (at0 + i * step) * D + d);
+    const float w = __builtin_amdgcn_exp2f(ml.x - high);
+    total += ml.y * w;
+    acc += v * w;
+  }
+#pragma unroll
+  for (int x = L; x < 64; x <<= 1) {
+    total += __shfl_xor(total, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], x);
+  }
+  if (part != 0) return;
+  const int node = r / a.group;
+  const int h = kvh * a.group + (r - node * a.group);
+  float out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = total == 0.f ? 0.f : acc[i] / total;
+  tk::store_vec<T, 4>(static_cast<T*>(a.o) + b * a.ob + h * a.oh + node * a.ot + d, out);
+  if (lane == 0)
+    a.lse[(int64_t(b) * a.q_heads + h) * a.nodes + node] =
+        total == 0.f ? -INFINITY : high + log2f(total);
+}
+
+// Rows per workgroup by the rows a KV head has: as few waves as hold them (each key tile costs
+// every wave its LDS reads), 256 at most.
+int rows_per_block(int64_t rows) {
+  for (int n : {16, 32, 64, 128})
+    if (rows <= n) return n;
+  return 256;
+}
+
+template <typename T, int D>
+void launch(const TreeArgs& a, bool combine, hipStream_t s) {
+  const int64_t pairs = tk::cdiv(int64_t(a.flat) * a.kv_heads, 8) * 8;
+  const dim3 grid(static_cast<uint32_t>(pairs * a.row_blocks));
+  switch (rows_per_block(a.rows)) {
+    case 16: hipLaunchKernelGGL((tree_split_kernel<T, D, 1, 1>), grid, dim3(64), 0, s, a); break;
+    case 32: hipLaunchKernelGGL((tree_split_kernel<T, D, 2, 1>), grid, dim3(128), 0, s, a); break;
+    case 64: hipLaunchKernelGGL((tree_split_kernel<T, D, 4, 1>), grid, dim3(256), 0, s, a); break;
+    case 128: hipLaunchKernelGGL((tree_split_kernel<T, D, 4, 2>), grid, dim3(256), 0, s, a); break;
+    default:
+      if constexpr (D == 128)
+        hipLaunchKernelGGL((tree_split_kernel<T, D, 8, 2>), grid, dim3(512), 0, s, a);
+      else
+        hipLaunchKernelGGL((tree_split_kernel<T, D, 4, 4>), grid, dim3(256), 0, s, a);
+  }
+  if (combine)
+    hipLaunchKernelGGL((tree_combine_kernel<T, D>),
+                       dim3(static_cast<uint32_t>(tk::cdiv(a.rows, kCombineWaves)), a.kv_heads,
+                            a.batch),
+                       dim3(64 * kCombineWaves), 0, s, a);
+}
+
+// Workgroups that run at once: two per CU (a 64 KiB ring each).
+constexpr int kResident = 512;
+constexpr int kMinChunk = 4;  // tiles
+
+// How the call is cut: runs (the tiles of all sequences over `runs` give the run length), the
+// bound on their number, row blocks. The sequences' last runs are shorter, so `runs` leaves room
+// for one more per sequence where that keeps the launch to one round of workgroups.
+struct Plan {
+  int64_t row_blocks, runs, flat;
+  bool combine;
+};
+Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, int64_t nodes) {
+  Plan p;
+  p.row_blocks = tk::cdiv(rows, rows_per_block(rows));
+  const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
+  const int64_t base = kResident / (kv_heads * p.row_blocks);
+  p.runs = base > 2 * batch ? base - batch : base > 1 ? base : 1;
+  p.combine = most > kMinChunk;
+  p.flat = p.runs + batch;
+  const int64_t bound = batch * tk::cdiv(most, kMinChunk);
+  if (p.flat > bound) p.flat = bound;
+  return p;
+}
+
+}  // namespace
+
+extern "C" int tk_tree_decode_slots(int64_t batch, int64_t kv_heads, int64_t group,
+                                    int64_t max_len, int64_t nodes) {
+  if (batch <= 0 || kv_heads <= 0 || group <= 0 || max_len <= 0 || nodes <= 0) return -1;
+  const Plan p = make_plan(batch, kv_heads, nodes * group, max_len, nodes);
+  if (!p.combine) return 0;
+  const int64_t slots = p.flat * kv_heads;
+  return slots > INT32_MAX ? -1 : static_cast<int>(slots);
+}
+
+extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, const void* v_cache,
+                              const void* k_tree, const void* v_tree, const void* mask,
+                              const int32_t* seqlens, void* o, float* lse, float* workspace,
+                              int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t max_len,
+                              int64_t nodes, int64_t head_dim, const int64_t* q_strides,
+                              const int64_t* k_strides, const int64_t* v_strides,
+                              const int64_t* k_tree_strides, const int64_t* v_tree_strides,
+                              const int64_t* mask_strides, const int64_t* o_strides, float scale,
+                              void* stream) {
+  if (dtype != TK_DTYPE_F16 && dtype != TK_DTYPE_BF16)
+    return tk::fail("tree decode: dtype must be float16 or bfloat16");
+  if (q == nullptr || k_cache == nullptr || v_cache == nullptr || k_tree == nullptr ||
+      v_tree == nullptr || mask == nullptr || o == nullptr || lse == nullptr ||
+      q_strides == nullptr || k_strides == nullptr || v_strides == nullptr ||
+      k_tree_strides == nullptr || v_tree_strides == nullptr || mask_strides == nullptr ||
+      o_strides == nullptr)
+    return tk::fail("tree decode: null pointer");
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_len <= 0 || nodes <= 0)
+    return tk::fail("tree decode: empty problem");
+  if (head_dim != 64 && head_dim != 128) return tk::fail("tree decode: head_dim must be 64 or 128");
+  if (q_heads % kv_heads != 0) return tk::fail("tree decode: q_heads must be a multiple of kv_heads");
+  if (nodes > kMaxNodes) return tk::fail("tree decode: at most %d nodes", kMaxNodes);
+  if (batch > 65535 || q_heads > 65535 || max_len > INT32_MAX - 65536)
+    return tk::fail("tree decode: problem too large");
+  const int64_t group = q_heads / kv_heads, rows = nodes * group;
+  const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
+  const Plan plan = make_plan(batch, kv_heads, rows, max_len, nodes);
+  if (batch * most > INT32_MAX / 2 || plan.flat * kv_heads * plan.row_blocks > (1 << 22))
+    return tk::fail("tree decode: problem too large");
+  if (plan.combine && workspace == nullptr) return tk::fail("tree decode: null pointer");
+  for (const void* p : {q, k_cache, v_cache, k_tree, v_tree, static_cast<const void*>(o),
+                        static_cast<const void*>(workspace)})
+    if (!tk::aligned16(p)) return tk::fail("tree decode: tensors must be 16-byte aligned");
+  for (const int64_t* st : {q_strides, k_strides, v_strides, k_tree_strides, v_tree_strides,
+                            o_strides})
+    for (int d = 0; d < 3; ++d)
+      if (st[d] < 0 || st[d] % 8 != 0 || st[d] >= (int64_t(1) << 40))
+        return tk::fail("tree decode: strides must be non-negative multiples of 8 elements");
+  if (mask_strides[0] < 0 || mask_strides[1] < 0 || mask_strides[0] >= (int64_t(1) << 40) ||
+      mask_strides[1] >= (int64_t(1) << 30))
+    return tk::fail("tree decode: mask strides must be non-negative and keep rows in range");
+  // The DMA addresses a tile's 32 rows through 32-bit buffer offsets.
+  for (const int64_t* st : {k_strides, v_strides, k_tree_strides, v_tree_strides})
+    if (st[2] >= (int64_t(1) << 24))
+      return tk::fail("tree decode: key strides must be below 2^24 elements");
+  TreeArgs a;
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.k_tree = k_tree;
+  a.v_tree = v_tree;
+  a.mask = static_cast<const uint8_t*>(mask);
+  a.seqlens = seqlens;
+  a.o = o;
+  a.lse = lse;
+  a.part_o = workspace;
+  a.part_ml = reinterpret_cast<float2*>(workspace + plan.flat * kv_heads * rows * head_dim);
+  a.qb = q_strides[0], a.qh = q_strides[1], a.qt = q_strides[2];
+  a.ob = o_strides[0], a.oh = o_strides[1], a.ot = o_strides[2];
+  a.kb = k_strides[0], a.kh = k_strides[1], a.kl = k_strides[2];
+  a.vb = v_strides[0], a.vh = v_strides[1], a.vl = v_strides[2];
+  a.ktb = k_tree_strides[0], a.kth = k_tree_strides[1], a.ktl = k_tree_strides[2];
+  a.vtb = v_tree_strides[0], a.vth = v_tree_strides[1], a.vtl = v_tree_strides[2];
+  a.mb = mask_strides[0], a.mt = mask_strides[1];
+  a.batch = static_cast<int>(batch);
+  a.q_heads = static_cast<int>(q_heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.group = static_cast<int>(group);
+  a.nodes = static_cast<int>(nodes);
+  a.rows = static_cast<int>(rows);
+  a.max_len = static_cast<int>(max_len);
+  a.tree_tiles = static_cast<int>(tk::cdiv(nodes, kTileKeys));
+  a.min_chunk = kMinChunk;
+  a.runs = static_cast<int>(plan.runs);
+  a.row_blocks = static_cast<int>(plan.row_blocks);
+  a.flat = static_cast<int>(plan.flat);
+  a.scale_log2 = scale * kLog2e;
+  hipStream_t s = tk::as_stream(stream);
+  if (dtype == TK_DTYPE_BF16) {
+    if (head_dim == 128)
+      launch<__bf16, 128>(a, plan.combine, s);
+    else
+      launch<__bf16, 64>(a, plan.combine, s);
+  } else {
+    if (head_dim == 128)
+      launch<_Float16, 128>(a, plan.combine, s);
+    else
+      launch<_Float16, 64>(a, plan.combine, s);
+  }
+  return tk::check_launch("tree decode");
+}

@@ -117,6 +117,7 @@ _SIGNATURES: dict[str, list[object]] = {
         _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
         _I64P, _P,
     ],
+    "tk_tree_decode": [_I32] + [_P] * 10 + [_I64] * 6 + [_I64P] * 7 + [_F32, _P],
     "tk_roof_copy": [_P, _P, _I64, _P],
     "tk_roof_stream": [_P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _P],
     "tk_roof_mfma": [_I32, _P, _I64, _I64, _P],
@@ -126,6 +127,7 @@ _SIGNATURES: dict[str, list[object]] = {
 _QUERIES: dict[str, list[object]] = {
     "tk_gemm_tile": [_P, _P] + [_I64] * 7,
     "tk_attn_fwd_rows": [_I64, _I64, _I64, _I64, _I64, _I64, _I32],
+    "tk_tree_decode_slots": [_I64] * 5,
 }
 
 EXPORTED_SYMBOLS: tuple[str, ...] = ("tk_abi_version", "tk_last_error", *_QUERIES, *_SIGNATURES)

@@ -1,0 +1,180 @@
+"""Attention of a tree (or chain) of drafted tokens over a grouped KV cache.
+
+The target's pass of speculative decoding: where ``gqa_decode`` answers one query token per
+sequence, :func:`tree_decode` answers all of a sequence's drafted tokens at once. Every drafted
+token sees the sequence's context in the cache, and those drafted tokens that a mask names (its
+ancestors and itself, :func:`tree_mask`). The drafted tokens' keys and values are tensors of their
+own, so a rejected draft never enters the cache (``commit_draft`` appends the accepted ones).
+Head mapping and arithmetic are ``gqa_decode``'s (``docs/research/gqa_decode_model.md``,
+"Semantic GQA mapping"; ``flash_attention.py:90-117, 248-264``): scores scaled by
+``scale * log2(e)``, P rounded to the storage dtype before the PV product, base-2 LSE. Inference
+only: there is no autograd.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from tklab import _hip
+
+_DTYPES = (torch.float16, torch.bfloat16)
+_HEAD_DIMS = (64, 128)
+_MAX_NODES = 256
+
+
+def tree_mask(parents: torch.Tensor) -> torch.Tensor:
+    """The mask of a tree: node ``i`` sees its ancestors and itself.
+
+    ``parents`` is an integer ``[nodes]`` or ``[batch, nodes]`` tensor, every parent before its
+    children; a parent outside ``[0, i)`` starts a tree of its own (node 0, padding). Returns bool
+    ``[(batch,) nodes, nodes]`` on the same device. Made once per tree shape.
+    """
+    if parents.ndim not in (1, 2) or parents.numel() == 0 or parents.is_floating_point():
+        raise ValueError("parents must be an integer [nodes] or [batch, nodes] tensor")
+    nodes = parents.shape[-1]
+    index = torch.arange(nodes, device=parents.device)
+    has_parent = (parents >= 0) & (parents < index)
+    reach = (index == parents[..., None]) & has_parent[..., None] | torch.eye(
+        nodes, dtype=torch.bool, device=parents.device)
+    steps = 1  # ancestors up to `steps` generations back are reached
+    while steps < nodes:
+        reach = torch.matmul(reach.float(), reach.float()) > 0
+        steps *= 2
+    return reach
+
+
+def tree_decode(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_tree: torch.Tensor,
+    v_tree: torch.Tensor,
+    mask: torch.Tensor,
+    cache_seqlens: torch.Tensor | None = None,
+    *,
+    scale: float | None = None,
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of ``nodes`` drafted tokens per sequence over the cache and each other.
+
+    Args:
+        q: ``[batch, q_heads, nodes, head_dim]`` float16/bfloat16; at most 256 nodes.
+        k_cache, v_cache: ``[batch, kv_heads, max_len, head_dim]``, same dtype; q_heads a
+            multiple of kv_heads; head_dim 64 or 128.
+        k_tree, v_tree: ``[batch, kv_heads, nodes, head_dim]``, the drafted tokens' own.
+        mask: bool ``[nodes, nodes]`` or ``[batch, nodes, nodes]``: ``mask[i, j]`` lets node
+            ``i`` see node ``j``. A key that a node does not see cannot reach its result, whatever
+            it holds (infinities and NaN included).
+        cache_seqlens: optional int32 ``[batch]`` context lengths, clamped to ``[0, max_len]``;
+            ``None`` means every sequence has ``max_len`` keys.
+        scale: score scale, default ``1 / sqrt(head_dim)``.
+        return_lse: also return the float32 base-2 LSE ``[batch, q_heads, nodes]``.
+
+    Returns:
+        The output in ``q``'s shape and memory order; a node that sees no key at all gives zeros
+        and an LSE of ``-inf``. Any strides whose rows are unit-stride and 16-byte aligned.
+
+    Raises:
+        ValueError: on an unsupported shape, dtype, layout or device.
+    """
+    _validate(q, k_cache, v_cache, k_tree, v_tree, mask, cache_seqlens)
+    batch, q_heads, nodes, head_dim = q.shape
+    kv_heads, max_len = k_cache.shape[1], k_cache.shape[2]
+    out = torch.empty_like(q)
+    if out.stride(-1) != 1 or any(s % 8 for s in out.stride()[:3]):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((batch, q_heads, nodes), dtype=torch.float32, device=q.device)
+    group = q_heads // kv_heads
+    slots = _hip.query("tk_tree_decode_slots", batch, kv_heads, group, max_len, nodes)
+    if slots < 0:
+        raise ValueError("tree_decode: the problem is too large")
+    workspace = torch.empty(slots * nodes * group * (head_dim + 2), dtype=torch.float32,
+                            device=q.device) if slots else None
+    _hip.call_on(
+        q,
+        "tk_tree_decode",
+        _hip.dtype_code(q.dtype),
+        q.data_ptr(),
+        k_cache.data_ptr(),
+        v_cache.data_ptr(),
+        k_tree.data_ptr(),
+        v_tree.data_ptr(),
+        mask.data_ptr(),
+        _hip.ptr(cache_seqlens),
+        out.data_ptr(),
+        lse.data_ptr(),
+        _hip.ptr(workspace),
+        batch,
+        q_heads,
+        kv_heads,
+        max_len,
+        nodes,
+        head_dim,
+        _hip.int64_array(q.stride()[:3]),
+        _hip.int64_array(k_cache.stride()[:3]),
+        _hip.int64_array(v_cache.stride()[:3]),
+        _hip.int64_array(k_tree.stride()[:3]),
+        _hip.int64_array(v_tree.stride()[:3]),
+        _hip.int64_array((mask.stride(0) if mask.ndim == 3 else 0, mask.stride(-2))),
+        _hip.int64_array(out.stride()[:3]),
+        head_dim ** -0.5 if scale is None else float(scale),
+        _hip.stream_of(q),
+    )
+    return (out, lse) if return_lse else out
+
+
+def _validate(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_tree: torch.Tensor,
+    v_tree: torch.Tensor,
+    mask: torch.Tensor,
+    cache_seqlens: torch.Tensor | None,
+) -> None:
+    """Check the contract."""
+    if q.ndim != 4 or k_cache.ndim != 4 or k_tree.ndim != 4:
+        raise ValueError("tree_decode expects q [batch, q_heads, nodes, head_dim], caches [batch, "
+                         "kv_heads, max_len, head_dim] and drafted keys and values [batch, "
+                         "kv_heads, nodes, head_dim]")
+    if v_cache.shape != k_cache.shape or v_tree.shape != k_tree.shape:
+        raise ValueError("keys and values must have identical shapes")
+    batch, q_heads, nodes, head_dim = q.shape
+    kv_heads = k_cache.shape[1]
+    if k_cache.shape[0] != batch or k_cache.shape[3] != head_dim:
+        raise ValueError("q and the caches disagree on batch or head_dim")
+    if tuple(k_tree.shape) != (batch, kv_heads, nodes, head_dim):
+        raise ValueError("k_tree and v_tree must be [batch, kv_heads, nodes, head_dim]")
+    if q.numel() == 0 or k_cache.numel() == 0:
+        raise ValueError("tree_decode does not support empty dimensions")
+    if nodes > _MAX_NODES:
+        raise ValueError(f"tree_decode supports at most {_MAX_NODES} nodes")
+    if batch > 65535 or q_heads > 65535:
+        raise ValueError("tree_decode supports at most 65535 sequences and heads")
+    if q_heads % kv_heads:
+        raise ValueError("q_heads must be a multiple of kv_heads")
+    if head_dim not in _HEAD_DIMS:
+        raise ValueError("tree_decode supports head_dim 64 and 128")
+    if q.dtype not in _DTYPES or any(t.dtype != q.dtype for t in (k_cache, v_cache, k_tree, v_tree)):
+        raise ValueError("q, caches and drafted keys and values must share a float16 or bfloat16 "
+                         "dtype")
+    if mask.dtype != torch.bool or tuple(mask.shape) not in ((nodes, nodes), (batch, nodes, nodes)):
+        raise ValueError("mask must be a bool [nodes, nodes] or [batch, nodes, nodes] tensor")
+    if q.device.type != "cuda":
+        raise ValueError("tree_decode requires CUDA (ROCm/HIP) tensors")
+    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_tree", k_tree),
+                    ("v_tree", v_tree)):
+        if t.device != q.device:
+            raise ValueError(f"{name} must be on q's device")
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name} requires a contiguous final dimension")
+        if t.data_ptr() % 16 or any(s % 8 or s < 0 for s in t.stride()[:3]):
+            raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of 8)")
+        if name != "q" and t.stride(2) >= 2**24:
+            raise ValueError(f"{name} key strides must be below 2**24 elements")
+    if mask.device != q.device or (nodes > 1 and mask.stride(-1) != 1):
+        raise ValueError("mask must be on q's device with a contiguous final dimension")
+    if cache_seqlens is not None and (
+            cache_seqlens.shape != (batch,) or cache_seqlens.dtype != torch.int32
+            or cache_seqlens.device != q.device or not cache_seqlens.is_contiguous()):
+        raise ValueError("cache_seqlens must be a contiguous int32 [batch] tensor on q's device")
