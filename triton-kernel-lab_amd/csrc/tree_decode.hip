@@ -58,7 +58,8 @@ struct TreeArgs {
   int64_t mb, mt;
   int batch, q_heads, kv_heads, group, nodes, rows, max_len;
   int tree_tiles, min_chunk, runs, row_blocks, flat;  // flat: upper bound on the flat splits
-  float scale_log2;
+  float scale_log2;  // positive
+  int flip;          // Q's sign bits to turn (a negative scale)
 };
 
 // ---- Runs of tiles
@@ -168,53 +169,69 @@ __device__ __forceinline__ void* uniform_ptr(const void* p) {
   return reinterpret_cast<void*>((uint64_t(hi) << 32) | lo);
 }
 
-// Where a run's tiles come from: context rows, then the tree's.
-template <typename T>
-struct Source {
-  const T *k, *v, *k_tree, *v_tree;
-  int64_t kl, vl, ktl, vtl;
-  int length, context_tiles, nodes, end;  // end: first tile past the run
-};
-
-// This wave's share of tile `tile` into ring stage `stage`. Tiles past the run's end (issued to
-// keep the wait counts static) have no rows: nothing is read, LDS gets zeros.
+// The stream of a run's tiles into the ring: context rows, then the tree's. All fields but the
+// lane offsets are wave-uniform.
 template <typename T, int D, int W>
-__device__ __forceinline__ void fetch(char* ring, const Source<T>& s, int tile, int stage, int wave,
-                                      const int* row, const int* kchunk, const int* vchunk) {
+struct Fetcher {
   using R = Ring<D>;
-  constexpr int PER = R::IPT / W;
-  const bool tree = tile >= s.context_tiles;
-  const int key0 = (tree ? tile - s.context_tiles : tile) * kTileKeys;
-  int rows = min((tree ? s.nodes : s.length) - key0, kTileKeys);
-  if (tile >= s.end) rows = 0;
-  const int64_t kl = tree ? s.ktl : s.kl, vl = tree ? s.vtl : s.vl;
-  const T* kp = (tree ? s.k_tree : s.k) + (rows > 0 ? key0 * kl : 0);
-  const T* vp = (tree ? s.v_tree : s.v) + (rows > 0 ? key0 * vl : 0);
-  // The last row ends D elements in: bytes past it are outside the range.
-  const uint32_t krange = rows > 0 ? uint32_t((rows - 1) * kl + D) * 2 : 0;
-  const uint32_t vrange = rows > 0 ? uint32_t((rows - 1) * vl + D) * 2 : 0;
-  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-      uniform_ptr(kp), (short)0, __builtin_amdgcn_readfirstlane(krange), 0x00020000);
-  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-      uniform_ptr(vp), (short)0, __builtin_amdgcn_readfirstlane(vrange), 0x00020000);
-  const uint32_t k2 = __builtin_amdgcn_readfirstlane(uint32_t(kl * 2));
-  const uint32_t v2 = __builtin_amdgcn_readfirstlane(uint32_t(vl * 2));
-  char* dst = ring + stage * R::STAGE + wave * PER * 1024;
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (tk_attn::lds_void*)(dst + i * 1024), 16,
-                                             row[i] * k2 + kchunk[i], 0, 0, kNonTemporal);
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (tk_attn::lds_void*)(dst + R::TILE + i * 1024), 16,
-                                             row[i] * v2 + vchunk[i], 0, 0, kNonTemporal);
-}
+  static constexpr int PER = R::IPT / W;  // this wave's instructions per tensor tile
+  const char *k, *v;        // first row of the next tile
+  const T *k_tree, *v_tree;
+  uint32_t k2, v2;          // bytes per row
+  uint32_t kt2, vt2;
+  int left;                 // rows from there to the segment's end
+  int tree_rows;            // of the tree's segment, 0 once it is the current one
+  int tiles;                // of the run, not yet issued
+  char* dst;                // this wave's share of the ring's first stage
+  uint32_t koff[PER], voff[PER];
 
-template <typename T>
-__device__ __forceinline__ i32x4 pack_probabilities(const float (&p)[2][4]) {
-  return i32x4{int(tk_attn::pack2<T>(p[0][0], p[0][1])), int(tk_attn::pack2<T>(p[0][2], p[0][3])),
-               int(tk_attn::pack2<T>(p[1][0], p[1][1])), int(tk_attn::pack2<T>(p[1][2], p[1][3]))};
-}
+  __device__ __forceinline__ void offsets(int wave, int lane) {
+    // Instruction i covers rows RPI (wave PER + i) .. +RPI-1; the lane fetches the chunk that
+    // belongs at its LDS slot.
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = (wave * PER + i) * R::RPI + lane / R::CPR;
+      const int slot = lane % R::CPR;
+      koff[i] = r * k2 + (slot ^ R::kswz(r)) * 16;
+      voff[i] = r * v2 + ((((slot >> 1) ^ R::vswz(r)) << 1) | (slot & 1)) * 16;
+    }
+  }
+
+  // The next tile into `stage`. Past the run's end (issued to keep the wait counts static) the
+  // range is empty: nothing is read, LDS gets zeros.
+  __device__ __forceinline__ void next(int stage, int wave, int lane) {
+    if (left <= 0 && tree_rows > 0) {
+      k = reinterpret_cast<const char*>(k_tree);
+      v = reinterpret_cast<const char*>(v_tree);
+      k2 = kt2;
+      v2 = vt2;
+      left = tree_rows;
+      tree_rows = 0;
+      offsets(wave, lane);
+    }
+    const int rows = tiles > 0 ? min(left, kTileKeys) : 0;
+    // The last row ends D elements in: bytes past it are outside the range.
+    const uint32_t krange = rows > 0 ? uint32_t(rows - 1) * k2 + D * 2 : 0;
+    const uint32_t vrange = rows > 0 ? uint32_t(rows - 1) * v2 + D * 2 : 0;
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+        uniform_ptr(k), (short)0, __builtin_amdgcn_readfirstlane(krange), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+        uniform_ptr(v), (short)0, __builtin_amdgcn_readfirstlane(vrange), 0x00020000);
+    char* to = dst + stage * R::STAGE;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (tk_attn::lds_void*)(to + i * 1024), 16, koff[i],
+                                               0, 0, kNonTemporal);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (tk_attn::lds_void*)(to + R::TILE + i * 1024),
+                                               16, voff[i], 0, 0, kNonTemporal);
+    k += kTileKeys * int64_t(k2);
+    v += kTileKeys * int64_t(v2);
+    left -= kTileKeys;
+    --tiles;
+  }
+};
 
 // Largest |x| bit pattern of packed 16-bit values, kept per half.
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -239,6 +256,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   using R = Ring<D>;
   constexpr int DC = D / 32, OC = D / 16, NS = R::NS, RB = R::RB, PER = R::IPT / W;
   constexpr int ROWS = 16 * W * MT;
+  constexpr int HB = 4;  // output chunks per batch of V reads
   constexpr int NONFINITE = __is_same(T, __bf16) ? 0x7F80 : 0x7C00;
   __shared__ __attribute__((aligned(1024))) char ring[NS * R::STAGE];
   __shared__ uint32_t seen[ROWS * kMaskWords];  // drafted keys by the block's nodes
@@ -256,38 +274,28 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   if (f >= a.flat || !find_run(a, lengths, f, lane, run)) return;
 
   const int b = run.b;
-  Source<T> src;
-  src.k = static_cast<const T*>(a.k) + b * a.kb + kvh * a.kh;
-  src.v = static_cast<const T*>(a.v) + b * a.vb + kvh * a.vh;
-  src.k_tree = static_cast<const T*>(a.k_tree) + b * a.ktb + kvh * a.kth;
-  src.v_tree = static_cast<const T*>(a.v_tree) + b * a.vtb + kvh * a.vth;
-  src.kl = a.kl;
-  src.vl = a.vl;
-  src.ktl = a.ktl;
-  src.vtl = a.vtl;
-  src.length = run.length;
-  src.nodes = a.nodes;
-  src.context_tiles = (run.length + kTileKeys - 1) / kTileKeys;
-  const int tiles = src.context_tiles + a.tree_tiles;
+  const int context_tiles = (run.length + kTileKeys - 1) / kTileKeys;
   const int t0 = run.split * lengths.chunk;
-  const int t1 = min(t0 + lengths.chunk, tiles);
-  src.end = t1;
+  const int t1 = min(t0 + lengths.chunk, context_tiles + a.tree_tiles);
+  const int c1 = min(t1, context_tiles);  // context tiles t0 .. c1-1, then drafted ones
 
   const int row16 = lane & 15;
   const int quad = lane >> 4;
   const int r0 = rb * ROWS;
   const int w0 = r0 + wave * 16 * MT;   // this wave's first row
   const bool busy = w0 < a.rows;        // waves past the last row only fetch
+  const int node0 = r0 / a.group;
 
-  // Q^T fragments: row w0 + 16 mt + row16 (zero past the last), dims 32 c + 8 quad .. +7.
+  // Q^T fragments: row w0 + 16 mt + row16 (zero past the last), dims 32 c + 8 quad .. +7. A
+  // negative scale is taken into Q's signs (exact), so that the largest score is the largest
+  // product.
   i32x4 qf[MT][DC];
-  int node[MT];  // the lane's rows' nodes
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int r = w0 + 16 * m + row16;
-    node[m] = r / a.group;
-    const int h = kvh * a.group + (r - node[m] * a.group);
-    const T* p = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + node[m] * a.qt + 8 * quad;
+    const int node = r / a.group;
+    const int h = kvh * a.group + (r - node * a.group);
+    const T* p = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + node * a.qt + 8 * quad;
 #pragma unroll
     for (int c = 0; c < DC; ++c)
       qf[m][c] = r < a.rows ? *reinterpret_cast<const i32x4*>(p + 32 * c) : i32x4{0, 0, 0, 0};
@@ -295,26 +303,38 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int c = 0; c < DC; ++c) tk_attn::pin(qf[m][c]);
+    for (int c = 0; c < DC; ++c) {
+      qf[m][c] ^= a.flip;
+      tk_attn::pin(qf[m][c]);
+    }
 
-  // DMA sources: instruction i of this wave's share covers rows RPI (wave PER + i) .. +RPI-1;
-  // the lane fetches the chunk that belongs at its LDS slot.
-  int drow[PER], kchunk[PER], vchunk[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int r = (wave * PER + i) * R::RPI + lane / R::CPR;
-    const int slot = lane % R::CPR;
-    drow[i] = r;
-    kchunk[i] = (slot ^ R::kswz(r)) * 16;
-    vchunk[i] = ((((slot >> 1) ^ R::vswz(r)) << 1) | (slot & 1)) * 16;
+  Fetcher<T, D, W> fetch;
+  {
+    const bool drafted = t0 >= context_tiles;
+    const int first = (drafted ? t0 - context_tiles : t0) * kTileKeys;
+    const T* kc = static_cast<const T*>(a.k) + b * a.kb + kvh * a.kh;
+    const T* vc = static_cast<const T*>(a.v) + b * a.vb + kvh * a.vh;
+    fetch.k_tree = static_cast<const T*>(a.k_tree) + b * a.ktb + kvh * a.kth;
+    fetch.v_tree = static_cast<const T*>(a.v_tree) + b * a.vtb + kvh * a.vth;
+    fetch.k = reinterpret_cast<const char*>(drafted ? fetch.k_tree + first * a.ktl
+                                                    : kc + first * a.kl);
+    fetch.v = reinterpret_cast<const char*>(drafted ? fetch.v_tree + first * a.vtl
+                                                    : vc + first * a.vl);
+    fetch.kt2 = uint32_t(a.ktl * 2);
+    fetch.vt2 = uint32_t(a.vtl * 2);
+    fetch.k2 = drafted ? fetch.kt2 : uint32_t(a.kl * 2);
+    fetch.v2 = drafted ? fetch.vt2 : uint32_t(a.vl * 2);
+    fetch.left = (drafted ? a.nodes : run.length) - first;
+    fetch.tree_rows = drafted ? 0 : a.nodes;
+    fetch.tiles = t1 - t0;
+    fetch.dst = ring + wave * PER * 1024;
+    fetch.offsets(wave, lane);
   }
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    fetch<T, D, W>(ring, src, t0 + i, i, wave, drow, kchunk, vchunk);
+  for (int i = 0; i < NS - 1; ++i) fetch.next(i, wave, lane);
 
   // The block's nodes' mask rows as bits, if the run holds drafted tiles.
-  const int node0 = r0 / a.group;
-  if (t1 > src.context_tiles) {
+  if (t1 > context_tiles) {
     const int last = min((min(r0 + ROWS, a.rows) - 1) / a.group, a.nodes - 1);
     const uint8_t* mask = a.mask + b * a.mb;
     for (int n = node0 + wave; n <= last; n += W)
@@ -330,12 +350,10 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   uint32_t ka[DC], va[OC];
 #pragma unroll
   for (int c = 0; c < DC; ++c) ka[c] = row16 * RB + (((4 * c + quad) ^ R::kswz(row16)) * 16);
-  {
-    const int trow = 4 * quad + (row16 >> 2);
+  const int trow = 4 * quad + (row16 >> 2);
 #pragma unroll
-    for (int c = 0; c < OC; ++c)
-      va[c] = R::TILE + trow * RB + ((c ^ R::vswz(trow)) * 32) + 8 * (row16 & 3);
-  }
+  for (int c = 0; c < OC; ++c)
+    va[c] = R::TILE + trow * RB + ((c ^ R::vswz(trow)) * 32) + 8 * (row16 & 3);
 
   f32x4 o[MT][OC];
   float top[MT], sum[MT];  // reference maximum of row row16, this lane's share of its sum
@@ -346,19 +364,20 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
 #pragma unroll
     for (int c = 0; c < OC; ++c) o[m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  const float scale = a.scale_log2;
 
-  for (int t = t0; t < t1; ++t) {
-    const int it = t - t0;
-    // Tile t has landed (this wave's share) once only the NS - 2 younger tiles' loads are
-    // outstanding; behind the barrier every wave's share has, and every wave has read the stage
-    // that tile t + NS - 1 takes.
+  int stage = 0;
+  // Tile t has landed (this wave's share) once only the NS - 2 younger tiles' loads are
+  // outstanding; behind the barrier every wave's share has, and every wave has read the stage
+  // that tile t + NS - 1 takes.
+  auto arrive = [&]() {
     tk_attn::wait_vmcnt<(NS - 2) * 2 * PER>();
     if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    fetch<T, D, W>(ring, src, t + NS - 1, (it + NS - 1) % NS, wave, drow, kchunk, vchunk);
+    fetch.next(stage == 0 ? NS - 1 : stage - 1, wave, lane);
     __builtin_amdgcn_sched_barrier(0);
-    if (!busy) continue;
-    const uint32_t sb = ring_base + (it % NS) * R::STAGE;
-
+  };
+  // s[m][i][r]: product of row row16 of row tile m and key 16 i + 4 quad + r.
+  auto products = [&](uint32_t sb, f32x4 (&s)[MT][2]) {
     i32x4 kc[2][DC];
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
@@ -371,142 +390,157 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       tk_attn::pin(kc[0][c]);
       tk_attn::pin(kc[1][c]);
     }
-    // sc[m][i][r]: row row16 of tile m, key 16 i + 4 quad + r.
-    float sc[MT][2][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        s[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < DC; ++c) acc = tk_attn::Mma16<T>::run(kc[i][c], qf[m][c], acc);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[m][i][r] = acc[r] * a.scale_log2;
+        for (int c = 0; c < DC; ++c) s[m][i] = tk_attn::Mma16<T>::run(kc[i][c], qf[m][c], s[m][i]);
       }
-    // V^T fragments, read while the softmax runs, in batches of four output chunks (8 reads:
-    // lgkmcnt counts at most 15).
-    constexpr int HB = 4;
-    i32x2 lo[OC], hi[OC];
-    const bool drafted = t >= src.context_tiles;
-    const int live = drafted ? kTileKeys : src.length - t * kTileKeys;
-    if (drafted) {
-      const int word = t - src.context_tiles;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const bool real = w0 + 16 * m + row16 < a.rows;
-        const uint32_t bits = real ? seen[(node[m] - node0) * kMaskWords + word] >> (4 * quad) : 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!((bits >> (16 * i + r)) & 1)) sc[m][i][r] = -INFINITY;
-      }
-    } else if (live < kTileKeys) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (16 * i + 4 * quad + r >= live) sc[m][i][r] = -INFINITY;
-    }
-#pragma unroll
-    for (int c = 0; c < HB; ++c) {
-      lo[c] = tk_attn::lds_read_tr16<0>(sb + va[c]);
-      hi[c] = tk_attn::lds_read_tr16<16 * RB>(sb + va[c]);
-    }
-    // Lazy rescale: the reference maximum moves only when the tile's exceeds it by more than 8
-    // (base 2), so p <= 2^8 and o and sum are rescaled in few tiles.
-    i32x4 pf[MT];
+  };
+  // P = exp2(scale s - top) into pf. The reference maximum moves only when the tile's exceeds
+  // it by more than 8 (base 2), so p <= 2^8 and o and sum are rescaled in few tiles: a lane
+  // whose exponentials sum to at most 2^8 has none above it, and then no maximum is formed.
+  auto softmax = [&](f32x4 (&s)[MT][2], i32x4 (&pf)[MT]) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      float high = sc[m][0][0];
+      f32x4 p[2];
+      float part;
+      auto weights = [&]() {
+        part = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) high = fmaxf(high, sc[m][i][r]);
-      high = tk_attn::max_over_column(high);
-      const bool grow = high > top[m] + 8.f;
-      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-        const float next = grow ? high : top[m];
-        float alpha = __builtin_amdgcn_exp2f(top[m] - next);
-        asm volatile("" : "+v"(alpha));  // keeps the multiplies inside the branch
+          for (int r = 0; r < 4; ++r) {
+            p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[m][i][r], scale, -top[m]));
+            part += p[i][r];
+          }
+      };
+      weights();
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(part <= 256.f)) != 0, 0)) {
+        float high = s[m][0][0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) high = fmaxf(high, s[m][i][r]);
+        high = tk_attn::max_over_column(high) * scale;
+        const float next = high > top[m] + 8.f ? high : top[m];
+        const float alpha = __builtin_amdgcn_exp2f(top[m] - next);
         top[m] = next;
         sum[m] *= alpha;
 #pragma unroll
         for (int c = 0; c < OC; ++c) o[m][c] *= alpha;
+        weights();
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sc[m][i][r] = __builtin_amdgcn_exp2f(sc[m][i][r] - top[m]);
-          sum[m] += sc[m][i][r];
-        }
-      pf[m] = pack_probabilities<T>(sc[m]);
+      sum[m] += part;
+      pf[m] = tk_attn::acc_frag2<T>(p[0], p[1]);
     }
-    bool by_key = false;
-    if (drafted) {
-      u16x2 most = {0, 0};
+  };
+  // o += V^T P^T; the first batch of V fragments is already on its way.
+  i32x2 lo[OC], hi[OC];
+  auto request_v = [&](uint32_t sb, int c0) {
 #pragma unroll
-      for (int c0 = 0; c0 < OC; c0 += HB) {
-        i32x4 vf[HB];
-#pragma unroll
-        for (int c = 0; c < HB; ++c) vf[c] = tk_attn::read_v16<0, RB>(sb + va[c0 + c]);
-        tk_attn::wait_lgkm<0>();
-#pragma unroll
-        for (int c = 0; c < HB; ++c) {
-          tk_attn::pin(vf[c]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) most = max_magnitude(most, vf[c][i]);
-        }
-      }
-      by_key = __ballot(most[0] >= NONFINITE || most[1] >= NONFINITE) != 0;
+    for (int c = c0; c < c0 + HB; ++c) {
+      lo[c] = tk_attn::lds_read_tr16<0>(sb + va[c]);
+      hi[c] = tk_attn::lds_read_tr16<16 * RB>(sb + va[c]);
     }
-    if (by_key) {
-      const int word = t - src.context_tiles;
-      for (int c0 = 0; c0 < OC; ++c0) {
-        // Selects a register by a loop index through unrolled comparisons.
-        i32x4 vf = tk_attn::read_v16<0, RB>(sb + R::TILE + (4 * quad + (row16 >> 2)) * RB +
-                                            ((c0 ^ R::vswz(4 * quad + (row16 >> 2))) * 32) +
-                                            8 * (row16 & 3));
-        tk_attn::wait_lgkm<0>();
-        tk_attn::pin(vf);
-        for (int j = 0; j < kTileKeys; ++j) {
-          const i32x4 vj = only_key(vf, j, quad);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const f32x4 one = tk_attn::Mma16<T>::run(vj, only_key(pf[m], j, quad),
-                                                     f32x4{0.f, 0.f, 0.f, 0.f});
-            const bool real = w0 + 16 * m + row16 < a.rows;
-            const bool sees =
-                real && ((seen[(node[m] - node0) * kMaskWords + word] >> j) & 1) != 0;
-#pragma unroll
-            for (int c = 0; c < OC; ++c)
-              if (c == c0 && sees) o[m][c] += one;
-          }
-        }
-      }
-      continue;
-    }
+  };
+  auto accumulate = [&](uint32_t sb, const i32x4 (&pf)[MT]) {
 #pragma unroll
     for (int c0 = 0; c0 < OC; c0 += HB) {
       tk_attn::wait_lgkm<0>();
 #pragma unroll
       for (int c = c0; c < c0 + HB; ++c) asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
-      if (c0 + HB < OC) {
-#pragma unroll
-        for (int c = c0 + HB; c < c0 + 2 * HB; ++c) {
-          lo[c] = tk_attn::lds_read_tr16<0>(sb + va[c]);
-          hi[c] = tk_attn::lds_read_tr16<16 * RB>(sb + va[c]);
-        }
-      }
+      if (c0 + HB < OC) request_v(sb, c0 + HB);
 #pragma unroll
       for (int c = c0; c < c0 + HB; ++c)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
           o[m][c] = tk_attn::Mma16<T>::run(i32x4{lo[c][0], lo[c][1], hi[c][0], hi[c][1]}, pf[m],
                                            o[m][c]);
+    }
+  };
+
+  for (int t = t0; t < c1; ++t) {
+    arrive();
+    const uint32_t sb = ring_base + stage * R::STAGE;
+    stage = stage == NS - 1 ? 0 : stage + 1;
+    if (!busy) continue;
+    f32x4 s[MT][2];
+    i32x4 pf[MT];
+    products(sb, s);
+    request_v(sb, 0);
+    const int live = run.length - t * kTileKeys;
+    if (__builtin_expect(live < kTileKeys, 0)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * i + 4 * quad + r >= live) s[m][i][r] = -INFINITY;
+    }
+    softmax(s, pf);
+    accumulate(sb, pf);
+  }
+
+  for (int t = max(t0, context_tiles); t < t1; ++t) {
+    arrive();
+    const uint32_t sb = ring_base + stage * R::STAGE;
+    stage = stage == NS - 1 ? 0 : stage + 1;
+    if (!busy) continue;
+    const int word = t - context_tiles;
+    uint32_t bits[MT];  // the tile's keys that row row16 sees
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = w0 + 16 * m + row16;
+      bits[m] = r < a.rows ? seen[(r / a.group - node0) * kMaskWords + word] : 0;
+    }
+    f32x4 s[MT][2];
+    i32x4 pf[MT];
+    products(sb, s);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!((bits[m] >> (16 * i + 4 * quad + r)) & 1)) s[m][i][r] = -INFINITY;
+    softmax(s, pf);
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int c0 = 0; c0 < OC; c0 += HB) {
+      request_v(sb, c0);
+      tk_attn::wait_lgkm<0>();
+#pragma unroll
+      for (int c = c0; c < c0 + HB; ++c) {
+        asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          most = max_magnitude(most, lo[c][i]);
+          most = max_magnitude(most, hi[c][i]);
+        }
+      }
+    }
+    if (__builtin_expect(__ballot(most[0] >= NONFINITE || most[1] >= NONFINITE) == 0, 1)) {
+      request_v(sb, 0);
+      accumulate(sb, pf);
+      continue;
+    }
+    for (int j = 0; j < kTileKeys; ++j) {
+      i32x4 pj[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) pj[m] = only_key(pf[m], j, quad);
+#pragma unroll
+      for (int c = 0; c < OC; ++c) {
+        const i32x4 vj = only_key(i32x4{lo[c][0], lo[c][1], hi[c][0], hi[c][1]}, j, quad);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const f32x4 one = tk_attn::Mma16<T>::run(vj, pj[m], f32x4{0.f, 0.f, 0.f, 0.f});
+          if ((bits[m] >> j) & 1) o[m][c] += one;
+        }
+      }
     }
   }
   // The tiles issued past the end still write (zeros) into the ring.
@@ -520,17 +554,19 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
     const int r = w0 + 16 * m + row16;
     if (r >= a.rows) continue;
     if (run.splits == 1) {
-      const int h = kvh * a.group + (r - node[m] * a.group);
-      T* dst = static_cast<T*>(a.o) + b * a.ob + h * a.oh + node[m] * a.ot + 4 * quad;
+      const int node = r / a.group;
+      const int h = kvh * a.group + (r - node * a.group);
+      const float share = l == 0.f ? 0.f : 1.f / l;
+      T* dst = static_cast<T*>(a.o) + b * a.ob + h * a.oh + node * a.ot + 4 * quad;
 #pragma unroll
       for (int c = 0; c < OC; ++c) {
         float out[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = l == 0.f ? 0.f : o[m][c][i] / l;
+        for (int i = 0; i < 4; ++i) out[i] = o[m][c][i] * share;
         tk::store_vec<T, 4>(dst + 16 * c, out);
       }
       if (quad == 0)
-        a.lse[(int64_t(b) * a.q_heads + h) * a.nodes + node[m]] =
+        a.lse[(int64_t(b) * a.q_heads + h) * a.nodes + node] =
             l == 0.f ? -INFINITY : top[m] + log2f(l);
     } else {
       const int64_t at = int64_t(slot) * a.rows + r;
@@ -598,20 +634,36 @@ int rows_per_block(int64_t rows) {
   return 256;
 }
 
+// Instantiated here by name: left to the launches below, the host compiler leaves some of these
+// kernels' launch stubs undefined.
+#define TK_TREE_SPLIT(T, D, W, MT) template __global__ void tree_split_kernel<T, D, W, MT>(TreeArgs)
+#define TK_TREE_SPLITS(T)                                                                       \
+  TK_TREE_SPLIT(T, 128, 1, 1); TK_TREE_SPLIT(T, 128, 2, 1); TK_TREE_SPLIT(T, 128, 4, 1);        \
+  TK_TREE_SPLIT(T, 128, 4, 2); TK_TREE_SPLIT(T, 128, 8, 2); TK_TREE_SPLIT(T, 64, 1, 1);         \
+  TK_TREE_SPLIT(T, 64, 2, 1); TK_TREE_SPLIT(T, 64, 4, 1); TK_TREE_SPLIT(T, 64, 4, 2);           \
+  TK_TREE_SPLIT(T, 64, 4, 4)
+TK_TREE_SPLITS(__bf16);
+TK_TREE_SPLITS(_Float16);
+
+template <typename T, int D, int W, int MT>
+void launch_split(const TreeArgs& a, dim3 grid, hipStream_t s) {
+  hipLaunchKernelGGL((tree_split_kernel<T, D, W, MT>), grid, dim3(64 * W), 0, s, a);
+}
+
 template <typename T, int D>
 void launch(const TreeArgs& a, bool combine, hipStream_t s) {
   const int64_t pairs = tk::cdiv(int64_t(a.flat) * a.kv_heads, 8) * 8;
   const dim3 grid(static_cast<uint32_t>(pairs * a.row_blocks));
   switch (rows_per_block(a.rows)) {
-    case 16: hipLaunchKernelGGL((tree_split_kernel<T, D, 1, 1>), grid, dim3(64), 0, s, a); break;
-    case 32: hipLaunchKernelGGL((tree_split_kernel<T, D, 2, 1>), grid, dim3(128), 0, s, a); break;
-    case 64: hipLaunchKernelGGL((tree_split_kernel<T, D, 4, 1>), grid, dim3(256), 0, s, a); break;
-    case 128: hipLaunchKernelGGL((tree_split_kernel<T, D, 4, 2>), grid, dim3(256), 0, s, a); break;
+    case 16: launch_split<T, D, 1, 1>(a, grid, s); break;
+    case 32: launch_split<T, D, 2, 1>(a, grid, s); break;
+    case 64: launch_split<T, D, 4, 1>(a, grid, s); break;
+    case 128: launch_split<T, D, 4, 2>(a, grid, s); break;
     default:
       if constexpr (D == 128)
-        hipLaunchKernelGGL((tree_split_kernel<T, D, 8, 2>), grid, dim3(512), 0, s, a);
+        launch_split<T, D, 8, 2>(a, grid, s);
       else
-        hipLaunchKernelGGL((tree_split_kernel<T, D, 4, 4>), grid, dim3(256), 0, s, a);
+        launch_split<T, D, 4, 4>(a, grid, s);
   }
   if (combine)
     hipLaunchKernelGGL((tree_combine_kernel<T, D>),
@@ -731,7 +783,9 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
   a.runs = static_cast<int>(plan.runs);
   a.row_blocks = static_cast<int>(plan.row_blocks);
   a.flat = static_cast<int>(plan.flat);
-  a.scale_log2 = scale * kLog2e;
+  // Not 0, which would turn a masked score (-inf) into NaN: 1e-30 leaves no score above 2^-20.
+  a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+  a.flip = scale < 0.f ? int(0x80008000u) : 0;
   hipStream_t s = tk::as_stream(stream);
   if (dtype == TK_DTYPE_BF16) {
     if (head_dim == 128)
