@@ -446,7 +446,7 @@ int tk_tree_decode(int dtype, const void* q, const void* k_cache, const void* v_
 /* Partial results that tk_tree_decode keeps per query row of a KV head for these sizes (group =
  * q_heads / kv_heads); -1 for sizes it does not take. No launch, no GPU. */
 int tk_tree_decode_slots(int64_t batch, int64_t kv_heads, int64_t group, int64_t max_len,
-                         int64_t nodes);
+                         int64_t nodes, int64_t head_dim);
 
 /* Verification of drafted tokens. Per sequence, `nodes` <= 256 nodes, node 0 the last token;
  * target[b][i] (strides {batch, node}, unit-stride entries) is the target's distribution behind

@@ -151,7 +151,6 @@ struct Ring {
   static constexpr int RB = D * 2;             // bytes per row
   static constexpr int TILE = kTileKeys * RB;  // bytes per tensor tile
   static constexpr int STAGE = 2 * TILE;
-  static constexpr int NS = D == 128 ? 4 : 8;  // 64 KiB: two workgroups share a CU
   static constexpr int IPT = TILE / 1024;      // DMA instructions per tensor tile
   static constexpr int RPI = 1024 / RB;        // rows per DMA instruction
   static constexpr int CPR = RB / 16;          // 16-byte chunks per row
@@ -179,9 +178,9 @@ struct Fetcher {
   const T *k_tree, *v_tree;
   uint32_t k2, v2;          // bytes per row
   uint32_t kt2, vt2;
-  int left;                 // rows from there to the segment's end
-  int tree_rows;            // of the tree's segment, 0 once it is the current one
-  int tiles;                // of the run, not yet issued
+  int left;                 // rows from there to the end of the run's part of the segment
+  int tiles;                // of this segment (padded with empty ones), not yet issued
+  int tree_rows;            // rows of the tree in the run, 0 once it is the current segment
   char* dst;                // this wave's share of the ring's first stage
   uint32_t koff[PER], voff[PER];
 
@@ -197,10 +196,10 @@ struct Fetcher {
     }
   }
 
-  // The next tile into `stage`. Past the run's end (issued to keep the wait counts static) the
-  // range is empty: nothing is read, LDS gets zeros.
+  // The next tile into `stage`. Tiles past a segment's rows (issued to fill a step and to keep
+  // the wait counts static) have an empty range: nothing is read, LDS gets zeros.
   __device__ __forceinline__ void next(int stage, int wave, int lane) {
-    if (left <= 0 && tree_rows > 0) {
+    if (tiles <= 0 && tree_rows > 0) {
       k = reinterpret_cast<const char*>(k_tree);
       v = reinterpret_cast<const char*>(v_tree);
       k2 = kt2;
@@ -209,7 +208,7 @@ struct Fetcher {
       tree_rows = 0;
       offsets(wave, lane);
     }
-    const int rows = tiles > 0 ? min(left, kTileKeys) : 0;
+    const int rows = min(left, kTileKeys);
     // The last row ends D elements in: bytes past it are outside the range.
     const uint32_t krange = rows > 0 ? uint32_t(rows - 1) * k2 + D * 2 : 0;
     const uint32_t vrange = rows > 0 ? uint32_t(rows - 1) * v2 + D * 2 : 0;
@@ -251,10 +250,14 @@ __device__ __forceinline__ i32x4 only_key(i32x4 f, int j, int quad) {
   return r;
 }
 
-template <typename T, int D, int W, int MT>
+// KT tiles per step (one barrier each), NS ring stages.
+template <typename T, int D, int W, int MT, int KT, int NS>
 __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(TreeArgs a) {
   using R = Ring<D>;
-  constexpr int DC = D / 32, OC = D / 16, NS = R::NS, RB = R::RB, PER = R::IPT / W;
+  static_assert(NS % KT == 0 && NS >= 2 * KT, "a step's stages are refilled while the next is read");
+  constexpr int DC = D / 32, OC = D / 16, RB = R::RB, PER = R::IPT / W;
+  // vmcnt is 6 bits: at most 63 DMA instructions may be outstanding.
+  static_assert((NS - KT) * 2 * PER < 64, "ring deeper than the vmcnt counter");
   constexpr int ROWS = 16 * W * MT;
   constexpr int HB = 4;  // output chunks per batch of V reads
   constexpr int NONFINITE = __is_same(T, __bf16) ? 0x7F80 : 0x7C00;
@@ -278,6 +281,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   const int t0 = run.split * lengths.chunk;
   const int t1 = min(t0 + lengths.chunk, context_tiles + a.tree_tiles);
   const int c1 = min(t1, context_tiles);  // context tiles t0 .. c1-1, then drafted ones
+  const int limit = min(run.length, c1 * kTileKeys);
 
   const int row16 = lane & 15;
   const int quad = lane >> 4;
@@ -285,6 +289,32 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   const int w0 = r0 + wave * 16 * MT;   // this wave's first row
   const bool busy = w0 < a.rows;        // waves past the last row only fetch
   const int node0 = r0 / a.group;
+
+  Fetcher<T, D, W> fetch;
+  {
+    const bool drafted = t0 >= context_tiles;
+    const int first = (drafted ? t0 - context_tiles : t0) * kTileKeys;
+    const T* kc = static_cast<const T*>(a.k) + b * a.kb + kvh * a.kh;
+    const T* vc = static_cast<const T*>(a.v) + b * a.vb + kvh * a.vh;
+    fetch.k_tree = static_cast<const T*>(a.k_tree) + b * a.ktb + kvh * a.kth;
+    fetch.v_tree = static_cast<const T*>(a.v_tree) + b * a.vtb + kvh * a.vth;
+    fetch.k = reinterpret_cast<const char*>(drafted ? fetch.k_tree + first * a.ktl
+                                                    : kc + first * a.kl);
+    fetch.v = reinterpret_cast<const char*>(drafted ? fetch.v_tree + first * a.vtl
+                                                    : vc + first * a.vl);
+    fetch.kt2 = uint32_t(a.ktl * 2);
+    fetch.vt2 = uint32_t(a.vtl * 2);
+    fetch.k2 = drafted ? fetch.kt2 : uint32_t(a.kl * 2);
+    fetch.v2 = drafted ? fetch.vt2 : uint32_t(a.vl * 2);
+    const int tree_rows = min(a.nodes, (t1 - context_tiles) * kTileKeys);
+    fetch.left = (drafted ? tree_rows : limit) - first;
+    fetch.tiles = ((max(c1 - t0, 0) + KT - 1) / KT) * KT;
+    fetch.tree_rows = drafted ? 0 : tree_rows;
+    fetch.dst = ring + wave * PER * 1024;
+    fetch.offsets(wave, lane);
+  }
+#pragma unroll
+  for (int i = 0; i < NS - KT; ++i) fetch.next(i, wave, lane);
 
   // Q^T fragments: row w0 + 16 mt + row16 (zero past the last), dims 32 c + 8 quad .. +7. A
   // negative scale is taken into Q's signs (exact), so that the largest score is the largest
@@ -307,31 +337,6 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       qf[m][c] ^= a.flip;
       tk_attn::pin(qf[m][c]);
     }
-
-  Fetcher<T, D, W> fetch;
-  {
-    const bool drafted = t0 >= context_tiles;
-    const int first = (drafted ? t0 - context_tiles : t0) * kTileKeys;
-    const T* kc = static_cast<const T*>(a.k) + b * a.kb + kvh * a.kh;
-    const T* vc = static_cast<const T*>(a.v) + b * a.vb + kvh * a.vh;
-    fetch.k_tree = static_cast<const T*>(a.k_tree) + b * a.ktb + kvh * a.kth;
-    fetch.v_tree = static_cast<const T*>(a.v_tree) + b * a.vtb + kvh * a.vth;
-    fetch.k = reinterpret_cast<const char*>(drafted ? fetch.k_tree + first * a.ktl
-                                                    : kc + first * a.kl);
-    fetch.v = reinterpret_cast<const char*>(drafted ? fetch.v_tree + first * a.vtl
-                                                    : vc + first * a.vl);
-    fetch.kt2 = uint32_t(a.ktl * 2);
-    fetch.vt2 = uint32_t(a.vtl * 2);
-    fetch.k2 = drafted ? fetch.kt2 : uint32_t(a.kl * 2);
-    fetch.v2 = drafted ? fetch.vt2 : uint32_t(a.vl * 2);
-    fetch.left = (drafted ? a.nodes : run.length) - first;
-    fetch.tree_rows = drafted ? 0 : a.nodes;
-    fetch.tiles = t1 - t0;
-    fetch.dst = ring + wave * PER * 1024;
-    fetch.offsets(wave, lane);
-  }
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i) fetch.next(i, wave, lane);
 
   // The block's nodes' mask rows as bits, if the run holds drafted tiles.
   if (t1 > context_tiles) {
@@ -367,17 +372,18 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   const float scale = a.scale_log2;
 
   int stage = 0;
-  // Tile t has landed (this wave's share) once only the NS - 2 younger tiles' loads are
-  // outstanding; behind the barrier every wave's share has, and every wave has read the stage
-  // that tile t + NS - 1 takes.
+  // A step's tiles have landed (this wave's share) once only the NS - 2 KT younger tiles' loads
+  // are outstanding; behind the barrier every wave's share has, and every wave has read the
+  // stages before it, which the tiles fetched now take.
   auto arrive = [&]() {
-    tk_attn::wait_vmcnt<(NS - 2) * 2 * PER>();
+    tk_attn::wait_vmcnt<(NS - 2 * KT) * 2 * PER>();
     if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    fetch.next(stage == 0 ? NS - 1 : stage - 1, wave, lane);
+#pragma unroll
+    for (int i = 0; i < KT; ++i) fetch.next((stage == 0 ? NS : stage) - KT + i, wave, lane);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // s[m][i][r]: product of row row16 of row tile m and key 16 i + 4 quad + r.
-  auto products = [&](uint32_t sb, f32x4 (&s)[MT][2]) {
+  // s[m][i][r]: product of row row16 of row tile m and key 16 i + 4 quad + r of the tiles.
+  auto products = [&](uint32_t sb, f32x4(&s)[MT][2]) {
     i32x4 kc[2][DC];
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
@@ -399,31 +405,33 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
         for (int c = 0; c < DC; ++c) s[m][i] = tk_attn::Mma16<T>::run(kc[i][c], qf[m][c], s[m][i]);
       }
   };
-  // P = exp2(scale s - top) into pf. The reference maximum moves only when the tile's exceeds
-  // it by more than 8 (base 2), so p <= 2^8 and o and sum are rescaled in few tiles: a lane
-  // whose exponentials sum to at most 2^8 has none above it, and then no maximum is formed.
-  auto softmax = [&](f32x4 (&s)[MT][2], i32x4 (&pf)[MT]) {
+  // P = exp2(scale s - top) of N tiles into pf. The reference maximum moves only when the
+  // tiles' exceeds it by more than 8 (base 2), so p <= 2^8 and o and sum are rescaled in few
+  // steps: a lane whose exponentials sum to at most 2^8 has none above it, and then no maximum
+  // is formed.
+  auto softmax = [&](auto& s, auto& pf) {
+    constexpr int N = sizeof(s) / sizeof(f32x4[MT][2]);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      f32x4 p[2];
-      float part;
-      auto weights = [&]() {
-        part = 0.f;
+      f32x4 p[N][2];
+      float part = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[m][i][r], scale, -top[m]));
-            part += p[i][r];
+            p[n][i][r] = __builtin_amdgcn_exp2f(fmaf(s[n][m][i][r], scale, -top[m]));
+            part += p[n][i][r];
           }
-      };
-      weights();
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(part <= 256.f)) != 0, 0)) {
-        float high = s[m][0][0];
+        float high = s[0][m][0][0];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) high = fmaxf(high, s[m][i][r]);
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) high = fmaxf(high, s[n][m][i][r]);
         high = tk_attn::max_over_column(high) * scale;
         const float next = high > top[m] + 8.f ? high : top[m];
         const float alpha = __builtin_amdgcn_exp2f(top[m] - next);
@@ -431,13 +439,24 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
         sum[m] *= alpha;
 #pragma unroll
         for (int c = 0; c < OC; ++c) o[m][c] *= alpha;
-        weights();
+        part = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              p[n][i][r] = __builtin_amdgcn_exp2f(fmaf(s[n][m][i][r], scale, -next));
+              part += p[n][i][r];
+            }
       }
       sum[m] += part;
-      pf[m] = tk_attn::acc_frag2<T>(p[0], p[1]);
+#pragma unroll
+      for (int n = 0; n < N; ++n) pf[n][m] = tk_attn::acc_frag2<T>(p[n][0], p[n][1]);
     }
   };
-  // o += V^T P^T; the first batch of V fragments is already on its way.
+  // o += V^T P^T of a tile; the first batch of its V fragments is already on its way, and that
+  // of the tile at `after` (none: 0) is sent for at the end.
   i32x2 lo[OC], hi[OC];
   auto request_v = [&](uint32_t sb, int c0) {
 #pragma unroll
@@ -446,99 +465,112 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       hi[c] = tk_attn::lds_read_tr16<16 * RB>(sb + va[c]);
     }
   };
-  auto accumulate = [&](uint32_t sb, const i32x4 (&pf)[MT]) {
+  auto accumulate = [&](uint32_t sb, const i32x4(&pf)[MT], uint32_t after) {
 #pragma unroll
     for (int c0 = 0; c0 < OC; c0 += HB) {
       tk_attn::wait_lgkm<0>();
+      i32x4 vf[HB];
 #pragma unroll
-      for (int c = c0; c < c0 + HB; ++c) asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
-      if (c0 + HB < OC) request_v(sb, c0 + HB);
+      for (int c = 0; c < HB; ++c) {
+        asm volatile("" : "+v"(lo[c0 + c]), "+v"(hi[c0 + c]));
+        vf[c] = i32x4{lo[c0 + c][0], lo[c0 + c][1], hi[c0 + c][0], hi[c0 + c][1]};
+      }
+      if (c0 + HB < OC)
+        request_v(sb, c0 + HB);
+      else if (after != 0)
+        request_v(after, 0);
 #pragma unroll
-      for (int c = c0; c < c0 + HB; ++c)
+      for (int c = 0; c < HB; ++c)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          o[m][c] = tk_attn::Mma16<T>::run(i32x4{lo[c][0], lo[c][1], hi[c][0], hi[c][1]}, pf[m],
-                                           o[m][c]);
+          o[m][c0 + c] = tk_attn::Mma16<T>::run(vf[c], pf[m], o[m][c0 + c]);
     }
   };
 
-  for (int t = t0; t < c1; ++t) {
+  for (int t = t0; t < c1; t += KT) {
     arrive();
     const uint32_t sb = ring_base + stage * R::STAGE;
-    stage = stage == NS - 1 ? 0 : stage + 1;
+    stage = stage == NS - KT ? 0 : stage + KT;
     if (!busy) continue;
-    f32x4 s[MT][2];
-    i32x4 pf[MT];
-    products(sb, s);
+    f32x4 s[KT][MT][2];
+    i32x4 pf[KT][MT];
+#pragma unroll
+    for (int n = 0; n < KT; ++n) products(sb + n * R::STAGE, s[n]);
     request_v(sb, 0);
-    const int live = run.length - t * kTileKeys;
-    if (__builtin_expect(live < kTileKeys, 0)) {
+    const int live = limit - t * kTileKeys;
+    if (__builtin_expect(live < KT * kTileKeys, 0)) {
+#pragma unroll
+      for (int n = 0; n < KT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (32 * n + 16 * i + 4 * quad + r >= live) s[n][m][i][r] = -INFINITY;
+    }
+    softmax(s, pf);
+#pragma unroll
+    for (int n = 0; n < KT; ++n)
+      accumulate(sb + n * R::STAGE, pf[n], n + 1 < KT ? sb + (n + 1) * R::STAGE : 0);
+  }
+
+  for (int t = max(t0, context_tiles); t < t1; t += KT) {
+    arrive();
+    uint32_t sb = ring_base + stage * R::STAGE;
+    stage = stage == NS - KT ? 0 : stage + KT;
+    if (!busy) continue;
+    for (int tile = t; tile < min(t + KT, t1); ++tile, sb += R::STAGE) {
+      const int word = tile - context_tiles;
+      uint32_t bits[MT];  // the tile's keys that row row16 sees
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int r = w0 + 16 * m + row16;
+        bits[m] = r < a.rows ? seen[(r / a.group - node0) * kMaskWords + word] : 0;
+      }
+      f32x4 s[1][MT][2];
+      i32x4 pf[1][MT];
+      products(sb, s[0]);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (16 * i + 4 * quad + r >= live) s[m][i][r] = -INFINITY;
-    }
-    softmax(s, pf);
-    accumulate(sb, pf);
-  }
-
-  for (int t = max(t0, context_tiles); t < t1; ++t) {
-    arrive();
-    const uint32_t sb = ring_base + stage * R::STAGE;
-    stage = stage == NS - 1 ? 0 : stage + 1;
-    if (!busy) continue;
-    const int word = t - context_tiles;
-    uint32_t bits[MT];  // the tile's keys that row row16 sees
+            if (!((bits[m] >> (16 * i + 4 * quad + r)) & 1)) s[0][m][i][r] = -INFINITY;
+      softmax(s, pf);
+      u16x2 most = {0, 0};
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int r = w0 + 16 * m + row16;
-      bits[m] = r < a.rows ? seen[(r / a.group - node0) * kMaskWords + word] : 0;
-    }
-    f32x4 s[MT][2];
-    i32x4 pf[MT];
-    products(sb, s);
+      for (int c0 = 0; c0 < OC; c0 += HB) {
+        request_v(sb, c0);
+        tk_attn::wait_lgkm<0>();
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int c = c0; c < c0 + HB; ++c) {
+          asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!((bits[m] >> (16 * i + 4 * quad + r)) & 1)) s[m][i][r] = -INFINITY;
-    softmax(s, pf);
-    u16x2 most = {0, 0};
-#pragma unroll
-    for (int c0 = 0; c0 < OC; c0 += HB) {
-      request_v(sb, c0);
-      tk_attn::wait_lgkm<0>();
-#pragma unroll
-      for (int c = c0; c < c0 + HB; ++c) {
-        asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          most = max_magnitude(most, lo[c][i]);
-          most = max_magnitude(most, hi[c][i]);
+          for (int i = 0; i < 2; ++i) {
+            most = max_magnitude(most, lo[c][i]);
+            most = max_magnitude(most, hi[c][i]);
+          }
         }
       }
-    }
-    if (__builtin_expect(__ballot(most[0] >= NONFINITE || most[1] >= NONFINITE) == 0, 1)) {
-      request_v(sb, 0);
-      accumulate(sb, pf);
-      continue;
-    }
-    for (int j = 0; j < kTileKeys; ++j) {
-      i32x4 pj[MT];
+      if (__builtin_expect(__ballot(most[0] >= NONFINITE || most[1] >= NONFINITE) == 0, 1)) {
+        request_v(sb, 0);
+        accumulate(sb, pf[0], 0);
+        continue;
+      }
+      for (int j = 0; j < kTileKeys; ++j) {
+        i32x4 pj[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) pj[m] = only_key(pf[m], j, quad);
+        for (int m = 0; m < MT; ++m) pj[m] = only_key(pf[0][m], j, quad);
 #pragma unroll
-      for (int c = 0; c < OC; ++c) {
-        const i32x4 vj = only_key(i32x4{lo[c][0], lo[c][1], hi[c][0], hi[c][1]}, j, quad);
+        for (int c = 0; c < OC; ++c) {
+          const i32x4 vj = only_key(i32x4{lo[c][0], lo[c][1], hi[c][0], hi[c][1]}, j, quad);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const f32x4 one = tk_attn::Mma16<T>::run(vj, pj[m], f32x4{0.f, 0.f, 0.f, 0.f});
-          if ((bits[m] >> j) & 1) o[m][c] += one;
+          for (int m = 0; m < MT; ++m) {
+            const f32x4 one = tk_attn::Mma16<T>::run(vj, pj[m], f32x4{0.f, 0.f, 0.f, 0.f});
+            if ((bits[m] >> j) & 1) o[m][c] += one;
+          }
         }
       }
     }
@@ -626,44 +658,51 @@ __global__ __launch_bounds__(64 * kCombineWaves) void tree_combine_kernel(TreeAr
         total == 0.f ? -INFINITY : high + log2f(total);
 }
 
-// Rows per workgroup by the rows a KV head has: as few waves as hold them (each key tile costs
-// every wave its LDS reads), 256 at most.
-int rows_per_block(int64_t rows) {
+// Workgroup shapes by the rows a KV head has: as few waves as hold them (each key tile costs
+// every wave its LDS reads), 256 rows at most. `resident`: workgroups that run at once, two per CU
+// with a 64 KiB ring, one with 128 KiB (256 rows at head_dim 128, eight waves of 256 registers).
+struct Shape {
+  int rows, resident;
+};
+Shape shape_for(int64_t rows, int64_t head_dim) {
   for (int n : {16, 32, 64, 128})
-    if (rows <= n) return n;
-  return 256;
+    if (rows <= n) return {n, 512};
+  return {256, head_dim == 128 ? 256 : 512};
 }
 
 // Instantiated here by name: left to the launches below, the host compiler leaves some of these
 // kernels' launch stubs undefined.
-#define TK_TREE_SPLIT(T, D, W, MT) template __global__ void tree_split_kernel<T, D, W, MT>(TreeArgs)
-#define TK_TREE_SPLITS(T)                                                                       \
-  TK_TREE_SPLIT(T, 128, 1, 1); TK_TREE_SPLIT(T, 128, 2, 1); TK_TREE_SPLIT(T, 128, 4, 1);        \
-  TK_TREE_SPLIT(T, 128, 4, 2); TK_TREE_SPLIT(T, 128, 8, 2); TK_TREE_SPLIT(T, 64, 1, 1);         \
-  TK_TREE_SPLIT(T, 64, 2, 1); TK_TREE_SPLIT(T, 64, 4, 1); TK_TREE_SPLIT(T, 64, 4, 2);           \
-  TK_TREE_SPLIT(T, 64, 4, 4)
+#define TK_TREE_SPLIT(T, D, W, MT, KT, NS) \
+  template __global__ void tree_split_kernel<T, D, W, MT, KT, NS>(TreeArgs)
+#define TK_TREE_SPLITS(T)                                                           \
+  TK_TREE_SPLIT(T, 128, 1, 1, 1, 4); TK_TREE_SPLIT(T, 128, 2, 1, 1, 4);             \
+  TK_TREE_SPLIT(T, 128, 4, 1, 1, 4); TK_TREE_SPLIT(T, 128, 4, 2, 1, 4);             \
+  TK_TREE_SPLIT(T, 128, 8, 2, 2, 8); TK_TREE_SPLIT(T, 64, 1, 1, 1, 8);              \
+  TK_TREE_SPLIT(T, 64, 2, 1, 1, 8); TK_TREE_SPLIT(T, 64, 4, 1, 1, 8);               \
+  TK_TREE_SPLIT(T, 64, 4, 2, 1, 8); TK_TREE_SPLIT(T, 64, 4, 4, 2, 8)
 TK_TREE_SPLITS(__bf16);
 TK_TREE_SPLITS(_Float16);
 
-template <typename T, int D, int W, int MT>
+template <typename T, int D, int W, int MT, int KT, int NS>
 void launch_split(const TreeArgs& a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((tree_split_kernel<T, D, W, MT>), grid, dim3(64 * W), 0, s, a);
+  hipLaunchKernelGGL((tree_split_kernel<T, D, W, MT, KT, NS>), grid, dim3(64 * W), 0, s, a);
 }
 
 template <typename T, int D>
 void launch(const TreeArgs& a, bool combine, hipStream_t s) {
+  constexpr int NS = D == 128 ? 4 : 8;
   const int64_t pairs = tk::cdiv(int64_t(a.flat) * a.kv_heads, 8) * 8;
   const dim3 grid(static_cast<uint32_t>(pairs * a.row_blocks));
-  switch (rows_per_block(a.rows)) {
-    case 16: launch_split<T, D, 1, 1>(a, grid, s); break;
-    case 32: launch_split<T, D, 2, 1>(a, grid, s); break;
-    case 64: launch_split<T, D, 4, 1>(a, grid, s); break;
-    case 128: launch_split<T, D, 4, 2>(a, grid, s); break;
+  switch (shape_for(a.rows, D).rows) {
+    case 16: launch_split<T, D, 1, 1, 1, NS>(a, grid, s); break;
+    case 32: launch_split<T, D, 2, 1, 1, NS>(a, grid, s); break;
+    case 64: launch_split<T, D, 4, 1, 1, NS>(a, grid, s); break;
+    case 128: launch_split<T, D, 4, 2, 1, NS>(a, grid, s); break;
     default:
       if constexpr (D == 128)
-        launch_split<T, D, 8, 2>(a, grid, s);
+        launch_split<T, D, 8, 2, 2, 8>(a, grid, s);
       else
-        launch_split<T, D, 4, 4>(a, grid, s);
+        launch_split<T, D, 4, 4, 2, 8>(a, grid, s);
   }
   if (combine)
     hipLaunchKernelGGL((tree_combine_kernel<T, D>),
@@ -672,8 +711,6 @@ void launch(const TreeArgs& a, bool combine, hipStream_t s) {
                        dim3(64 * kCombineWaves), 0, s, a);
 }
 
-// Workgroups that run at once: two per CU (a 64 KiB ring each).
-constexpr int kResident = 512;
 constexpr int kMinChunk = 4;  // tiles
 
 // How the call is cut: runs (the tiles of all sequences over `runs` give the run length), the
@@ -683,11 +720,13 @@ struct Plan {
   int64_t row_blocks, runs, flat;
   bool combine;
 };
-Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, int64_t nodes) {
+Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, int64_t nodes,
+               int64_t head_dim) {
   Plan p;
-  p.row_blocks = tk::cdiv(rows, rows_per_block(rows));
+  const Shape shape = shape_for(rows, head_dim);
+  p.row_blocks = tk::cdiv(rows, shape.rows);
   const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
-  const int64_t base = kResident / (kv_heads * p.row_blocks);
+  const int64_t base = shape.resident / (kv_heads * p.row_blocks);
   p.runs = base > 2 * batch ? base - batch : base > 1 ? base : 1;
   p.combine = most > kMinChunk;
   p.flat = p.runs + batch;
@@ -699,9 +738,9 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, i
 }  // namespace
 
 extern "C" int tk_tree_decode_slots(int64_t batch, int64_t kv_heads, int64_t group,
-                                    int64_t max_len, int64_t nodes) {
+                                    int64_t max_len, int64_t nodes, int64_t head_dim) {
   if (batch <= 0 || kv_heads <= 0 || group <= 0 || max_len <= 0 || nodes <= 0) return -1;
-  const Plan p = make_plan(batch, kv_heads, nodes * group, max_len, nodes);
+  const Plan p = make_plan(batch, kv_heads, nodes * group, max_len, nodes, head_dim);
   if (!p.combine) return 0;
   const int64_t slots = p.flat * kv_heads;
   return slots > INT32_MAX ? -1 : static_cast<int>(slots);
@@ -733,7 +772,7 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
     return tk::fail("tree decode: problem too large");
   const int64_t group = q_heads / kv_heads, rows = nodes * group;
   const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
-  const Plan plan = make_plan(batch, kv_heads, rows, max_len, nodes);
+  const Plan plan = make_plan(batch, kv_heads, rows, max_len, nodes, head_dim);
   if (batch * most > INT32_MAX / 2 || plan.flat * kv_heads * plan.row_blocks > (1 << 22))
     return tk::fail("tree decode: problem too large");
   if (plan.combine && workspace == nullptr) return tk::fail("tree decode: null pointer");

@@ -127,7 +127,7 @@ _SIGNATURES: dict[str, list[object]] = {
 _QUERIES: dict[str, list[object]] = {
     "tk_gemm_tile": [_P, _P] + [_I64] * 7,
     "tk_attn_fwd_rows": [_I64, _I64, _I64, _I64, _I64, _I64, _I32],
-    "tk_tree_decode_slots": [_I64] * 5,
+    "tk_tree_decode_slots": [_I64] * 6,
 }
 
 EXPORTED_SYMBOLS: tuple[str, ...] = ("tk_abi_version", "tk_last_error", *_QUERIES, *_SIGNATURES)

@@ -85,7 +85,8 @@ def tree_decode(
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((batch, q_heads, nodes), dtype=torch.float32, device=q.device)
     group = q_heads // kv_heads
-    slots = _hip.query("tk_tree_decode_slots", batch, kv_heads, group, max_len, nodes)
+    slots = _hip.query("tk_tree_decode_slots", batch, kv_heads, group, max_len, nodes,
+                       head_dim)
     if slots < 0:
         raise ValueError("tree_decode: the problem is too large")
     workspace = torch.empty(slots * nodes * group * (head_dim + 2), dtype=torch.float32,
