@@ -382,28 +382,42 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
     for (int i = 0; i < KT; ++i) fetch.next((stage == 0 ? NS : stage) - KT + i, wave, lane);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // s[m][i][r]: product of row row16 of row tile m and key 16 i + 4 quad + r of the tiles.
-  auto products = [&](uint32_t sb, f32x4(&s)[MT][2]) {
-    i32x4 kc[2][DC];
+  // s[n][m][i][r]: product of row row16 of row tile m and key 16 i + 4 quad + r of the n-th of N
+  // tiles. Four 32-feature steps' fragments are in flight at a time, so that the first products
+  // start while the later reads are still on their way.
+  auto products = [&](uint32_t sb, auto& s) {
+    constexpr int N = sizeof(s) / sizeof(f32x4[MT][2]), U = N * DC, DEPTH = 4 < U ? 4 : U;
+    i32x4 kc[U][2];
+    auto request = [&](int u) {
+      kc[u][0] = tk_attn::lds_read_b128<0>(sb + (u / DC) * R::STAGE + ka[u % DC]);
+      kc[u][1] = tk_attn::lds_read_b128<16 * RB>(sb + (u / DC) * R::STAGE + ka[u % DC]);
+    };
 #pragma unroll
-    for (int c = 0; c < DC; ++c) {
-      kc[0][c] = tk_attn::lds_read_b128<0>(sb + ka[c]);
-      kc[1][c] = tk_attn::lds_read_b128<16 * RB>(sb + ka[c]);
+    for (int u = 0; u < DEPTH; ++u) request(u);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int younger = (u + DEPTH < U ? u + DEPTH : U) - (u + 1);
+      if (younger >= 3)
+        tk_attn::wait_lgkm<6>();
+      else if (younger == 2)
+        tk_attn::wait_lgkm<4>();
+      else if (younger == 1)
+        tk_attn::wait_lgkm<2>();
+      else
+        tk_attn::wait_lgkm<0>();
+      tk_attn::pin(kc[u][0]);
+      tk_attn::pin(kc[u][1]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          s[u / DC][m][i] = tk_attn::Mma16<T>::run(
+              kc[u][i], qf[m][u % DC],
+              u % DC == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[u / DC][m][i]);
+      if (u + DEPTH < U) request(u + DEPTH);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    tk_attn::wait_lgkm<0>();
-#pragma unroll
-    for (int c = 0; c < DC; ++c) {
-      tk_attn::pin(kc[0][c]);
-      tk_attn::pin(kc[1][c]);
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < DC; ++c) s[m][i] = tk_attn::Mma16<T>::run(kc[i][c], qf[m][c], s[m][i]);
-      }
   };
   // P = exp2(scale s - top) of N tiles into pf. The reference maximum moves only when the
   // tiles' exceeds it by more than 8 (base 2), so p <= 2^8 and o and sum are rescaled in few
@@ -494,8 +508,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
     if (!busy) continue;
     f32x4 s[KT][MT][2];
     i32x4 pf[KT][MT];
-#pragma unroll
-    for (int n = 0; n < KT; ++n) products(sb + n * R::STAGE, s[n]);
+    products(sb, s);
     request_v(sb, 0);
     const int live = limit - t * kTileKeys;
     if (__builtin_expect(live < KT * kTileKeys, 0)) {
@@ -530,7 +543,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       }
       f32x4 s[1][MT][2];
       i32x4 pf[1][MT];
-      products(sb, s[0]);
+      products(sb, s);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -727,7 +740,7 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, i
   p.row_blocks = tk::cdiv(rows, shape.rows);
   const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
   const int64_t base = shape.resident / (kv_heads * p.row_blocks);
-  p.runs = base > 2 * batch ? base - batch : base > 1 ? base : 1;
+  p.runs = base > 2 * batch ? base - batch + 1 : base > 1 ? base : 1;
   p.combine = most > kMinChunk;
   p.flat = p.runs + batch;
   const int64_t bound = batch * tk::cdiv(most, kMinChunk);
