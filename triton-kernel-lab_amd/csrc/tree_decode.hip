@@ -254,15 +254,21 @@ __device__ __forceinline__ i32x4 only_key(i32x4 f, int j, int quad) {
 template <typename T, int D, int W, int MT, int KT, int NS>
 __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(TreeArgs a) {
   using R = Ring<D>;
-  static_assert(NS % KT == 0 && NS >= 2 * KT, "a step's stages are refilled while the next is read");
+  // Ping-pong (eight waves, two per SIMD): see the context loop.
+  constexpr bool PP = W == 8;
+  constexpr int RS = NS / KT;          // steps the ring holds
+  constexpr int LA = PP ? 2 : RS - 1;  // steps fetched ahead
+  static_assert(NS % KT == 0 && RS >= 2 && (!PP || RS >= 4), "a stage is refilled while it is read");
   constexpr int DC = D / 32, OC = D / 16, RB = R::RB, PER = R::IPT / W;
   // vmcnt is 6 bits: at most 63 DMA instructions may be outstanding.
-  static_assert((NS - KT) * 2 * PER < 64, "ring deeper than the vmcnt counter");
+  constexpr int STEP = KT * 2 * PER;   // this wave's DMA instructions per step
+  static_assert(LA * STEP < 64, "ring deeper than the vmcnt counter");
   constexpr int ROWS = 16 * W * MT;
   constexpr int HB = 4;  // output chunks per batch of V reads
   constexpr int NONFINITE = __is_same(T, __bf16) ? 0x7F80 : 0x7C00;
   __shared__ __attribute__((aligned(1024))) char ring[NS * R::STAGE];
-  __shared__ uint32_t seen[ROWS * kMaskWords];  // drafted keys by the block's nodes
+  // Drafted keys by the block's nodes; behind them the waves' SIMDs.
+  __shared__ uint32_t seen[ROWS * kMaskWords + W];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
     fetch.offsets(wave, lane);
   }
 #pragma unroll
-  for (int i = 0; i < NS - KT; ++i) fetch.next(i, wave, lane);
+  for (int i = 0; i < LA * KT; ++i) fetch.next(i, wave, lane);
 
   // Q^T fragments: row w0 + 16 mt + row16 (zero past the last), dims 32 c + 8 quad .. +7. A
   // negative scale is taken into Q's signs (exact), so that the largest score is the largest
@@ -371,30 +377,38 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   }
   const float scale = a.scale_log2;
 
-  int stage = 0;
-  // A step's tiles have landed (this wave's share) once only the NS - 2 KT younger tiles' loads
-  // are outstanding; behind the barrier every wave's share has, and every wave has read the
-  // stages before it, which the tiles fetched now take.
-  auto arrive = [&]() {
-    tk_attn::wait_vmcnt<(NS - 2 * KT) * 2 * PER>();
-    if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  int step = 0;  // modulo RS, the ring's next step to read
+  auto fetch_step = [&](int slot) {
 #pragma unroll
-    for (int i = 0; i < KT; ++i) fetch.next((stage == 0 ? NS : stage) - KT + i, wave, lane);
+    for (int i = 0; i < KT; ++i) fetch.next(slot * KT + i, wave, lane);
     __builtin_amdgcn_sched_barrier(0);
   };
+  // A step has landed (this wave's share) once only the LA - 1 younger steps' loads are
+  // outstanding; behind the barrier every wave's share has, and every wave has read the step
+  // before it, whose slot (or a free one) the step fetched now takes. Returns the step's stage.
+  auto arrive = [&]() {
+    tk_attn::wait_vmcnt<(LA - 1) * STEP>();
+    if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    fetch_step(step + LA < RS ? step + LA : step + LA - RS);
+    const uint32_t sb = ring_base + step * KT * R::STAGE;
+    step = step == RS - 1 ? 0 : step + 1;
+    return sb;
+  };
   // s[n][m][i][r]: product of row row16 of row tile m and key 16 i + 4 quad + r of the n-th of N
-  // tiles. Four 32-feature steps' fragments are in flight at a time, so that the first products
-  // start while the later reads are still on their way.
-  auto products = [&](uint32_t sb, auto& s) {
-    constexpr int N = sizeof(s) / sizeof(f32x4[MT][2]), U = N * DC, DEPTH = 4 < U ? 4 : U;
-    i32x4 kc[U][2];
-    auto request = [&](int u) {
-      kc[u][0] = tk_attn::lds_read_b128<0>(sb + (u / DC) * R::STAGE + ka[u % DC]);
-      kc[u][1] = tk_attn::lds_read_b128<16 * RB>(sb + (u / DC) * R::STAGE + ka[u % DC]);
-    };
+  // tiles. The fragments of DEPTH 32-feature steps are in flight at a time, so that the first
+  // products start while the later reads are still on their way.
+  constexpr int DEPTH = 4 < DC ? 4 : DC;
+  auto request_k = [&](uint32_t sb, auto& kc, int u) {
+    kc[u][0] = tk_attn::lds_read_b128<0>(sb + (u / DC) * R::STAGE + ka[u % DC]);
+    kc[u][1] = tk_attn::lds_read_b128<16 * RB>(sb + (u / DC) * R::STAGE + ka[u % DC]);
+  };
+  auto request_first_k = [&](uint32_t sb, auto& kc) {
 #pragma unroll
-    for (int u = 0; u < DEPTH; ++u) request(u);
+    for (int u = 0; u < DEPTH; ++u) request_k(sb, kc, u);
     __builtin_amdgcn_sched_barrier(0);
+  };
+  auto products = [&](uint32_t sb, auto& kc, auto& s) {
+    constexpr int U = sizeof(kc) / sizeof(kc[0]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int younger = (u + DEPTH < U ? u + DEPTH : U) - (u + 1);
@@ -415,7 +429,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
           s[u / DC][m][i] = tk_attn::Mma16<T>::run(
               kc[u][i], qf[m][u % DC],
               u % DC == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[u / DC][m][i]);
-      if (u + DEPTH < U) request(u + DEPTH);
+      if (u + DEPTH < U) request_k(sb, kc, u + DEPTH);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -469,8 +483,8 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       for (int n = 0; n < N; ++n) pf[n][m] = tk_attn::acc_frag2<T>(p[n][0], p[n][1]);
     }
   };
-  // o += V^T P^T of a tile; the first batch of its V fragments is already on its way, and that
-  // of the tile at `after` (none: 0) is sent for at the end.
+  // o += V^T P^T of a tile; the first batch of its V fragments is already on its way, and what
+  // comes next is sent for before the last batch's products.
   i32x2 lo[OC], hi[OC];
   auto request_v = [&](uint32_t sb, int c0) {
 #pragma unroll
@@ -479,7 +493,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       hi[c] = tk_attn::lds_read_tr16<16 * RB>(sb + va[c]);
     }
   };
-  auto accumulate = [&](uint32_t sb, const i32x4(&pf)[MT], uint32_t after) {
+  auto accumulate = [&](uint32_t sb, const i32x4(&pf)[MT], auto&& request_next) {
 #pragma unroll
     for (int c0 = 0; c0 < OC; c0 += HB) {
       tk_attn::wait_lgkm<0>();
@@ -491,8 +505,9 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       }
       if (c0 + HB < OC)
         request_v(sb, c0 + HB);
-      else if (after != 0)
-        request_v(after, 0);
+      else
+        request_next();
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < HB; ++c)
 #pragma unroll
@@ -500,16 +515,17 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
           o[m][c0 + c] = tk_attn::Mma16<T>::run(vf[c], pf[m], o[m][c0 + c]);
     }
   };
-
-  for (int t = t0; t < c1; t += KT) {
-    arrive();
-    const uint32_t sb = ring_base + stage * R::STAGE;
-    stage = stage == NS - KT ? 0 : stage + KT;
-    if (!busy) continue;
-    f32x4 s[KT][MT][2];
-    i32x4 pf[KT][MT];
-    products(sb, s);
-    request_v(sb, 0);
+  auto accumulate_step = [&](uint32_t sb, const i32x4(&pf)[KT][MT], auto&& request_next) {
+    if constexpr (KT == 2) {
+      accumulate(sb, pf[0], [&]() { request_v(sb + R::STAGE, 0); });
+      accumulate(sb + R::STAGE, pf[1], request_next);
+    } else {
+      accumulate(sb, pf[0], request_next);
+    }
+  };
+  auto nothing = []() {};
+  // The keys past the run's context in the step from tile t on are no keys.
+  auto cut = [&](int t, f32x4(&s)[KT][MT][2]) {
     const int live = limit - t * kTileKeys;
     if (__builtin_expect(live < KT * kTileKeys, 0)) {
 #pragma unroll
@@ -522,16 +538,94 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
             for (int r = 0; r < 4; ++r)
               if (32 * n + 16 * i + 4 * quad + r >= live) s[n][m][i][r] = -INFINITY;
     }
-    softmax(s, pf);
+  };
+
+  if constexpr (!PP) {
+    for (int t = t0; t < c1; t += KT) {
+      const uint32_t sb = arrive();
+      if (!busy) continue;
+      f32x4 s[KT][MT][2];
+      i32x4 pf[KT][MT], kc[KT * DC][2];
+      request_first_k(sb, kc);
+      products(sb, kc, s);
+      request_v(sb, 0);
+      cut(t, s);
+      softmax(s, pf);
+      accumulate_step(sb, pf, nothing);
+    }
+  } else if (c1 > t0) {
+    // Eight waves, two per SIMD, in phases ended by barriers: a wave alternates a matrix phase
+    // (step j - 1's output products, then step j's scores) with a softmax phase, the second wave
+    // of each SIMD (by the hardware's SIMD id) one phase behind the first, so that one wave's
+    // exponentials run beside the other's products. Step j's slot is read in phases 2j .. 2j + 3;
+    // step j + 2, fetched from phase 2j on, takes the slot of step j - 2. Waves without rows run
+    // along on zeros.
+    const int steps = (c1 - t0 + KT - 1) / KT;
+    int second = 0;
+    {
+      int* simd = reinterpret_cast<int*>(&seen[ROWS * kMaskWords]);
+      if (lane == 0) simd[wave] = tk_attn::simd_id();
+      tk_attn::wait_vmcnt<STEP>();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int n = 0; n < KT; ++n)
-      accumulate(sb + n * R::STAGE, pf[n], n + 1 < KT ? sb + (n + 1) * R::STAGE : 0);
+      for (int w = 0; w < W; ++w) second += w < wave && simd[w] == simd[wave] ? 1 : 0;
+      second = __builtin_amdgcn_readfirstlane(second) & 1;
+    }
+    f32x4 s[KT][MT][2];
+    i32x4 pf[KT][MT];
+    auto stage_of = [&](int j) { return ring_base + (j % RS) * KT * R::STAGE; };
+    // Step j + 2 is fetched from phase 2j on, and step j + 1 has landed by the end of phase 2j + 1.
+    auto matrix_end = [&](int j) {
+#pragma unroll
+      for (int n = 0; n < KT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          tk_attn::pin(s[n][m][0]);
+          tk_attn::pin(s[n][m][1]);
+        }
+      if (second) tk_attn::wait_vmcnt<STEP>();
+      tk_attn::barrier_no_fence();
+      if (second && j + 1 < steps) fetch_step((j + 3) % RS);
+    };
+    auto softmax_phase = [&](int j) {
+      cut(t0 + j * KT, s);
+      softmax(s, pf);
+#pragma unroll
+      for (int n = 0; n < KT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) tk_attn::pin(pf[n][m]);
+      if (!second) tk_attn::wait_vmcnt<STEP>();
+      tk_attn::barrier_no_fence();
+      if (!second && j + 1 < steps) fetch_step((j + 3) % RS);
+    };
+    fetch_step(2 % RS);
+    if (second) tk_attn::barrier_no_fence();
+    {
+      i32x4 kc[KT * DC][2];
+      request_first_k(stage_of(0), kc);
+      products(stage_of(0), kc, s);
+    }
+    matrix_end(0);
+    softmax_phase(0);
+    for (int j = 1; j < steps; ++j) {
+      i32x4 kc[KT * DC][2];
+      const uint32_t now = stage_of(j), last = stage_of(j + RS - 1);
+      request_v(last, 0);
+      accumulate_step(last, pf, [&]() { request_first_k(now, kc); });
+      products(now, kc, s);
+      matrix_end(j);
+      softmax_phase(j);
+    }
+    request_v(stage_of(steps - 1), 0);
+    accumulate_step(stage_of(steps - 1), pf, nothing);
+    // Both waves of a SIMD have passed 2 steps + 2 barriers, so the ring is read by none.
+    tk_attn::barrier_no_fence();
+    if (!second) tk_attn::barrier_no_fence();
+    step = steps % RS;
   }
 
   for (int t = max(t0, context_tiles); t < t1; t += KT) {
-    arrive();
-    uint32_t sb = ring_base + stage * R::STAGE;
-    stage = stage == NS - KT ? 0 : stage + KT;
+    uint32_t sb = arrive();
     if (!busy) continue;
     for (int tile = t; tile < min(t + KT, t1); ++tile, sb += R::STAGE) {
       const int word = tile - context_tiles;
@@ -542,8 +636,9 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
         bits[m] = r < a.rows ? seen[(r / a.group - node0) * kMaskWords + word] : 0;
       }
       f32x4 s[1][MT][2];
-      i32x4 pf[1][MT];
-      products(sb, s);
+      i32x4 pf[1][MT], kc[DC][2];
+      request_first_k(sb, kc);
+      products(sb, kc, s);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -569,7 +664,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       }
       if (__builtin_expect(__ballot(most[0] >= NONFINITE || most[1] >= NONFINITE) == 0, 1)) {
         request_v(sb, 0);
-        accumulate(sb, pf[0], 0);
+        accumulate(sb, pf[0], nothing);
         continue;
       }
       for (int j = 0; j < kTileKeys; ++j) {
