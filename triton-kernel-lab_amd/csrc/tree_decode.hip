@@ -57,6 +57,7 @@ struct TreeArgs {
   int64_t ktb, kth, ktl, vtb, vth, vtl;
   int64_t mb, mt;
   int batch, q_heads, kv_heads, group, nodes, rows, max_len;
+  tk::FastDiv by_group, by_kv_heads, by_row_blocks;
   int tree_tiles, min_chunk, runs, row_blocks, flat;  // flat: upper bound on the flat splits
   float scale_log2;  // positive
   int flip;          // Q's sign bits to turn (a negative scale)
@@ -70,13 +71,19 @@ __device__ __forceinline__ int context_length(const TreeArgs& a, int b) {
   return min(max(n, 0), a.max_len);
 }
 
-// Sum over lane and prefix of it, by one wave.
-__device__ __forceinline__ int wave_prefix(int v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(v, d);
-    if (lane >= d) v += up;
-  }
+// Inclusive prefix sums over the wave's lanes: within rows of 16 lanes by shifts, then the rows'
+// and the halves' last sums broadcast to the next ones.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_part(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += dpp_part<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v += dpp_part<0x112, 0xF>(v);
+  v += dpp_part<0x114, 0xF>(v);
+  v += dpp_part<0x118, 0xF>(v);
+  v += dpp_part<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp_part<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
@@ -94,7 +101,7 @@ __device__ __forceinline__ Lengths read_lengths(const TreeArgs& a, int lane) {
   r.first = lane < a.batch ? context_length(a, lane) : 0;
   int sum = lane < a.batch ? tiles_of(a, r.first) : 0;
   for (int b = lane + 64; b < a.batch; b += 64) sum += tiles_of(a, context_length(a, b));
-  const int total = __builtin_amdgcn_readlane(wave_prefix(sum, lane), 63);
+  const int total = __builtin_amdgcn_readlane(wave_prefix(sum), 63);
   r.chunk = max(a.min_chunk, (total + a.runs - 1) / a.runs);
   return r;
 }
@@ -111,7 +118,7 @@ __device__ __forceinline__ bool find_run(const TreeArgs& a, const Lengths& n, in
     const int b = b0 + lane;
     const int len = b0 == 0 ? n.first : (b < a.batch ? context_length(a, b) : 0);
     const int mine = b < a.batch ? (tiles_of(a, len) + n.chunk - 1) / n.chunk : 0;
-    const int upto = before + wave_prefix(mine, lane);
+    const int upto = before + wave_prefix(mine);
     const uint64_t hit = __ballot(upto > f);
     if (hit != 0) {
       const int at = __builtin_ctzll(hit);
@@ -135,7 +142,7 @@ __device__ __forceinline__ void sequence_runs(const TreeArgs& a, const Lengths& 
     const int i = b0 + lane;
     const int len = b0 == 0 ? n.first : (i < a.batch ? context_length(a, i) : 0);
     const int mine = i < a.batch ? (tiles_of(a, len) + n.chunk - 1) / n.chunk : 0;
-    const int upto = before + wave_prefix(mine, lane);
+    const int upto = before + wave_prefix(mine);
     if (b < b0 + 64) {
       out.splits = __builtin_amdgcn_readlane(mine, b - b0);
       out.flat0 = __builtin_amdgcn_readlane(upto, b - b0) - out.splits;
@@ -274,9 +281,10 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroup -> (flat split, KV head, row block): the row blocks of a run are dealt to one XCD
   // (workgroup index modulo 8), one after the other, so that they share its L2.
-  const int pair = (blockIdx.x / (8 * a.row_blocks)) * 8 + blockIdx.x % 8;
-  const int rb = (blockIdx.x / 8) % a.row_blocks;
-  const int f = pair / a.kv_heads;
+  const int eighth = a.by_row_blocks.div(blockIdx.x / 8);
+  const int pair = eighth * 8 + blockIdx.x % 8;
+  const int rb = blockIdx.x / 8 - eighth * a.row_blocks;
+  const int f = a.by_kv_heads.div(pair);
   const int kvh = pair - f * a.kv_heads;
   const Lengths lengths = read_lengths(a, lane);
   Run run;
@@ -294,7 +302,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   const int r0 = rb * ROWS;
   const int w0 = r0 + wave * 16 * MT;   // this wave's first row
   const bool busy = w0 < a.rows;        // waves past the last row only fetch
-  const int node0 = r0 / a.group;
+  const int node0 = a.by_group.div(r0);
 
   Fetcher<T, D, W> fetch;
   {
@@ -329,12 +337,36 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int r = w0 + 16 * m + row16;
-    const int node = r / a.group;
+    const int node = a.by_group.div(r);
     const int h = kvh * a.group + (r - node * a.group);
     const T* p = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + node * a.qt + 8 * quad;
 #pragma unroll
     for (int c = 0; c < DC; ++c)
       qf[m][c] = r < a.rows ? *reinterpret_cast<const i32x4*>(p + 32 * c) : i32x4{0, 0, 0, 0};
+  }
+  // The block's nodes' mask rows as bits, if the run holds drafted tiles; eight rows of a wave
+  // are requested at a time.
+  if (t1 > context_tiles) {
+    const int last = a.by_group.div(min(r0 + ROWS, a.rows) - 1);
+    const uint8_t* mask = a.mask + b * a.mb;
+    for (int j0 = 0; j0 < a.nodes; j0 += 64) {
+      const int j = j0 + lane;
+      for (int n0 = node0 + wave; n0 <= last; n0 += 8 * W) {
+        uint8_t byte[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int n = n0 + i * W;
+          byte[i] = j < a.nodes && n <= last ? mask[n * a.mt + j] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int n = n0 + i * W;
+          const uint64_t bits = __ballot(byte[i] != 0);
+          if (lane < 2 && n <= last)
+            seen[(n - node0) * kMaskWords + j0 / 32 + lane] = uint32_t(bits >> (32 * lane));
+        }
+      }
+    }
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -343,19 +375,6 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       qf[m][c] ^= a.flip;
       tk_attn::pin(qf[m][c]);
     }
-
-  // The block's nodes' mask rows as bits, if the run holds drafted tiles.
-  if (t1 > context_tiles) {
-    const int last = min((min(r0 + ROWS, a.rows) - 1) / a.group, a.nodes - 1);
-    const uint8_t* mask = a.mask + b * a.mb;
-    for (int n = node0 + wave; n <= last; n += W)
-      for (int j0 = 0; j0 < a.nodes; j0 += 64) {
-        const int j = j0 + lane;
-        const uint64_t bits = __ballot(j < a.nodes && mask[n * a.mt + j] != 0);
-        if (lane < 2 && j0 / 32 + lane < kMaskWords)
-          seen[(n - node0) * kMaskWords + j0 / 32 + lane] = uint32_t(bits >> (32 * lane));
-      }
-  }
 
   const uint32_t ring_base = (uint32_t)(uintptr_t)(tk_attn::lds_void*)ring;
   uint32_t ka[DC], va[OC];
@@ -633,7 +652,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int r = w0 + 16 * m + row16;
-        bits[m] = r < a.rows ? seen[(r / a.group - node0) * kMaskWords + word] : 0;
+        bits[m] = r < a.rows ? seen[(a.by_group.div(r) - node0) * kMaskWords + word] : 0;
       }
       f32x4 s[1][MT][2];
       i32x4 pf[1][MT], kc[DC][2];
@@ -694,7 +713,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
     const int r = w0 + 16 * m + row16;
     if (r >= a.rows) continue;
     if (run.splits == 1) {
-      const int node = r / a.group;
+      const int node = a.by_group.div(r);
       const int h = kvh * a.group + (r - node * a.group);
       const float share = l == 0.f ? 0.f : 1.f / l;
       T* dst = static_cast<T*>(a.o) + b * a.ob + h * a.oh + node * a.ot + 4 * quad;
@@ -755,7 +774,7 @@ __global__ __launch_bounds__(64 * kCombineWaves) void tree_combine_kernel(TreeAr
     for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], x);
   }
   if (part != 0) return;
-  const int node = r / a.group;
+  const int node = a.by_group.div(r);
   const int h = kvh * a.group + (r - node * a.group);
   float out[4];
 #pragma unroll
@@ -929,6 +948,9 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
   a.min_chunk = kMinChunk;
   a.runs = static_cast<int>(plan.runs);
   a.row_blocks = static_cast<int>(plan.row_blocks);
+  a.by_group = tk::FastDiv(static_cast<uint32_t>(group));
+  a.by_kv_heads = tk::FastDiv(static_cast<uint32_t>(kv_heads));
+  a.by_row_blocks = tk::FastDiv(static_cast<uint32_t>(plan.row_blocks));
   a.flat = static_cast<int>(plan.flat);
   // Not 0, which would turn a masked score (-inf) into NaN: 1e-30 leaves no score above 2^-20.
   a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
