@@ -838,13 +838,19 @@ void launch(const TreeArgs& a, bool combine, hipStream_t s) {
                        dim3(64 * kCombineWaves), 0, s, a);
 }
 
-constexpr int kMinChunk = 4;  // tiles
+// Tiles of the shortest run.
+constexpr int kMinChunk = 4;
+// A call of at most this many tiles per sequence is not split: writing and joining partial results
+// costs more than the tiles that runs of their own would save (a tile takes a workgroup about
+// 0.75 us; joining 5 us, and 10 us where there is a pair for every other CU and with it 8 MB of
+// partial results and more).
+int64_t whole_tiles(int64_t pairs) { return pairs >= 128 ? 20 : 8; }
 
 // How the call is cut: runs (the tiles of all sequences over `runs` give the run length), the
 // bound on their number, row blocks. The sequences' last runs are shorter, so `runs` leaves room
 // for one more per sequence where that keeps the launch to one round of workgroups.
 struct Plan {
-  int64_t row_blocks, runs, flat;
+  int64_t row_blocks, runs, flat, min_chunk;
   bool combine;
 };
 Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, int64_t nodes,
@@ -855,9 +861,11 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, i
   const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
   const int64_t base = shape.resident / (kv_heads * p.row_blocks);
   p.runs = base > 2 * batch ? base - batch + 1 : base > 1 ? base : 1;
-  p.combine = most > kMinChunk;
+  const int64_t whole = whole_tiles(batch * kv_heads * p.row_blocks);
+  p.combine = most > whole;
+  p.min_chunk = p.combine ? kMinChunk : whole;
   p.flat = p.runs + batch;
-  const int64_t bound = batch * tk::cdiv(most, kMinChunk);
+  const int64_t bound = batch * tk::cdiv(most, p.min_chunk);
   if (p.flat > bound) p.flat = bound;
   return p;
 }
@@ -945,7 +953,7 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
   a.rows = static_cast<int>(rows);
   a.max_len = static_cast<int>(max_len);
   a.tree_tiles = static_cast<int>(tk::cdiv(nodes, kTileKeys));
-  a.min_chunk = kMinChunk;
+  a.min_chunk = static_cast<int>(plan.min_chunk);
   a.runs = static_cast<int>(plan.runs);
   a.row_blocks = static_cast<int>(plan.row_blocks);
   a.by_group = tk::FastDiv(static_cast<uint32_t>(group));
