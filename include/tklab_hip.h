@@ -427,8 +427,8 @@ int tk_rotary(int dtype, const void* q, void* q_out, const void* k, void* k_out,
 /* Attention of drafted tokens over a KV cache and each other: query row (b, h, t) sees the first
  * clamp(seqlens[b], 0, max_len) cache keys of KV head h / (q_heads / kv_heads) (all max_len when
  * `seqlens` is NULL) and the drafted keys j < nodes with mask[b][t][j] != 0 (bytes; strides
- * {batch, row}, unit-stride entries). o in the storage dtype, lse float32 [batch][q_heads][nodes],
- * base 2; a row that sees nothing gets 0 and -inf. A key that a row does not see does not reach
+ * {batch, row}, unit-stride entries). o in the storage dtype, `lse` (nullable) float32
+ * [batch][q_heads][nodes], base 2; a row that sees nothing gets 0 and -inf. A key that a row does not see does not reach
  * it, infinities and NaN included. Strides {batch, head, position} in elements, multiples of 8,
  * key strides below 2^24, bases 16-byte aligned; dtype F16 or BF16, head_dim 64 or 128, nodes <=
  * 256. `workspace`: tk_tree_decode_slots(...) * nodes * (q_heads / kv_heads) * (head_dim + 2)

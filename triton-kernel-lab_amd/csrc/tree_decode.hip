@@ -724,7 +724,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
         for (int i = 0; i < 4; ++i) out[i] = o[m][c][i] * share;
         tk::store_vec<T, 4>(dst + 16 * c, out);
       }
-      if (quad == 0)
+      if (quad == 0 && a.lse != nullptr)
         a.lse[(int64_t(b) * a.q_heads + h) * a.nodes + node] =
             l == 0.f ? -INFINITY : top[m] + log2f(l);
     } else {
@@ -780,7 +780,7 @@ __global__ __launch_bounds__(64 * kCombineWaves) void tree_combine_kernel(TreeAr
 #pragma unroll
   for (int i = 0; i < 4; ++i) out[i] = total == 0.f ? 0.f : acc[i] / total;
   tk::store_vec<T, 4>(static_cast<T*>(a.o) + b * a.ob + h * a.oh + node * a.ot + d, out);
-  if (lane == 0)
+  if (lane == 0 && a.lse != nullptr)
     a.lse[(int64_t(b) * a.q_heads + h) * a.nodes + node] =
         total == 0.f ? -INFINITY : high + log2f(total);
 }
@@ -893,7 +893,7 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
   if (dtype != TK_DTYPE_F16 && dtype != TK_DTYPE_BF16)
     return tk::fail("tree decode: dtype must be float16 or bfloat16");
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || k_tree == nullptr ||
-      v_tree == nullptr || mask == nullptr || o == nullptr || lse == nullptr ||
+      v_tree == nullptr || mask == nullptr || o == nullptr ||
       q_strides == nullptr || k_strides == nullptr || v_strides == nullptr ||
       k_tree_strides == nullptr || v_tree_strides == nullptr || mask_strides == nullptr ||
       o_strides == nullptr)

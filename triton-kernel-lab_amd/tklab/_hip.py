@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -200,6 +201,14 @@ def int64_array(values: tuple[int, ...] | list[int]) -> ctypes.Array[ctypes.c_in
     return (_INT64_ARRAYS[n] if n < 5 else ctypes.c_int64 * n)(*values)
 
 
+_PACKERS = tuple(struct.Struct(f"{n}q").pack for n in range(5))
+
+
+def int64_bytes(values: tuple[int, ...]) -> bytes:
+    """Up to four integers as a C ``int64_t[]`` (a third of :func:`int64_array`'s time)."""
+    return _PACKERS[len(values)](*values)
+
+
 _bound: dict[str, ctypes._CFuncPtr] = {}
 
 
@@ -209,7 +218,8 @@ def _function(name: str) -> ctypes._CFuncPtr:
     if fn is None:
         fn = getattr(load_library(), name)
         fn.restype = ctypes.c_int
-        fn.argtypes = _SIGNATURES[name]
+        # Untyped pointers take arrays (int64_array) and packed integers (int64_bytes) alike.
+        fn.argtypes = [_P if kind is _I64P else kind for kind in _SIGNATURES[name]]
         _bound[name] = fn
     return fn
 
@@ -224,11 +234,24 @@ def call(name: str, *args: object) -> None:
 
 def call_on(tensor: torch.Tensor, name: str, *args: object) -> None:
     """:func:`call` with ``tensor``'s device current, whichever device the caller has selected."""
-    if tensor.get_device() == torch.cuda.current_device():
+    if tensor.get_device() == torch._C._cuda_getDevice():
         call(name, *args)
         return
     with torch.cuda.device(tensor.device):
         call(name, *args)
+
+
+def row_layout(tensor: torch.Tensor, name: str, device: int) -> tuple[int, bytes]:
+    """Address and packed leading strides of a 4-D 16-bit tensor on GPU ``device``, whose rows must
+    be unit-stride and 16-byte aligned (``ValueError`` otherwise)."""
+    address, strides = tensor.data_ptr(), tensor.stride()
+    if tensor.get_device() != device:
+        raise ValueError(f"{name} must be on the other tensors' device")
+    if strides[3] != 1:
+        raise ValueError(f"{name} requires a contiguous final dimension")
+    if (strides[0] | strides[1] | strides[2]) & 7 or address & 15:
+        raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of 8)")
+    return address, _PACKERS[3](strides[0], strides[1], strides[2])
 
 
 def query(name: str, *args: int | None) -> int:

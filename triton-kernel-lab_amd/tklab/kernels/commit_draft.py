@@ -48,15 +48,20 @@ def commit_draft(
     """
     _validate(k_cache, v_cache, cache_seqlens, k_tree, v_tree, path, count)
     batch, kv_heads, max_len, head_dim = k_cache.shape
+    device = k_cache.get_device()
+    k_ptr, k_strides = _hip.row_layout(k_cache, "k_cache", device)
+    v_ptr, v_strides = _hip.row_layout(v_cache, "v_cache", device)
+    kt_ptr, kt_strides = _hip.row_layout(k_tree, "k_tree", device)
+    vt_ptr, vt_strides = _hip.row_layout(v_tree, "v_tree", device)
     lengths = torch.empty_like(cache_seqlens)
     _hip.call_on(
         k_cache,
         "tk_commit_draft",
-        _hip.dtype_code(k_cache.dtype),
-        k_cache.data_ptr(),
-        v_cache.data_ptr(),
-        k_tree.data_ptr(),
-        v_tree.data_ptr(),
+        _hip.DTYPE_CODES[k_cache.dtype],
+        k_ptr,
+        v_ptr,
+        kt_ptr,
+        vt_ptr,
         cache_seqlens.data_ptr(),
         path.data_ptr(),
         count.data_ptr(),
@@ -66,10 +71,10 @@ def commit_draft(
         max_len,
         k_tree.shape[2],
         head_dim,
-        _hip.int64_array(k_cache.stride()[:3]),
-        _hip.int64_array(v_cache.stride()[:3]),
-        _hip.int64_array(k_tree.stride()[:3]),
-        _hip.int64_array(v_tree.stride()[:3]),
+        k_strides,
+        v_strides,
+        kt_strides,
+        vt_strides,
         _hip.stream_of(k_cache),
     )
     return lengths
@@ -84,17 +89,18 @@ def _validate(
     path: torch.Tensor,
     count: torch.Tensor,
 ) -> None:
-    """Check the contract."""
-    if k_cache.ndim != 4 or k_tree.ndim != 4:
+    """Check the contract, up to the rows' layout."""
+    cache_shape, tree_shape = k_cache.shape, k_tree.shape
+    if len(cache_shape) != 4 or len(tree_shape) != 4:
         raise ValueError("commit_draft expects caches [batch, kv_heads, max_len, head_dim] and "
                          "drafted keys and values [batch, kv_heads, nodes, head_dim]")
-    if v_cache.shape != k_cache.shape or v_tree.shape != k_tree.shape:
+    if v_cache.shape != cache_shape or v_tree.shape != tree_shape:
         raise ValueError("keys and values must have identical shapes")
-    batch, kv_heads, max_len, head_dim = k_cache.shape
-    nodes = k_tree.shape[2]
-    if (k_tree.shape[0], k_tree.shape[1], k_tree.shape[3]) != (batch, kv_heads, head_dim):
+    batch, kv_heads, max_len, head_dim = cache_shape
+    tree_batch, tree_heads, nodes, tree_dim = tree_shape
+    if tree_batch != batch or tree_heads != kv_heads or tree_dim != head_dim:
         raise ValueError("the caches and the drafted keys disagree on batch, kv_heads or head_dim")
-    if k_cache.numel() == 0 or k_tree.numel() == 0:
+    if not (batch and kv_heads and max_len and nodes and head_dim):
         raise ValueError("commit_draft does not support empty dimensions")
     if nodes > _MAX_NODES or batch > 65535 or kv_heads > 65535 or head_dim > 65535:
         raise ValueError("commit_draft supports at most 65535 nodes, sequences, heads and features")
@@ -102,26 +108,20 @@ def _validate(
         raise ValueError("commit_draft supports caches below 2**30 positions")
     if head_dim % 8:
         raise ValueError("commit_draft requires a head_dim that is a multiple of 8")
-    if k_cache.dtype not in _DTYPES or any(
-            t.dtype != k_cache.dtype for t in (v_cache, k_tree, v_tree)):
+    dtype = k_cache.dtype
+    if dtype not in _DTYPES or not dtype == v_cache.dtype == k_tree.dtype == v_tree.dtype:
         raise ValueError("caches and drafted keys and values must share a float16 or bfloat16 "
                          "dtype")
-    if k_cache.device.type != "cuda":
+    if not k_cache.is_cuda:
         raise ValueError("commit_draft requires CUDA (ROCm/HIP) tensors")
-    for name, tensor in (("k_cache", k_cache), ("v_cache", v_cache), ("k_tree", k_tree),
-                         ("v_tree", v_tree)):
-        if tensor.device != k_cache.device:
-            raise ValueError(f"{name} must be on the caches' device")
-        if tensor.stride(-1) != 1:
-            raise ValueError(f"{name} requires a contiguous final dimension")
-        if tensor.data_ptr() % 16 or any(s % 8 or s < 0 for s in tensor.stride()[:3]):
-            raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of 8)")
+    device = k_cache.get_device()
     for name, tensor in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if any(s == 0 and n > 1 for s, n in zip(tensor.stride(), tensor.shape)):
+        strides = tensor.stride()
+        if 0 in strides and any(strides[d] == 0 and cache_shape[d] > 1 for d in range(3)):
             raise ValueError(f"{name} is written: its rows may not share memory")
     for name, tensor, shape in (("cache_seqlens", cache_seqlens, (batch,)),
                                 ("count", count, (batch,)), ("path", path, (batch, nodes))):
-        if (tuple(tensor.shape) != shape or tensor.dtype != torch.int32
-                or tensor.device != k_cache.device or not tensor.is_contiguous()):
+        if (tensor.shape != shape or tensor.dtype != torch.int32
+                or tensor.get_device() != device or not tensor.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor on the "
                              "caches' device")

@@ -167,32 +167,44 @@ def _launch(
     inverse: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Allocate the outputs and enqueue the rotation of tensors already checked."""
-    q_out = _output(q)
-    k_out = None if k is None else _output(k)
-    packed = q.ndim == 3
-    tokens = q.shape[0] if packed else q.shape[2]
-    position_strides = positions.stride() if positions.ndim == 2 else (0, positions.stride(0))
+    q_out = torch.empty_like(q)
+    q_strides, q_out_strides = q.stride(), q_out.stride()
+    if q_out_strides[-1] != 1:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out_strides = q_out.stride()
+    shape, position_strides = q.shape, positions.stride()
+    packed = len(shape) == 3
+    if k is None:
+        k_out = k_ptr = k_out_ptr = k_table = k_out_table = None
+        kv_heads = 0
+    else:
+        k_out = torch.empty_like(k)
+        if k_out.stride(-1) != 1:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        kv_heads, k_ptr, k_out_ptr = k.shape[1], k.data_ptr(), k_out.data_ptr()
+        k_table, k_out_table = _strides(k.stride(), packed), _strides(k_out.stride(), packed)
     _hip.call_on(
         q,
         "tk_rotary",
-        _hip.dtype_code(q.dtype),
+        _hip.DTYPE_CODES[q.dtype],
         q.data_ptr(),
         q_out.data_ptr(),
-        _hip.ptr(k),
-        _hip.ptr(k_out),
+        k_ptr,
+        k_out_ptr,
         positions.data_ptr(),
         frequencies.data_ptr(),
-        1 if packed else q.shape[0],
-        tokens,
-        q.shape[1],
-        0 if k is None else k.shape[1],
-        q.shape[-1],
+        1 if packed else shape[0],
+        shape[0] if packed else shape[2],
+        shape[1],
+        kv_heads,
+        shape[-1],
         2 * frequencies.shape[0],
-        _strides(q),
-        _strides(q_out),
-        None if k is None else _strides(k),
-        None if k_out is None else _strides(k_out),
-        _hip.int64_array(position_strides),
+        _strides(q_strides, packed),
+        _strides(q_out_strides, packed),
+        k_table,
+        k_out_table,
+        _hip.int64_bytes(position_strides if len(position_strides) == 2
+                         else (0, position_strides[0])),
         magnitude,
         int(interleaved),
         int(positions.dtype == torch.int64),
@@ -202,18 +214,9 @@ def _launch(
     return q_out, k_out
 
 
-def _output(x: torch.Tensor) -> torch.Tensor:
-    """A tensor like ``x`` in its memory order, rows unit-stride and no element shared."""
-    out = torch.empty_like(x, requires_grad=False)
-    if out.stride(-1) != 1:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    return out
-
-
-def _strides(x: torch.Tensor) -> Any:
+def _strides(strides: tuple[int, ...], packed: bool) -> bytes:
     """``{batch, head, token}`` strides."""
-    s = x.stride()
-    return _hip.int64_array((0, s[1], s[0]) if x.ndim == 3 else s[:3])
+    return _hip.int64_bytes((0, strides[1], strides[0]) if packed else strides[:3])
 
 
 def _validate(
@@ -223,41 +226,45 @@ def _validate(
     frequencies: torch.Tensor,
 ) -> None:
     """Check the rotation's contract."""
-    if q.ndim not in (3, 4):
+    shape, dtype = q.shape, q.dtype
+    rank = len(shape)
+    if rank != 3 and rank != 4:
         raise ValueError("rotary_embedding expects q [batch, heads, tokens, head_dim] or packed "
                          "[tokens, heads, head_dim]")
-    if q.numel() == 0:
+    if 0 in shape:
         raise ValueError("rotary_embedding does not support empty dimensions")
     if k is not None:
-        if k.ndim != q.ndim:
+        k_shape = k.shape
+        if len(k_shape) != rank:
             raise ValueError("q and k must both be packed or both be batched")
-        if k.numel() == 0:
+        if 0 in k_shape:
             raise ValueError("rotary_embedding does not support empty dimensions")
-        other = [d for d in range(q.ndim) if d != 1]
-        if any(k.shape[d] != q.shape[d] for d in other):
+        if k_shape[0] != shape[0] or k_shape[2:] != shape[2:]:
             raise ValueError("q and k may differ only in their head counts")
-        if k.dtype != q.dtype or k.device != q.device:
+        if k.dtype != dtype or k.device != q.device:
             raise ValueError("q and k must share a dtype and a device")
-    if q.dtype not in _DTYPES:
+    if dtype not in _DTYPES:
         raise ValueError("rotary_embedding supports float16, bfloat16 and float32 tensors")
-    tokens = q.shape[0] if q.ndim == 3 else q.shape[2]
-    shapes = [(tokens,)] if q.ndim == 3 else [(tokens,), (q.shape[0], tokens)]
-    if tuple(positions.shape) not in shapes:
-        raise ValueError("positions must be [tokens]" + (" or [batch, tokens]" * (q.ndim == 4)))
+    wanted, given = (shape[0] if rank == 3 else shape[2],), positions.shape
+    if given != wanted and (rank == 3 or given != (shape[0], *wanted)):
+        raise ValueError("positions must be [tokens]" + (" or [batch, tokens]" * (rank == 4)))
     if positions.dtype not in _POSITION_DTYPES:
         raise ValueError("positions must be int32 or int64")
-    if frequencies.ndim != 1 or frequencies.dtype != torch.float64:
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
         raise ValueError("frequencies must be a float64 [rotary_dim // 2] tensor")
-    if frequencies.numel() == 0 or 2 * frequencies.numel() > q.shape[-1]:
+    pairs = frequencies.shape[0]
+    if pairs == 0 or 2 * pairs > shape[-1]:
         raise ValueError("frequencies must cover at least one pair and at most head_dim features")
-    if frequencies.stride(0) != 1:
+    if pairs > 1 and frequencies.stride(0) != 1:
         raise ValueError("frequencies must be contiguous")
-    if q.shape[-1] > _MAX_HEAD_DIM:
+    if shape[-1] > _MAX_HEAD_DIM:
         raise ValueError(f"rotary_embedding supports head_dim up to {_MAX_HEAD_DIM}")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise ValueError("rotary_embedding requires CUDA (ROCm/HIP) tensors")
-    if positions.device != q.device or frequencies.device != q.device:
+    device = q.get_device()
+    if positions.get_device() != device or frequencies.get_device() != device:
         raise ValueError("q, positions and frequencies must be on one device")
-    for name, tensor in (("q", q), ("k", k)):
-        if tensor is not None and tensor.stride(-1) != 1:
-            raise ValueError(f"{name} requires a contiguous final dimension")
+    if q.stride(-1) != 1:
+        raise ValueError("q requires a contiguous final dimension")
+    if k is not None and k.stride(-1) != 1:
+        raise ValueError("k requires a contiguous final dimension")

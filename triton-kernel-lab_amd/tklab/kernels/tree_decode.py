@@ -13,6 +13,8 @@ only: there is no autograd.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from tklab import _hip
@@ -79,49 +81,66 @@ def tree_decode(
     """
     _validate(q, k_cache, v_cache, k_tree, v_tree, mask, cache_seqlens)
     batch, q_heads, nodes, head_dim = q.shape
-    kv_heads, max_len = k_cache.shape[1], k_cache.shape[2]
-    out = torch.empty_like(q)
-    if out.stride(-1) != 1 or any(s % 8 for s in out.stride()[:3]):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((batch, q_heads, nodes), dtype=torch.float32, device=q.device)
+    _, kv_heads, max_len, _ = k_cache.shape
+    device = q.get_device()
+    q_ptr, q_strides = _hip.row_layout(q, "q", device)
+    k_ptr, k_strides = _hip.row_layout(k_cache, "k_cache", device)
+    v_ptr, v_strides = _hip.row_layout(v_cache, "v_cache", device)
+    kt_ptr, kt_strides = _hip.row_layout(k_tree, "k_tree", device)
+    vt_ptr, vt_strides = _hip.row_layout(v_tree, "v_tree", device)
     group = q_heads // kv_heads
-    slots = _hip.query("tk_tree_decode_slots", batch, kv_heads, group, max_len, nodes,
-                       head_dim)
+    slots = _slots(batch, kv_heads, group, max_len, nodes, head_dim)
     if slots < 0:
         raise ValueError("tree_decode: the problem is too large")
-    workspace = torch.empty(slots * nodes * group * (head_dim + 2), dtype=torch.float32,
-                            device=q.device) if slots else None
+    out = torch.empty_like(q)
+    out_strides = out.stride()
+    if out_strides[3] != 1 or (out_strides[0] | out_strides[1] | out_strides[2]) & 7:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out_strides = out.stride()
+    lse = workspace = None
+    if return_lse:
+        lse = torch.empty((batch, q_heads, nodes), dtype=torch.float32, device=q.device)
+    if slots:
+        workspace = torch.empty(slots * nodes * group * (head_dim + 2), dtype=torch.float32,
+                                device=q.device)
+    mask_strides = mask.stride()
     _hip.call_on(
         q,
         "tk_tree_decode",
-        _hip.dtype_code(q.dtype),
-        q.data_ptr(),
-        k_cache.data_ptr(),
-        v_cache.data_ptr(),
-        k_tree.data_ptr(),
-        v_tree.data_ptr(),
+        _hip.DTYPE_CODES[q.dtype],
+        q_ptr,
+        k_ptr,
+        v_ptr,
+        kt_ptr,
+        vt_ptr,
         mask.data_ptr(),
-        _hip.ptr(cache_seqlens),
+        None if cache_seqlens is None else cache_seqlens.data_ptr(),
         out.data_ptr(),
-        lse.data_ptr(),
-        _hip.ptr(workspace),
+        None if lse is None else lse.data_ptr(),
+        None if workspace is None else workspace.data_ptr(),
         batch,
         q_heads,
         kv_heads,
         max_len,
         nodes,
         head_dim,
-        _hip.int64_array(q.stride()[:3]),
-        _hip.int64_array(k_cache.stride()[:3]),
-        _hip.int64_array(v_cache.stride()[:3]),
-        _hip.int64_array(k_tree.stride()[:3]),
-        _hip.int64_array(v_tree.stride()[:3]),
-        _hip.int64_array((mask.stride(0) if mask.ndim == 3 else 0, mask.stride(-2))),
-        _hip.int64_array(out.stride()[:3]),
+        q_strides,
+        k_strides,
+        v_strides,
+        kt_strides,
+        vt_strides,
+        _hip.int64_bytes((0 if len(mask_strides) == 2 else mask_strides[0], mask_strides[-2])),
+        _hip.int64_bytes(out_strides[:3]),
         head_dim ** -0.5 if scale is None else float(scale),
         _hip.stream_of(q),
     )
     return (out, lse) if return_lse else out
+
+
+@lru_cache(maxsize=256)
+def _slots(batch: int, kv_heads: int, group: int, max_len: int, nodes: int, head_dim: int) -> int:
+    """Partial results per row that the library asks for (a function of the sizes alone)."""
+    return _hip.query("tk_tree_decode_slots", batch, kv_heads, group, max_len, nodes, head_dim)
 
 
 def _validate(
@@ -133,20 +152,21 @@ def _validate(
     mask: torch.Tensor,
     cache_seqlens: torch.Tensor | None,
 ) -> None:
-    """Check the contract."""
-    if q.ndim != 4 or k_cache.ndim != 4 or k_tree.ndim != 4:
+    """Check the contract, up to the rows' layout."""
+    q_shape, cache_shape, tree_shape = q.shape, k_cache.shape, k_tree.shape
+    if len(q_shape) != 4 or len(cache_shape) != 4 or len(tree_shape) != 4:
         raise ValueError("tree_decode expects q [batch, q_heads, nodes, head_dim], caches [batch, "
                          "kv_heads, max_len, head_dim] and drafted keys and values [batch, "
                          "kv_heads, nodes, head_dim]")
-    if v_cache.shape != k_cache.shape or v_tree.shape != k_tree.shape:
+    if v_cache.shape != cache_shape or v_tree.shape != tree_shape:
         raise ValueError("keys and values must have identical shapes")
-    batch, q_heads, nodes, head_dim = q.shape
-    kv_heads = k_cache.shape[1]
-    if k_cache.shape[0] != batch or k_cache.shape[3] != head_dim:
+    batch, q_heads, nodes, head_dim = q_shape
+    cache_batch, kv_heads, max_len, cache_dim = cache_shape
+    if cache_batch != batch or cache_dim != head_dim:
         raise ValueError("q and the caches disagree on batch or head_dim")
-    if tuple(k_tree.shape) != (batch, kv_heads, nodes, head_dim):
+    if tree_shape != (batch, kv_heads, nodes, head_dim):
         raise ValueError("k_tree and v_tree must be [batch, kv_heads, nodes, head_dim]")
-    if q.numel() == 0 or k_cache.numel() == 0:
+    if not (batch and q_heads and nodes and head_dim and kv_heads and max_len):
         raise ValueError("tree_decode does not support empty dimensions")
     if nodes > _MAX_NODES:
         raise ValueError(f"tree_decode supports at most {_MAX_NODES} nodes")
@@ -156,26 +176,25 @@ def _validate(
         raise ValueError("q_heads must be a multiple of kv_heads")
     if head_dim not in _HEAD_DIMS:
         raise ValueError("tree_decode supports head_dim 64 and 128")
-    if q.dtype not in _DTYPES or any(t.dtype != q.dtype for t in (k_cache, v_cache, k_tree, v_tree)):
+    dtype = q.dtype
+    if dtype not in _DTYPES or not (
+            dtype == k_cache.dtype == v_cache.dtype == k_tree.dtype == v_tree.dtype):
         raise ValueError("q, caches and drafted keys and values must share a float16 or bfloat16 "
                          "dtype")
-    if mask.dtype != torch.bool or tuple(mask.shape) not in ((nodes, nodes), (batch, nodes, nodes)):
+    mask_shape = mask.shape
+    if mask.dtype != torch.bool or (mask_shape != (nodes, nodes)
+                                    and mask_shape != (batch, nodes, nodes)):
         raise ValueError("mask must be a bool [nodes, nodes] or [batch, nodes, nodes] tensor")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise ValueError("tree_decode requires CUDA (ROCm/HIP) tensors")
-    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_tree", k_tree),
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_tree", k_tree),
                     ("v_tree", v_tree)):
-        if t.device != q.device:
-            raise ValueError(f"{name} must be on q's device")
-        if t.stride(-1) != 1:
-            raise ValueError(f"{name} requires a contiguous final dimension")
-        if t.data_ptr() % 16 or any(s % 8 or s < 0 for s in t.stride()[:3]):
-            raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of 8)")
-        if name != "q" and t.stride(2) >= 2**24:
+        if t.stride(2) >= 2**24:
             raise ValueError(f"{name} key strides must be below 2**24 elements")
-    if mask.device != q.device or (nodes > 1 and mask.stride(-1) != 1):
+    device = q.get_device()
+    if mask.get_device() != device or (nodes > 1 and mask.stride(-1) != 1):
         raise ValueError("mask must be on q's device with a contiguous final dimension")
     if cache_seqlens is not None and (
             cache_seqlens.shape != (batch,) or cache_seqlens.dtype != torch.int32
-            or cache_seqlens.device != q.device or not cache_seqlens.is_contiguous()):
+            or cache_seqlens.get_device() != device or not cache_seqlens.is_contiguous()):
         raise ValueError("cache_seqlens must be a contiguous int32 [batch] tensor on q's device")

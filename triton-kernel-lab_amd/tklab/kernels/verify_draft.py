@@ -66,25 +66,34 @@ def verify_draft(
     """
     _validate(target_probs, draft_tokens, uniforms, parents, draft_probs)
     batch, nodes, vocabulary = target_probs.shape
-    device = target_probs.device
+    device, int32 = target_probs.device, torch.int32
     chunk = chunk_length(batch, vocabulary)
     splits = -(-vocabulary // chunk)
-    path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
-    count = torch.empty(batch, dtype=torch.int32, device=device)
+    path = torch.empty((batch, nodes), dtype=int32, device=device)
+    count = torch.empty(batch, dtype=int32, device=device)
     next_token = torch.empty(batch, dtype=torch.int64, device=device)
     # Two float64 sums per split, then four words and a list of rejected tokens per sequence.
     workspace = torch.empty(batch * (2 * splits + (4 + nodes + 1) // 2), dtype=torch.float64,
                             device=device)
     if nodes == 1:
         draft_probs = None
+    target_strides = target_probs.stride()
+    draft_ptr = draft_strides = parents_ptr = None
+    parents_stride = 0
+    if draft_probs is not None:
+        draft_ptr = draft_probs.data_ptr()
+        draft_strides = _hip.int64_bytes(draft_probs.stride()[:2])
+    if parents is not None:
+        parents_ptr = parents.data_ptr()
+        parents_stride = parents.stride(0) if parents.dim() == 2 else 0
     _hip.call_on(
         target_probs,
         "tk_verify_draft",
-        _hip.dtype_code(target_probs.dtype),
+        _hip.DTYPE_CODES[target_probs.dtype],
         target_probs.data_ptr(),
-        _hip.ptr(draft_probs),
+        draft_ptr,
         draft_tokens.data_ptr(),
-        _hip.ptr(parents),
+        parents_ptr,
         uniforms.data_ptr(),
         path.data_ptr(),
         count.data_ptr(),
@@ -94,13 +103,9 @@ def verify_draft(
         nodes,
         vocabulary,
         chunk,
-        _hip.int64_array(target_probs.stride()[:2]),
-        None if draft_probs is None else _hip.int64_array(draft_probs.stride()[:2]),
-        _hip.int64_array((
-            draft_tokens.stride(0),
-            parents.stride(0) if parents is not None and parents.ndim == 2 else 0,
-            uniforms.stride(0),
-        )),
+        _hip.int64_bytes(target_strides[:2]),
+        draft_strides,
+        _hip.int64_bytes((draft_tokens.stride(0), parents_stride, uniforms.stride(0))),
         int(draft_tokens.dtype == torch.int64),
         _hip.stream_of(target_probs),
     )
@@ -122,39 +127,43 @@ def _validate(
     draft_probs: torch.Tensor | None,
 ) -> None:
     """Check the verification's contract."""
-    if target_probs.ndim != 3:
+    shape, dtype = target_probs.shape, target_probs.dtype
+    if len(shape) != 3:
         raise ValueError("verify_draft expects target_probs [batch, nodes, vocabulary]")
-    batch, nodes, vocabulary = target_probs.shape
-    if target_probs.numel() == 0:
+    if 0 in shape:
         raise ValueError("verify_draft does not support empty dimensions")
+    batch, nodes, vocabulary = shape
     if nodes > _MAX_NODES:
         raise ValueError(f"verify_draft supports at most {_MAX_NODES} nodes")
     if batch > 65535 or vocabulary > _MAX_VOCABULARY:
         raise ValueError("verify_draft supports at most 65535 sequences and a vocabulary of "
                          f"{_MAX_VOCABULARY}")
-    if target_probs.dtype not in _DTYPES:
+    if dtype not in _DTYPES:
         raise ValueError("verify_draft supports float16, bfloat16 and float32 probabilities")
-    if draft_tokens.shape != (batch, nodes) or draft_tokens.dtype not in _TOKEN_DTYPES:
+    per_node = (batch, nodes)
+    if draft_tokens.shape != per_node or draft_tokens.dtype not in _TOKEN_DTYPES:
         raise ValueError("draft_tokens must be an int32 or int64 [batch, nodes] tensor")
-    if uniforms.shape != (batch, nodes) or uniforms.dtype != torch.float32:
+    if uniforms.shape != per_node or uniforms.dtype != torch.float32:
         raise ValueError("uniforms must be a float32 [batch, nodes] tensor")
     if parents is not None:
-        if tuple(parents.shape) not in ((nodes,), (batch, nodes)) or parents.dtype != torch.int32:
+        if (parents.shape != per_node and parents.shape != (nodes,)) or (
+                parents.dtype != torch.int32):
             raise ValueError("parents must be an int32 [nodes] or [batch, nodes] tensor")
         if draft_probs is not None:
             raise ValueError("draft_probs belong to a chain: they cannot be given with parents")
     if draft_probs is not None and (draft_probs.shape != (batch, nodes - 1, vocabulary)
-                                    or draft_probs.dtype != target_probs.dtype):
+                                    or draft_probs.dtype != dtype):
         raise ValueError("draft_probs must be [batch, nodes - 1, vocabulary] in target_probs' "
                          "dtype")
-    if target_probs.device.type != "cuda":
+    if not target_probs.is_cuda:
         raise ValueError("verify_draft requires CUDA (ROCm/HIP) tensors")
+    device = target_probs.get_device()
     for name, tensor in (("target_probs", target_probs), ("draft_tokens", draft_tokens),
                          ("uniforms", uniforms), ("parents", parents),
                          ("draft_probs", draft_probs)):
         if tensor is None:
             continue
-        if tensor.device != target_probs.device:
+        if tensor.get_device() != device:
             raise ValueError(f"{name} must be on target_probs' device")
-        if tensor.numel() and tensor.shape[-1] > 1 and tensor.stride(-1) != 1:
+        if tensor.stride(-1) != 1 and tensor.numel() and tensor.shape[-1] > 1:
             raise ValueError(f"{name} requires a contiguous final dimension")
