@@ -26,6 +26,8 @@
 // every workgroup from the lengths (which only the device knows), so a ragged batch fills the
 // chip evenly whatever max_len is. A sequence that is one run is normalized and written by its
 // workgroup; longer ones are joined by the combine kernel in a fixed order.
+#include <type_traits>
+
 #include "attention_dma.hpp"
 #include "tk_common.hpp"
 
@@ -617,26 +619,88 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
       tk_attn::barrier_no_fence();
       if (!second && j + 1 < steps) fetch_step((j + 3) % RS);
     };
+    // A matrix phase as a pipeline of read units, four of them in flight: output units (a tile's
+    // pair of output chunks: four transposing reads) of the step before, then score units (a
+    // tile's 32-feature step: two reads).
+    auto matrix_phase = [&](auto with_output, auto with_scores, uint32_t last, uint32_t now) {
+      constexpr int NV = decltype(with_output)::value ? KT * OC / 2 : 0;
+      constexpr int NU = NV + (decltype(with_scores)::value ? KT * DC : 0);
+      constexpr int IN_FLIGHT = 4;
+      i32x2 vlo[KT * OC / 2][2], vhi[KT * OC / 2][2];
+      i32x4 kc[KT * DC][2];
+      auto issue = [&](int u) {
+        if (u < NV) {
+          const uint32_t at = last + (u / (OC / 2)) * R::STAGE;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t v = at + va[2 * (u % (OC / 2)) + x];
+            vlo[u][x] = tk_attn::lds_read_tr16<0>(v);
+            vhi[u][x] = tk_attn::lds_read_tr16<16 * RB>(v);
+          }
+        } else {
+          request_k(now, kc, u - NV);
+        }
+      };
+#pragma unroll
+      for (int u = 0; u < IN_FLIGHT && u < NU; ++u) issue(u);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        int younger = 0;  // reads that may still be in flight
+        for (int x = u + 1; x < u + IN_FLIGHT && x < NU; ++x) younger += x < NV ? 4 : 2;
+        if (younger == 12)
+          tk_attn::wait_lgkm<12>();
+        else if (younger == 10)
+          tk_attn::wait_lgkm<10>();
+        else if (younger == 8)
+          tk_attn::wait_lgkm<8>();
+        else if (younger == 6)
+          tk_attn::wait_lgkm<6>();
+        else if (younger == 4)
+          tk_attn::wait_lgkm<4>();
+        else if (younger == 2)
+          tk_attn::wait_lgkm<2>();
+        else
+          tk_attn::wait_lgkm<0>();
+        if (u < NV) {
+          const int n = u / (OC / 2), c = 2 * (u % (OC / 2));
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            asm volatile("" : "+v"(vlo[u][x]), "+v"(vhi[u][x]));
+            const i32x4 vf = {vlo[u][x][0], vlo[u][x][1], vhi[u][x][0], vhi[u][x][1]};
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              o[m][c + x] = tk_attn::Mma16<T>::run(vf, pf[n][m], o[m][c + x]);
+          }
+        } else {
+          const int k = u - NV;
+          tk_attn::pin(kc[k][0]);
+          tk_attn::pin(kc[k][1]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              s[k / DC][m][i] = tk_attn::Mma16<T>::run(
+                  kc[k][i], qf[m][k % DC],
+                  k % DC == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[k / DC][m][i]);
+        }
+        if (u + IN_FLIGHT < NU) issue(u + IN_FLIGHT);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    const std::true_type yes;
+    const std::false_type no;
     fetch_step(2 % RS);
     if (second) tk_attn::barrier_no_fence();
-    {
-      i32x4 kc[KT * DC][2];
-      request_first_k(stage_of(0), kc);
-      products(stage_of(0), kc, s);
-    }
+    matrix_phase(no, yes, 0u, stage_of(0));
     matrix_end(0);
     softmax_phase(0);
     for (int j = 1; j < steps; ++j) {
-      i32x4 kc[KT * DC][2];
-      const uint32_t now = stage_of(j), last = stage_of(j + RS - 1);
-      request_v(last, 0);
-      accumulate_step(last, pf, [&]() { request_first_k(now, kc); });
-      products(now, kc, s);
+      matrix_phase(yes, yes, stage_of(j + RS - 1), stage_of(j));
       matrix_end(j);
       softmax_phase(j);
     }
-    request_v(stage_of(steps - 1), 0);
-    accumulate_step(stage_of(steps - 1), pf, nothing);
+    matrix_phase(yes, no, stage_of(steps - 1), 0u);
     // Both waves of a SIMD have passed 2 steps + 2 barriers, so the ring is read by none.
     tk_attn::barrier_no_fence();
     if (!second) tk_attn::barrier_no_fence();
