@@ -1,0 +1,51 @@
+"""Calls on tensors of a GPU that is not the current one are made with that GPU current."""
+
+from __future__ import annotations
+
+import contextlib
+
+import pytest
+import torch
+
+from tklab import _hip
+
+
+class _Tensor:
+    device = torch.device("cuda", 1)
+
+    def get_device(self):
+        return 1
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_call_on_selects_the_tensors_device(monkeypatch, current) -> None:
+    events = []
+
+    @contextlib.contextmanager
+    def selected(device):
+        events.append(("select", device))
+        yield
+        events.append(("restore", device))
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current)
+    monkeypatch.setattr(torch.cuda, "device", selected)
+    monkeypatch.setattr(_hip, "call", lambda name, *args: events.append((name, args)))
+    _hip.call_on(_Tensor(), "tk_rotary", 1, 2)
+    call = ("tk_rotary", (1, 2))
+    device = torch.device("cuda", 1)
+    assert events == ([call] if current == 1 else [("select", device), call, ("restore", device)])
+
+
+def test_row_layout_packs_strides_and_refuses_rows_the_kernels_cannot_read() -> None:
+    x = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16)
+    address, strides = _hip.row_layout(x, "x", -1)
+    assert address == x.data_ptr() and strides == _hip.int64_bytes((768, 256, 64))
+    assert list(memoryview(strides).cast("q")) == [768, 256, 64]
+    with pytest.raises(ValueError, match="x must be on"):
+        _hip.row_layout(x, "x", 0)
+    with pytest.raises(ValueError, match="contiguous final"):
+        _hip.row_layout(x.transpose(2, 3), "x", -1)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        _hip.row_layout(x[..., 1:], "x", -1)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        _hip.row_layout(torch.zeros(2, 3, 4, 60, dtype=torch.bfloat16), "x", -1)

@@ -250,7 +250,8 @@ extern "C" int tk_rotary(int dtype, const void* q, void* q_out, const void* k, v
     return tk::fail("rotary: rotary_dim must be even, positive and at most head_dim");
   const int64_t heads = q_heads + (with_k ? kv_heads : 0);
   int64_t total;
-  if (__builtin_mul_overflow(batch, tokens, &total) || total > INT32_MAX || heads > 65535)
+  if (__builtin_mul_overflow(batch, tokens, &total) || total > INT32_MAX - 65536 ||
+      heads > 65535)
     return tk::fail("rotary: problem too large");
 
   RotaryArgs a;
