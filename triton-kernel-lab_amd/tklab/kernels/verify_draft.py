@@ -19,9 +19,10 @@ _MAX_NODES = 256
 _MAX_VOCABULARY = 2**31 - 65537
 _MAX_SPLITS = 64
 _CHUNK = 2048
-# Workgroups that weigh rows: enough of them to fill the 256 CUs, few enough that the walk each
-# repeats stays small beside its share of a row.
-_TARGET_WORKGROUPS = 2048
+# Workgroups that weigh rows, about: four for each of the 256 CUs. 64 rows of 131072 float32 take
+# 14.8 us in 1024 workgroups and 16.9 in 2048 (each repeats the walk); with few bytes to read, more
+# and shorter shares are faster (32 rows of 65537 bfloat16: 6.4 us in 1056, 7.2 in 544).
+_TARGET_WORKGROUPS = 1024
 
 
 def verify_draft(
@@ -113,10 +114,10 @@ def verify_draft(
 
 
 def chunk_length(batch: int, vocabulary: int) -> int:
-    """Row entries per workgroup: a multiple of 2048, at most 64 of them per row, and about
+    """Row entries per workgroup: a multiple of 2048, at most 64 shares per row, and about
     _TARGET_WORKGROUPS in all once the batch has that much to read."""
-    per = max(-(-vocabulary // _MAX_SPLITS), -(-batch * vocabulary // _TARGET_WORKGROUPS))
-    return -(-per // _CHUNK) * _CHUNK
+    least = -(-vocabulary // (_MAX_SPLITS * _CHUNK))
+    return _CHUNK * max(least, batch * vocabulary // (_TARGET_WORKGROUPS * _CHUNK))
 
 
 def _validate(
