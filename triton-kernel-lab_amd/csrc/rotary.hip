@@ -12,6 +12,10 @@
 // tokens would leave CUs idle, a run of one token's heads), evaluates their angles once into
 // LDS, one per thread, and then streams the rows. The first rows are requested before the
 // angles are formed, so the two latencies overlap.
+//
+// Bound by HBM: q and k are read and written once. B2 N8192 Hq32 Hkv8 D128 bf16 (336 MB a pass):
+// 60 us, 5.6 TB/s, with about four units a thread and non-temporal accesses; two units 65 us, eight
+// 66, plain loads 64. One token of the same heads: 2.8 us.
 #include "tk_common.hpp"
 
 namespace {
@@ -36,7 +40,7 @@ struct RotaryArgs {
   int pos64, inverse;
 };
 
-// sin and cos of `turns` quarter-reduced: r in [-pi/4, pi/4], Taylor coefficients 1/n!.
+// sin and cos of r in [-pi/4, pi/4] by their Taylor series (coefficients 1/n!).
 __device__ __forceinline__ void sincos_reduced(double r, double& s, double& c) {
   const double z = r * r;
   double p = -1.0 / 39916800.0;

@@ -26,6 +26,20 @@
 // every workgroup from the lengths (which only the device knows), so a ragged batch fills the
 // chip evenly whatever max_len is. A sequence that is one run is normalized and written by its
 // workgroup; longer ones are joined by the combine kernel in a fixed order.
+//
+// What bounds it (D128 bf16, Hkv8, split + combine kernel): up to 128 rows per KV head HBM, and for
+// short contexts the chain of latencies (2.5 us to find the run, 1.5 to the first tile, about 0.75
+// per tile, 1.5 and more for the partial results). B1 T8 G4 L2000 (32 rows): 9 + 4 us. B16 T16 G4
+// of lengths up to 8192 (64 rows, 304 MB): 57 + 6.4 us, 5.3 TB/s in the split kernel; equal lengths
+// of 8192 with 16 or 32 rows 6.3 to 6.5 TB/s. With 256 rows the matrix and vector work per tile:
+// B1 T64 G4 L131072 (538 MB, 137.5 GFLOP): 141 to 146 + 7.6 us, 0.95 PFLOP/s; of it 10 us before
+// the key loop and 6 to 10 behind it (33.5 MB of partial results). Half the LDS reads, or the same
+// tile read again and again, takes as long there; without the exponentials it is 8 % shorter.
+// Measured and not kept: four waves of 64 rows, one per SIMD, with the exponentials of one tile
+// between the products of another (175 to 193 us: a wave issues in order, and its issue slots are
+// the bound); the DMA spread over the matrix phase (150 us against 147); default-policy loads
+// (B16: 66.8 us against 57.8); non-temporal stores of partial results (B16 L1024 24.8 -> 21.3 us,
+// ragged 57 -> 61); all V reads of a tile up front (B1 L2000 9.1 -> 9.7 us).
 #include <type_traits>
 
 #include "attention_dma.hpp"
@@ -578,7 +592,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
     // Eight waves, two per SIMD, in phases ended by barriers: a wave alternates a matrix phase
     // (step j - 1's output products, then step j's scores) with a softmax phase, the second wave
     // of each SIMD (by the hardware's SIMD id) one phase behind the first, so that one wave's
-    // exponentials run beside the other's products. Step j's slot is read in phases 2j .. 2j + 3;
+    // exponentials run beside the other's products (B1 T64 G4 L131072 148 -> 143 us). Step j's slot is read in phases 2j .. 2j + 3;
     // step j + 2, fetched from phase 2j on, takes the slot of step j - 2. Waves without rows run
     // along on zeros.
     const int steps = (c1 - t0 + KT - 1) / KT;
@@ -849,9 +863,11 @@ __global__ __launch_bounds__(64 * kCombineWaves) void tree_combine_kernel(TreeAr
         total == 0.f ? -INFINITY : high + log2f(total);
 }
 
-// Workgroup shapes by the rows a KV head has: as few waves as hold them (each key tile costs
-// every wave its LDS reads), 256 rows at most. `resident`: workgroups that run at once, two per CU
-// with a 64 KiB ring, one with 128 KiB (256 rows at head_dim 128, eight waves of 256 registers).
+// Workgroup shapes by the rows a KV head has: 16 rows a wave up to four waves, then more rows a
+// wave, 256 rows at most. `resident`: workgroups that run at once, two per CU with a 64 KiB ring,
+// one with 128 KiB (256 rows at head_dim 128, eight waves of 256 registers). Half the waves with
+// twice the rows each: 32 rows 12.1 us against 10.1 (B1 L2000) and 89.5 against 87 (B16 L8192), 64
+// rows level, 128 rows 67 against 57 (B8 L8192).
 struct Shape {
   int rows, resident;
 };
