@@ -592,9 +592,9 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
     // Eight waves, two per SIMD, in phases ended by barriers: a wave alternates a matrix phase
     // (step j - 1's output products, then step j's scores) with a softmax phase, the second wave
     // of each SIMD (by the hardware's SIMD id) one phase behind the first, so that one wave's
-    // exponentials run beside the other's products (B1 T64 G4 L131072 148 -> 143 us). Step j's slot is read in phases 2j .. 2j + 3;
-    // step j + 2, fetched from phase 2j on, takes the slot of step j - 2. Waves without rows run
-    // along on zeros.
+    // exponentials run beside the other's products (B1 T64 G4 L131072 148 -> 143 us). Step j's
+    // slot is read in phases 2j .. 2j + 3; step j + 2, fetched from phase 2j on, takes the slot of
+    // step j - 2. Waves without rows run along on zeros.
     const int steps = (c1 - t0 + KT - 1) / KT;
     int second = 0;
     {
