@@ -10,13 +10,6 @@ import torch
 from tklab import _hip
 
 
-class _Tensor:
-    device = torch.device("cuda", 1)
-
-    def get_device(self):
-        return 1
-
-
 @pytest.mark.parametrize("current", [0, 1])
 def test_call_on_selects_the_tensors_device(monkeypatch, current) -> None:
     events = []
@@ -29,11 +22,18 @@ def test_call_on_selects_the_tensors_device(monkeypatch, current) -> None:
 
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current)
     monkeypatch.setattr(torch.cuda, "device", selected)
-    monkeypatch.setattr(_hip, "call", lambda name, *args: events.append((name, args)))
-    _hip.call_on(_Tensor(), "tk_rotary", 1, 2)
-    call = ("tk_rotary", (1, 2))
-    device = torch.device("cuda", 1)
-    assert events == ([call] if current == 1 else [("select", device), call, ("restore", device)])
+    monkeypatch.setitem(_hip._bound, "tk_rotary", lambda *args: events.append(args) or 0)
+    _hip.call_on(1, "tk_rotary", 4, 2)
+    assert events == ([(4, 2)] if current == 1 else [("select", 1), (4, 2), ("restore", 1)])
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_call_on_raises_for_a_failed_call(monkeypatch, current) -> None:
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current)
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    monkeypatch.setitem(_hip._bound, "tk_rotary", lambda *args: 1)
+    with pytest.raises(_hip.HipLibraryError, match="tk_rotary failed"):
+        _hip.call_on(1, "tk_rotary", 4, 2)
 
 
 def test_row_layout_packs_strides_and_refuses_rows_the_kernels_cannot_read() -> None:

@@ -228,17 +228,28 @@ def call(name: str, *args: object) -> None:
     """Invoke ``name`` and raise :class:`HipLibraryError` on a non-zero status."""
     status = (_bound.get(name) or _function(name))(*args)
     if status != 0:
-        message = load_library().tk_last_error().decode(errors="replace")
-        raise HipLibraryError(f"{name} failed: {message}")
+        _fail(name)
 
 
-def call_on(tensor: torch.Tensor, name: str, *args: object) -> None:
-    """:func:`call` with ``tensor``'s device current, whichever device the caller has selected."""
-    if tensor.get_device() == torch._C._cuda_getDevice():
-        call(name, *args)
+def _fail(name: str) -> None:
+    """Raise with the library's message for the failed entry point ``name``."""
+    message = load_library().tk_last_error().decode(errors="replace")
+    raise HipLibraryError(f"{name} failed: {message}")
+
+
+def call_on(device: int, name: str, *args: object) -> None:
+    """:func:`call` with GPU ``device`` current, whichever the caller has selected."""
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            call(name, *args)
         return
-    with torch.cuda.device(tensor.device):
-        call(name, *args)
+    if (_bound.get(name) or _function(name))(*args) != 0:
+        _fail(name)
+
+
+def stream_on(device: int) -> int:
+    """Handle of PyTorch's current stream on GPU ``device`` (:func:`stream_of` by index)."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def row_layout(tensor: torch.Tensor, name: str, device: int) -> tuple[int, bytes]:

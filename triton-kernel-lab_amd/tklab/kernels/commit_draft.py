@@ -55,7 +55,7 @@ def commit_draft(
     vt_ptr, vt_strides = _hip.row_layout(v_tree, "v_tree", device)
     lengths = torch.empty_like(cache_seqlens)
     _hip.call_on(
-        k_cache,
+        device,
         "tk_commit_draft",
         _hip.DTYPE_CODES[k_cache.dtype],
         k_ptr,
@@ -75,7 +75,7 @@ def commit_draft(
         v_strides,
         kt_strides,
         vt_strides,
-        _hip.stream_of(k_cache),
+        _hip.stream_on(device),
     )
     return lengths
 

@@ -183,8 +183,9 @@ def _launch(
             k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         kv_heads, k_ptr, k_out_ptr = k.shape[1], k.data_ptr(), k_out.data_ptr()
         k_table, k_out_table = _strides(k.stride(), packed), _strides(k_out.stride(), packed)
+    device = q.get_device()
     _hip.call_on(
-        q,
+        device,
         "tk_rotary",
         _hip.DTYPE_CODES[q.dtype],
         q.data_ptr(),
@@ -209,7 +210,7 @@ def _launch(
         int(interleaved),
         int(positions.dtype == torch.int64),
         int(inverse),
-        _hip.stream_of(q),
+        _hip.stream_on(device),
     )
     return q_out, k_out
 

@@ -101,11 +101,11 @@ def tree_decode(
     if return_lse:
         lse = torch.empty((batch, q_heads, nodes), dtype=torch.float32, device=q.device)
     if slots:
-        workspace = torch.empty(slots * nodes * group * (head_dim + 2), dtype=torch.float32,
-                                device=q.device)
+        # Float32 partial results, as twice as many elements of q's type.
+        workspace = q.new_empty(2 * slots * nodes * group * (head_dim + 2))
     mask_strides = mask.stride()
     _hip.call_on(
-        q,
+        device,
         "tk_tree_decode",
         _hip.DTYPE_CODES[q.dtype],
         q_ptr,
@@ -132,7 +132,7 @@ def tree_decode(
         _hip.int64_bytes((0 if len(mask_strides) == 2 else mask_strides[0], mask_strides[-2])),
         _hip.int64_bytes(out_strides[:3]),
         head_dim ** -0.5 if scale is None else float(scale),
-        _hip.stream_of(q),
+        _hip.stream_on(device),
     )
     return (out, lse) if return_lse else out
 

@@ -67,15 +67,17 @@ def verify_draft(
     """
     _validate(target_probs, draft_tokens, uniforms, parents, draft_probs)
     batch, nodes, vocabulary = target_probs.shape
-    device, int32 = target_probs.device, torch.int32
+    device = target_probs.get_device()
     chunk = chunk_length(batch, vocabulary)
     splits = -(-vocabulary // chunk)
-    path = torch.empty((batch, nodes), dtype=int32, device=device)
-    count = torch.empty(batch, dtype=int32, device=device)
-    next_token = torch.empty(batch, dtype=torch.int64, device=device)
-    # Two float64 sums per split, then four words and a list of rejected tokens per sequence.
-    workspace = torch.empty(batch * (2 * splits + (4 + nodes + 1) // 2), dtype=torch.float64,
-                            device=device)
+    path = torch.empty_like(uniforms, dtype=torch.int32, memory_format=torch.contiguous_format)
+    count = path.new_empty(batch)
+    if draft_tokens.dtype == torch.int64:
+        next_token = draft_tokens.new_empty(batch)
+    else:
+        next_token = torch.empty(batch, dtype=torch.int64, device=target_probs.device)
+    # Words: two float64 sums per split, then four and a list of rejected tokens per sequence.
+    workspace = path.new_empty(batch * (4 * splits + 4 + nodes))
     if nodes == 1:
         draft_probs = None
     target_strides = target_probs.stride()
@@ -88,7 +90,7 @@ def verify_draft(
         parents_ptr = parents.data_ptr()
         parents_stride = parents.stride(0) if parents.dim() == 2 else 0
     _hip.call_on(
-        target_probs,
+        device,
         "tk_verify_draft",
         _hip.DTYPE_CODES[target_probs.dtype],
         target_probs.data_ptr(),
@@ -108,7 +110,7 @@ def verify_draft(
         draft_strides,
         _hip.int64_bytes((draft_tokens.stride(0), parents_stride, uniforms.stride(0))),
         int(draft_tokens.dtype == torch.int64),
-        _hip.stream_of(target_probs),
+        _hip.stream_on(device),
     )
     return path, count, next_token
 
