@@ -264,6 +264,20 @@ def test_offsets_past_32_bits() -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 40])
+def test_the_last_entry_of_the_longest_row(batch) -> None:
+    """The last share's end, counted from its start in whole shares, lies past 32 bits."""
+    vocabulary = 2 ** 31 - 65537
+    row = torch.zeros(vocabulary, dtype=torch.float16, device="cuda")
+    row[-1] = 0.5
+    target = row.expand(batch, 1, vocabulary)
+    tokens = torch.zeros(batch, 1, dtype=torch.int64, device="cuda")
+    path, count, token = verify_draft(target, tokens, torch.full((batch, 1), 0.5, device="cuda"))
+    assert bool((token == vocabulary - 1).all())
+    assert bool((path == 0).all()) and bool((count == 1).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("sampled", [False, True])
 def test_what_comes_out_is_distributed_like_the_target(sampled) -> None:
     """Over a grid of random numbers, the first token that comes out follows p: each of its
@@ -352,3 +366,8 @@ def test_chunks_cover_the_row_in_at_most_64_splits() -> None:
         for vocabulary in (1, 2048, 2049, 131072, 2 ** 31 - 65537):
             chunk = chunk_length(batch, vocabulary)
             assert chunk % 8 == 0 and -(-vocabulary // chunk) <= 64
+
+
+def test_shares_stay_within_what_the_library_counts() -> None:
+    for batch in (1, 40, 1024, 65535):
+        assert chunk_length(batch, 2 ** 31 - 65537) <= 2 ** 30

@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kWeighThreads) void verify_weigh_kernel(VerifyArgs 
   const int split = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c0 = split * a.chunk;
-  const int c1 = min(c0 + a.chunk, a.vocabulary);
+  const int c1 = c0 + min(a.chunk, a.vocabulary - c0);  // c0 + chunk may pass 32 bits
   constexpr int C = kMaxNodes / 64;
   if (wave == 0) {
     Walk w;
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a)
   const int split = past != 0 ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
   double base = split > 0 ? lane_value(upto, split - 1) : 0.0;
   const int c0 = split * a.chunk;
-  const int c1 = min(c0 + a.chunk, a.vocabulary);
+  const int c1 = c0 + min(a.chunk, a.vocabulary - c0);  // c0 + chunk may pass 32 bits
   if (tid < 2) winner[tid] = kDrawThreads;
   __syncthreads();
 

@@ -117,9 +117,11 @@ def verify_draft(
 
 def chunk_length(batch: int, vocabulary: int) -> int:
     """Row entries per workgroup: a multiple of 2048, at most 64 shares per row, and about
-    _TARGET_WORKGROUPS in all once the batch has that much to read."""
+    _TARGET_WORKGROUPS in all once the batch has that much to read (2**30 at most: the library
+    counts in 32 bits)."""
     least = -(-vocabulary // (_MAX_SPLITS * _CHUNK))
-    return _CHUNK * max(least, batch * vocabulary // (_TARGET_WORKGROUPS * _CHUNK))
+    share = max(least, batch * vocabulary // (_TARGET_WORKGROUPS * _CHUNK))
+    return min(_CHUNK * share, 2**30)
 
 
 def _validate(
