@@ -130,6 +130,17 @@ def test_far_negative_and_expanded_positions(dtype) -> None:
 
 
 @pytest.mark.gpu
+def test_positions_whose_angles_pass_53_bits() -> None:
+    """Angles are float64, so such a position's is that of its nearest float64; the reference is
+    formed from the same one."""
+    freq, _ = rotary_frequencies(64, device="cuda")
+    q = _make((2, 4, 7, 64), torch.float32, 18)
+    pos = torch.tensor([2 ** 50 + 1, -2 ** 52 + 1, 2 ** 53 + 2, 10 ** 17 + 16, -10 ** 18, 2 ** 62 + 4096,
+                        -2 ** 63], device="cuda")
+    _check(rotary_embedding(q, None, pos, freq), q, pos, freq)
+
+
+@pytest.mark.gpu
 def test_position_zero_is_the_identity_and_quarter_turns_are_exact_swaps() -> None:
     q = _make((6, 2, 8), torch.float32, 9)
     pos = torch.arange(6, device="cuda")
@@ -254,6 +265,41 @@ def test_a_captured_call_replays_with_new_positions_on_another_stream() -> None:
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(q_out, eager[0]) and torch.equal(k_out, eager[1])
+
+
+@pytest.mark.gpu
+def test_a_captured_forward_and_backward_replays() -> None:
+    """No eager graph of the captured leaves is alive: they are made for the capture's stream."""
+    freq, _ = rotary_frequencies(48, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+
+    def step(q, k, pos, dq, dk):
+        return torch.autograd.grad(rotary_embedding(q, k, pos, freq), (q, k), (dq, dk))
+
+    def made(seed):
+        q, k = _make((2, 4, 33, 64), torch.bfloat16, seed), _make((2, 2, 33, 64), torch.bfloat16, seed + 1)
+        return (q.requires_grad_(), k.requires_grad_(), torch.arange(33, device="cuda") * seed,
+                _make(q.shape, torch.bfloat16, seed + 2), _make(k.shape, torch.bfloat16, seed + 3))
+
+    with torch.cuda.stream(stream):
+        step(*made(1))
+        inputs = made(2)
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            grads = step(*inputs)
+    torch.cuda.synchronize()
+    for seed in (3, 4, 5):
+        other = made(seed)
+        eager = step(*other)
+        with torch.no_grad():
+            for held, new in zip(inputs, other):
+                held.copy_(new)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(grads, eager))
 
 
 # ------------------------------------------------------------------ without a GPU

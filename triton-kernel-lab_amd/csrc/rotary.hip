@@ -161,15 +161,18 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     const double pos = a.pos64 ? double(static_cast<const int64_t*>(a.positions)[at])
                                : double(static_cast<const int32_t*>(a.positions)[at]);
     const double x = pos * a.frequencies[pair];
-    // x = k pi/2 + r; pi/2 in two parts, the first with all 53 bits.
+    // x = k pi/2 + r; pi/2 in two parts, the first with all 53 bits. Past 2^51 the rounding of
+    // x * 2/pi is off by whole quarter turns: the second pass takes off those that are left.
     const double k = rint(x * 0.63661977236758134308);
     double r = fma(k, -1.5707963267948965580, x);
     r = fma(k, -6.1232339957367658e-17, r);
+    const double more = rint(r * 0.63661977236758134308);
+    r = fma(more, -1.5707963267948965580, r);
+    r = fma(more, -6.1232339957367658e-17, r);
     double s, c;
     sincos_reduced(r, s, c);
-    // k modulo 4, exact for every finite k (2^53 and above are multiples of 4 or refused by
-    // rounding: such angles have no fraction left anyway).
-    const int quarter = int(k - 4.0 * floor(0.25 * k));
+    // k modulo 4 is exact for every finite k.
+    const int quarter = int(k - 4.0 * floor(0.25 * k)) + int(more);
     if (quarter & 1) {
       const double swap = s;
       s = c;

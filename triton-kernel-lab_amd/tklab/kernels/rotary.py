@@ -105,7 +105,9 @@ def rotary_embedding(
         positions: int32 or int64, ``[batch, tokens]`` or ``[tokens]`` (shared by the batch);
             ``[tokens]`` for packed tensors. Any value, negative ones included.
         frequencies: float64 ``[rotary_dim // 2]`` on the same device
-            (:func:`rotary_frequencies`); features past ``rotary_dim`` are copied.
+            (:func:`rotary_frequencies`), at most 1 where positions reach 2**62 (an angle's
+            magnitude is at most 2**63); they get no gradient; features past ``rotary_dim`` are
+            copied.
         interleaved: pairs are ``(2i, 2i + 1)``; otherwise ``(i, i + rotary_dim // 2)``.
         magnitude: multiplies cosine and sine (rounded to float32).
 
