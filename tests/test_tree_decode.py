@@ -281,6 +281,21 @@ def test_tree_mask_names_ancestors() -> None:
             tree_mask(wrong)
 
 
+@pytest.mark.parametrize("nodes", [1, 2, 3, 31, 100, 256])
+def test_tree_mask_is_the_closure_of_the_parents(nodes) -> None:
+    gen = torch.Generator().manual_seed(nodes)
+    parents = torch.randint(-2, nodes + 2, (3, nodes), generator=gen, dtype=torch.int32)
+    mask = tree_mask(parents)
+    for b in range(3):
+        for i in range(nodes):
+            seen, at = {i}, i
+            while 0 <= int(parents[b, at]) < at:
+                at = int(parents[b, at])
+                seen.add(at)
+            assert set(mask[b, i].nonzero().flatten().tolist()) == seen
+    assert torch.equal(tree_mask(parents[1]), mask[1])
+
+
 def _meta(*shape, dtype=torch.bfloat16):
     return torch.empty(shape, dtype=dtype, device="meta")
 
@@ -300,6 +315,9 @@ def _meta(*shape, dtype=torch.bfloat16):
     (dict(v_tree=_meta(2, 2, 5, 64, dtype=torch.float16)), "share"),
     (dict(mask=_meta(5, 5, dtype=torch.uint8)), "mask must be a bool"),
     (dict(mask=_meta(1, 5, 5, dtype=torch.bool)), "mask must be a bool"),
+    (dict(scale=math.nan), "scale must be"),
+    (dict(scale=-math.inf), "scale must be"),
+    (dict(scale=1e300), "scale must be"),
     (dict(), "requires CUDA"),
 ])
 def test_refusals(change, message) -> None:

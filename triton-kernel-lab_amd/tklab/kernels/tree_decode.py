@@ -35,12 +35,13 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
         raise ValueError("parents must be an integer [nodes] or [batch, nodes] tensor")
     nodes = parents.shape[-1]
     index = torch.arange(nodes, device=parents.device)
-    has_parent = (parents >= 0) & (parents < index)
-    reach = (index == parents[..., None]) & has_parent[..., None] | torch.eye(
-        nodes, dtype=torch.bool, device=parents.device)
-    steps = 1  # ancestors up to `steps` generations back are reached
-    while steps < nodes:
-        reach = torch.matmul(reach.float(), reach.float()) > 0
+    # The ancestor `steps` generations back, or the tree's root, and who is reached in fewer.
+    ancestor = torch.where((parents >= 0) & (parents < index), parents.long(), index)
+    reach = torch.eye(nodes, dtype=torch.bool, device=parents.device).expand(*parents.shape, nodes)
+    steps = 1
+    while steps <= nodes:
+        reach = reach | reach.gather(-2, ancestor[..., None].expand(*parents.shape, nodes))
+        ancestor = ancestor.gather(-1, ancestor)
         steps *= 2
     return reach
 
@@ -79,7 +80,7 @@ def tree_decode(
     Raises:
         ValueError: on an unsupported shape, dtype, layout or device.
     """
-    _validate(q, k_cache, v_cache, k_tree, v_tree, mask, cache_seqlens)
+    _validate(q, k_cache, v_cache, k_tree, v_tree, mask, cache_seqlens, scale)
     batch, q_heads, nodes, head_dim = q.shape
     _, kv_heads, max_len, _ = k_cache.shape
     device = q.get_device()
@@ -151,6 +152,7 @@ def _validate(
     v_tree: torch.Tensor,
     mask: torch.Tensor,
     cache_seqlens: torch.Tensor | None,
+    scale: float | None,
 ) -> None:
     """Check the contract, up to the rows' layout."""
     q_shape, cache_shape, tree_shape = q.shape, k_cache.shape, k_tree.shape
@@ -182,6 +184,8 @@ def _validate(
         raise ValueError("q, caches and drafted keys and values must share a float16 or bfloat16 "
                          "dtype")
     mask_shape = mask.shape
+    if scale is not None and not abs(scale) < 2.0**126:
+        raise ValueError("scale must be finite and below 2**126")
     if mask.dtype != torch.bool or (mask_shape != (nodes, nodes)
                                     and mask_shape != (batch, nodes, nodes)):
         raise ValueError("mask must be a bool [nodes, nodes] or [batch, nodes, nodes] tensor")
