@@ -119,6 +119,14 @@ def test_sampled_chains(dtype, vocabulary) -> None:
 
 
 @pytest.mark.gpu
+def test_a_chain_without_drafts_takes_draft_probs_without_rows() -> None:
+    target, tokens, uniforms, _ = _problem(3, 1, 500, torch.float32, 11)
+    _check(target, tokens, uniforms)
+    given = verify_draft(target, tokens, uniforms, draft_probs=target[:, 1:])
+    assert all(torch.equal(x, y) for x, y in zip(given, verify_draft(target, tokens, uniforms)))
+
+
+@pytest.mark.gpu
 def test_sampled_chains_end_everywhere() -> None:
     target, tokens, uniforms, draft = _problem(64, 5, 1000, torch.float32, 1, sampled=True)
     _, counts, _ = _check(target, tokens, uniforms, draft_probs=draft)

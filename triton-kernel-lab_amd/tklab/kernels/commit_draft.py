@@ -29,6 +29,7 @@ def commit_draft(
     Cache position ``cache_seqlens[b] + i`` of every KV head takes node ``path[b, i]``'s key and
     value, for ``i < count[b]``. Rows that would lie past the cache's end are not written and not
     counted; all other cache rows are left as they were. ``cache_seqlens`` is not changed.
+    Inference only: autograd does not know of the write.
 
     Args:
         k_cache, v_cache: ``[batch, kv_heads, max_len, head_dim]`` float16 or bfloat16, written
