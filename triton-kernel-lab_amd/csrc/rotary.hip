@@ -15,7 +15,7 @@
 //
 // Bound by HBM: q and k are read and written once. B2 N8192 Hq32 Hkv8 D128 bf16 (336 MB a pass):
 // 60 us, 5.6 TB/s, with about four units a thread and non-temporal accesses; two units 65 us, eight
-// 66, plain loads 64. One token of the same heads: 2.8 us.
+// 66, plain loads 64. One token of the same heads: 2.9 us.
 #include "tk_common.hpp"
 
 namespace {
