@@ -121,6 +121,25 @@ def test_batches_past_one_wave_of_lengths(batch) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,nodes", [(128, 9), (64, 70)])
+def test_whole_and_split_sequences_in_one_batch(dim, nodes) -> None:
+    """128 pairs of a sequence and a KV head: up to 40 tiles are one run, longer sequences several."""
+    q, k, v, kt, vt = _problem(16, 16, 8, nodes, 2900, dim, torch.bfloat16, 4)
+    edge = (40 - -(-nodes // 32)) * 32
+    lens = [0, 1, edge - 1, edge, edge + 1, 2900, 33, 640, edge + 32, 1, 2899, 500, edge, 31, 32, 1700]
+    _check(q, k, v, kt, vt, tree_mask(_tree(nodes).cuda()), _ints(lens))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,tiles", [(1, 10), (4, 10), (16, 18), (64, 40)])
+@pytest.mark.parametrize("more", [0, 1])
+def test_caches_at_the_limit_of_unsplit_calls(batch, tiles, more) -> None:
+    length = (tiles - 1) * 32 + more
+    q, k, v, kt, vt = _problem(batch, 4, 2, 7, length, 64, torch.float16, 5)
+    _check(q, k, v, kt, vt, tree_mask(_tree(7).cuda()))
+
+
+@pytest.mark.gpu
 def test_one_long_sequence_among_short_ones() -> None:
     q, k, v, kt, vt = _problem(6, 4, 1, 5, 40000, 64, torch.float16, 3)
     _check(q, k, v, kt, vt, tree_mask(_tree(5).cuda()), _ints([3, 40000, 0, 77, 32, 900]))

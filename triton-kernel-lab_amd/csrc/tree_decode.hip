@@ -74,7 +74,10 @@ struct TreeArgs {
   int64_t mb, mt;
   int batch, q_heads, kv_heads, group, nodes, rows, max_len;
   tk::FastDiv by_group, by_kv_heads, by_row_blocks;
-  int tree_tiles, min_chunk, runs, row_blocks, flat;  // flat: upper bound on the flat splits
+  int tree_tiles, runs, row_blocks, flat;  // flat: upper bound on the flat splits
+  int whole;         // a sequence of at most this many tiles is one run
+  int heads_blocks;  // kv_heads * row_blocks
+  int many;          // tiles of all sequences that make 128 * 16 with heads_blocks
   float scale_log2;  // positive
   int flip;          // Q's sign bits to turn (a negative scale)
 };
@@ -103,6 +106,9 @@ __device__ __forceinline__ int wave_prefix(int v) {
   return v;
 }
 
+// Tiles of the shortest run of a sequence that is split.
+constexpr int kMinChunk = 4;
+
 struct Lengths {
   int first;  // this lane's sequence's length (sequence = lane)
   int chunk;  // tiles per run
@@ -118,8 +124,21 @@ __device__ __forceinline__ Lengths read_lengths(const TreeArgs& a, int lane) {
   int sum = lane < a.batch ? tiles_of(a, r.first) : 0;
   for (int b = lane + 64; b < a.batch; b += 64) sum += tiles_of(a, context_length(a, b));
   const int total = __builtin_amdgcn_readlane(wave_prefix(sum), 63);
-  r.chunk = max(a.min_chunk, (total + a.runs - 1) / a.runs);
+  // One round of workgroups, unless that makes runs of less than 8 tiles: then about 128
+  // workgroups with runs of 4 to 16, as fewer partial results are worth more than idle CUs (D128
+  // Hkv8, split + combine: B4 64 rows L1024 20.4 -> 17.1 us, B8 128 rows L1024 33.9 -> 29.8; with
+  // longer runs for all that make less than 16, B4 128 rows L4096 37.2 -> 39.7).
+  r.chunk = (total + a.runs - 1) / a.runs;
+  if (r.chunk < 8) {
+    const int few = total >= a.many ? 16 : int(uint32_t(total * a.heads_blocks) / 128);
+    r.chunk = max(max(few, r.chunk), kMinChunk);
+  }
   return r;
+}
+
+// Runs of a sequence of `tiles` tiles.
+__device__ __forceinline__ int runs_of(const TreeArgs& a, const Lengths& n, int tiles) {
+  return tiles <= a.whole ? 1 : (tiles + n.chunk - 1) / n.chunk;
 }
 
 struct Run {
@@ -133,7 +152,7 @@ __device__ __forceinline__ bool find_run(const TreeArgs& a, const Lengths& n, in
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int b = b0 + lane;
     const int len = b0 == 0 ? n.first : (b < a.batch ? context_length(a, b) : 0);
-    const int mine = b < a.batch ? (tiles_of(a, len) + n.chunk - 1) / n.chunk : 0;
+    const int mine = b < a.batch ? runs_of(a, n, tiles_of(a, len)) : 0;
     const int upto = before + wave_prefix(mine);
     const uint64_t hit = __ballot(upto > f);
     if (hit != 0) {
@@ -157,7 +176,7 @@ __device__ __forceinline__ void sequence_runs(const TreeArgs& a, const Lengths& 
   for (int b0 = 0; b0 <= b; b0 += 64) {
     const int i = b0 + lane;
     const int len = b0 == 0 ? n.first : (i < a.batch ? context_length(a, i) : 0);
-    const int mine = i < a.batch ? (tiles_of(a, len) + n.chunk - 1) / n.chunk : 0;
+    const int mine = i < a.batch ? runs_of(a, n, tiles_of(a, len)) : 0;
     const int upto = before + wave_prefix(mine);
     if (b < b0 + 64) {
       out.splits = __builtin_amdgcn_readlane(mine, b - b0);
@@ -309,7 +328,8 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void tree_split_kernel(Tree
   const int b = run.b;
   const int context_tiles = (run.length + kTileKeys - 1) / kTileKeys;
   const int t0 = run.split * lengths.chunk;
-  const int t1 = min(t0 + lengths.chunk, context_tiles + a.tree_tiles);
+  const int tiles = context_tiles + a.tree_tiles;
+  const int t1 = run.splits == 1 ? tiles : min(t0 + lengths.chunk, tiles);
   const int c1 = min(t1, context_tiles);  // context tiles t0 .. c1-1, then drafted ones
   const int limit = min(run.length, c1 * kTileKeys);
 
@@ -918,19 +938,19 @@ void launch(const TreeArgs& a, bool combine, hipStream_t s) {
                        dim3(64 * kCombineWaves), 0, s, a);
 }
 
-// Tiles of the shortest run.
-constexpr int kMinChunk = 4;
-// A call of at most this many tiles per sequence is not split: writing and joining partial results
-// costs more than the tiles that runs of their own would save (a tile takes a workgroup about
-// 0.75 us; joining 5 us, and 10 us where there is a pair for every other CU and with it 8 MB of
-// partial results and more).
-int64_t whole_tiles(int64_t pairs) { return pairs >= 128 ? 20 : 8; }
+// A call of at most this many tiles per sequence is not split, by its pairs of a sequence's KV head
+// and a row block: writing and joining partial results costs more than the tiles that runs of their
+// own would save. D128 Hkv8, whole against split + combine: B16 (128 pairs) L1024 64 rows 24 against
+// 30 us, 128 rows 32 against 40, 256 rows 45 against 55; L2048 39 against 39, 52 against 49, 70
+// against 67. B4 and B8 L512 16 against 15 to 18, 21 against 21 to 24, 29 against 29 to 35; L1024
+// 24 against 20, 31 against 28, 42 against 38. B1 L256 11 to 15 against as much; L512 14 against 11.
+int64_t whole_tiles(int64_t pairs) { return pairs >= 128 ? 40 : pairs >= 32 ? 18 : 10; }
 
 // How the call is cut: runs (the tiles of all sequences over `runs` give the run length), the
 // bound on their number, row blocks. The sequences' last runs are shorter, so `runs` leaves room
 // for one more per sequence where that keeps the launch to one round of workgroups.
 struct Plan {
-  int64_t row_blocks, runs, flat, min_chunk;
+  int64_t row_blocks, runs, flat, whole;
   bool combine;
 };
 Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, int64_t nodes,
@@ -941,11 +961,14 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, i
   const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
   const int64_t base = shape.resident / (kv_heads * p.row_blocks);
   p.runs = base > 2 * batch ? base - batch + 1 : base > 1 ? base : 1;
-  const int64_t whole = whole_tiles(batch * kv_heads * p.row_blocks);
-  p.combine = most > whole;
-  p.min_chunk = p.combine ? kMinChunk : whole;
+  const int64_t pairs = batch * kv_heads * p.row_blocks;
+  p.whole = whole_tiles(pairs);
+  p.combine = most > p.whole;
+  // Where the lengths may ask for the combine kernel it runs in any case, and a short sequence is
+  // worth splitting unless there are workgroups enough without.
+  if (p.combine && pairs < 128) p.whole = 0;
   p.flat = p.runs + batch;
-  const int64_t bound = batch * tk::cdiv(most, p.min_chunk);
+  const int64_t bound = p.combine ? batch * tk::cdiv(most, kMinChunk) : batch;
   if (p.flat > bound) p.flat = bound;
   return p;
 }
@@ -1033,7 +1056,9 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
   a.rows = static_cast<int>(rows);
   a.max_len = static_cast<int>(max_len);
   a.tree_tiles = static_cast<int>(tk::cdiv(nodes, kTileKeys));
-  a.min_chunk = static_cast<int>(plan.min_chunk);
+  a.whole = static_cast<int>(plan.whole);
+  a.heads_blocks = static_cast<int>(kv_heads * plan.row_blocks);
+  a.many = static_cast<int>(tk::cdiv(16 * 128, kv_heads * plan.row_blocks));
   a.runs = static_cast<int>(plan.runs);
   a.row_blocks = static_cast<int>(plan.row_blocks);
   a.by_group = tk::FastDiv(static_cast<uint32_t>(group));
