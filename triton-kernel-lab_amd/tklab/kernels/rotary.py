@@ -82,7 +82,8 @@ def rotary_frequencies(
         return half * math.log(original_length / (turns * 2 * math.pi)) / math.log(base)
 
     low = max(math.floor(pair_turning(fast_turns)), 0)
-    high = min(math.ceil(pair_turning(slow_turns)), half - 1)
+    # The ramp may end past the last pair, which then turns more than slow_turns times.
+    high = min(math.ceil(pair_turning(slow_turns)), rotary_dim - 1)
     ramp = ((index - low) / max(high - low, 1e-3)).clamp(0, 1)
     return plain * (1 - ramp) + plain / factor * ramp, 0.1 * math.log(factor) + 1.0
 
