@@ -18,7 +18,7 @@ from tklab.kernels.rotary import rotary_frequencies
 
 CASES = [(dim, base, length)
          for dim, base in ((2, 1e4), (4, 1e4), (16, 1e4), (64, 1e4), (128, 1e4), (128, 5e5))
-         for length in (7, 64, 2048, 8192, 32768, 65536, 131072, 1048576)]
+         for length in (1, 3, 6, 7, 64, 2048, 8192, 32768, 65536, 131072, 1048576)]
 
 
 @pytest.mark.parametrize("factor", [4.0, 40.0])

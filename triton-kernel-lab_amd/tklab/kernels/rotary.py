@@ -84,7 +84,10 @@ def rotary_frequencies(
     low = max(math.floor(pair_turning(fast_turns)), 0)
     # The ramp may end past the last pair, which then turns more than slow_turns times.
     high = min(math.ceil(pair_turning(slow_turns)), rotary_dim - 1)
-    ramp = ((index - low) / max(high - low, 1e-3)).clamp(0, 1)
+    if high <= 0:  # no pair turns more than slow_turns times
+        ramp = torch.ones_like(index)
+    else:
+        ramp = ((index - low) / max(high - low, 1e-3)).clamp(0, 1)
     return plain * (1 - ramp) + plain / factor * ramp, 0.1 * math.log(factor) + 1.0
 
 
