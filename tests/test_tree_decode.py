@@ -284,6 +284,18 @@ def test_captured_calls_replay_with_other_lengths_on_another_stream() -> None:
             assert all(torch.equal(x, y) for x, y in zip(out, eager))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-60, 2.0 ** -149, 2.0 ** -103, -(2.0 ** -103), 2.0 ** -100])
+@pytest.mark.parametrize("dim,nodes,group", [(64, 6, 2), (128, 6, 2), (128, 40, 4)])
+def test_scales_of_nothing_and_next_to_nothing(scale, dim, nodes, group) -> None:
+    """Products of 2^100 and a scale that takes them to nothing, or to a handful."""
+    q, k, v, kt, vt = _problem(2, 2 * group, 2, nodes, 150, dim, torch.bfloat16, 14)
+    far = 2.0 ** 50
+    mask = tree_mask(_tree(nodes).cuda())
+    mask[nodes - 2] = False
+    _check(q * far, k * far, v, kt * far, vt, mask, _ints([150, 0]), scale=scale)
+
+
 # ------------------------------------------------------------------ without a GPU
 
 

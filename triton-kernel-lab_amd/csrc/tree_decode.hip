@@ -1065,8 +1065,10 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
   a.by_kv_heads = tk::FastDiv(static_cast<uint32_t>(kv_heads));
   a.by_row_blocks = tk::FastDiv(static_cast<uint32_t>(plan.row_blocks));
   a.flat = static_cast<int>(plan.flat);
-  // Not 0, which would turn a masked score (-inf) into NaN: 1e-30 leaves no score above 2^-20.
-  a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+  // Not 0, which would turn a masked score (-inf) into NaN: the least subnormal float (which the
+  // kernel's multiplications keep) leaves no score at or above 2^-149 * 2^128 = 2^-21, as good as 0
+  // to the hardware exponential. Scales this small are off by 2^-150, scores then by 2^-22.
+  a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 0x1p-149f);
   a.flip = scale < 0.f ? int(0x80008000u) : 0;
   hipStream_t s = tk::as_stream(stream);
   if (dtype == TK_DTYPE_BF16) {
