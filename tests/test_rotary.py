@@ -342,6 +342,25 @@ def test_refuses_rows_without_a_unit_stride() -> None:
         rotary_embedding(q, None, torch.arange(5, device="cuda"), freq)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dual", ["q", "k"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused_not_dropped(dual, grad) -> None:
+    """A tangent is an error, as it is for ``rope``, whether or not anything requires a gradient."""
+    from torch.autograd import forward_ad
+
+    x = {name: torch.randn(1, 2, 5, 8, device="cuda") for name in "qk"}
+    freq, _ = rotary_frequencies(8, device="cuda")
+    positions = torch.arange(5, device="cuda")
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        plain = rotary_embedding(x["q"], x["k"], positions, freq)
+        x[dual] = forward_ad.make_dual(x[dual], torch.ones_like(x[dual]))
+        with pytest.raises(RuntimeError, match="forward mode AD"):
+            rotary_embedding(x["q"], x["k"], positions, freq)
+    again = rotary_embedding(x["q"], x["k"], positions, freq)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+
+
 def test_plain_and_linear_frequencies() -> None:
     freq, magnitude = rotary_frequencies(8, base=10000.0)
     assert freq.dtype == torch.float64 and magnitude == 1.0

@@ -14,6 +14,7 @@ import math
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from tklab import _hip
@@ -118,13 +119,16 @@ def rotary_embedding(
     Returns:
         The turned ``q``, or ``(q, k)``, with the inputs' shape and memory order. Angles are
         float64, the rotation float32, rounded once to the dtype. Differentiable in ``q`` and
-        ``k``.
+        ``k``, in reverse mode only.
 
     Raises:
         ValueError: on an unsupported shape, dtype, layout or device.
+        RuntimeError: on a forward-mode tangent.
     """
     _validate(q, k, positions, frequencies)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    # Within a forward-mode level the inputs may carry tangents, which autograd's function refuses.
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            q.requires_grad or (k is not None and k.requires_grad)):
         out = _RotaryFunction.apply(q, k, positions, frequencies, interleaved, float(magnitude))
         return out if k is not None else out[0]
     turned_q, turned_k = _launch(q, k, positions, frequencies, interleaved, float(magnitude))
