@@ -188,3 +188,23 @@ def test_sizes_whose_product_overflows_are_rejected() -> None:
             values[1] = 0  # kind
         message = _rejected_before_launch(name, values)
         assert "too large" in message or "in range" in message or "columns" in message, message
+
+
+@pytest.mark.parametrize("name", sorted(n for n, kinds in _hip._SIGNATURES.items() if _hip._I64P in kinds))
+def test_stride_tables_are_typed(name: str) -> None:
+    """An entry point refuses an address or an array of another type where it reads int64_t[]; those
+    called with packed integers take these beside arrays."""
+    kinds = _hip._SIGNATURES[name]
+    bound = _hip._function(name).argtypes
+    for kind, argument in zip(kinds, bound):
+        if kind is not _hip._I64P:
+            assert argument is kind
+            continue
+        argument.from_param(_hip.int64_array([1, 2, 3]))
+        if name in _hip._PACKED_STRIDES:
+            argument.from_param(_hip.int64_bytes((1, 2, 3)))
+            continue
+        for wrong in (1 << 20, (ctypes.c_int32 * 3)(), b"12345678"):
+            with pytest.raises((TypeError, ctypes.ArgumentError)):
+                argument.from_param(wrong)
+    assert _hip._PACKED_STRIDES == {"tk_rotary", "tk_tree_decode", "tk_verify_draft", "tk_commit_draft"}

@@ -124,6 +124,9 @@ _SIGNATURES: dict[str, list[object]] = {
     "tk_roof_mfma": [_I32, _P, _I64, _I64, _P],
 }
 
+# Entry points whose int64_t[] arguments are called with packed integers (int64_bytes).
+_PACKED_STRIDES = frozenset({"tk_rotary", "tk_verify_draft", "tk_commit_draft", "tk_tree_decode"})
+
 # Queries: their int result is an answer, not a status.
 _QUERIES: dict[str, list[object]] = {
     "tk_gemm_tile": [_P, _P] + [_I64] * 7,
@@ -218,8 +221,11 @@ def _function(name: str) -> ctypes._CFuncPtr:
     if fn is None:
         fn = getattr(load_library(), name)
         fn.restype = ctypes.c_int
-        # Untyped pointers take arrays (int64_array) and packed integers (int64_bytes) alike.
-        fn.argtypes = [_P if kind is _I64P else kind for kind in _SIGNATURES[name]]
+        kinds = _SIGNATURES[name]
+        if name in _PACKED_STRIDES:
+            # Untyped pointers take arrays (int64_array) and packed integers alike.
+            kinds = [_P if kind is _I64P else kind for kind in kinds]
+        fn.argtypes = kinds
         _bound[name] = fn
     return fn
 
