@@ -374,3 +374,32 @@ def test_refuses_layouts_the_kernel_cannot_read() -> None:
         tree_decode(q, k, v, kt, vt, torch.ones(4, 8, dtype=torch.bool, device="cuda")[:, ::2])
     with pytest.raises(ValueError, match="cache_seqlens"):
         tree_decode(q, k, v, kt, vt, mask, torch.zeros(2, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.parametrize("sizes", [
+    (65535, 128, 1, 32, 1, 64),        # 2^23 workgroups
+    (1, 1, 1, 64, 257, 64),            # nodes
+    (65536, 1, 1, 64, 1, 64),          # sequences
+    (1, 65536, 1, 64, 1, 64),          # heads
+    (1, 2, 32768, 64, 1, 64),
+    (1, 1, 1, 2 ** 31 - 1, 1, 64),     # positions
+    (60000, 1, 1, 2 ** 21, 1, 64),     # tiles in all
+    (1, 1, 1, 64, 1, 96),              # head_dim
+    (0, 1, 1, 64, 1, 64),
+])
+def test_sizes_the_library_does_not_take_have_no_plan(sizes) -> None:
+    from tklab import _hip
+
+    assert _hip.query("tk_tree_decode_slots", *sizes) == -1
+
+
+@pytest.mark.gpu
+def test_too_many_workgroups_are_a_value_error() -> None:
+    def wide(*shape):
+        return torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda").expand(shape)
+
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="too large"):
+        tree_decode(wide(65535, 128, 1, 64), *(wide(65535, 128, 1, 64) for _ in range(4)),
+                    torch.ones(1, 1, dtype=torch.bool, device="cuda"))
+    assert torch.cuda.memory_allocated() <= before + 4096  # refused before the output is made

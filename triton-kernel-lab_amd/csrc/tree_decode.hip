@@ -973,15 +973,30 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_len, i
   return p;
 }
 
+// Why a problem of these (positive) sizes is not taken, or null. The grid holds at most 2^22
+// workgroups, and tiles and partial results are counted in 32 bits.
+const char* unsupported(int64_t batch, int64_t kv_heads, int64_t group, int64_t max_len,
+                        int64_t nodes, int64_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return "head_dim must be 64 or 128";
+  if (nodes > kMaxNodes) return "at most 256 nodes";
+  if (batch > 65535 || kv_heads > 65535 || group > 65535 || kv_heads * group > 65535 ||
+      max_len > INT32_MAX - 65536)
+    return "problem too large";
+  const Plan p = make_plan(batch, kv_heads, nodes * group, max_len, nodes, head_dim);
+  const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
+  if (batch * most > INT32_MAX / 2 || p.flat * kv_heads * p.row_blocks > (1 << 22))
+    return "problem too large";
+  return nullptr;
+}
+
 }  // namespace
 
 extern "C" int tk_tree_decode_slots(int64_t batch, int64_t kv_heads, int64_t group,
                                     int64_t max_len, int64_t nodes, int64_t head_dim) {
   if (batch <= 0 || kv_heads <= 0 || group <= 0 || max_len <= 0 || nodes <= 0) return -1;
+  if (unsupported(batch, kv_heads, group, max_len, nodes, head_dim) != nullptr) return -1;
   const Plan p = make_plan(batch, kv_heads, nodes * group, max_len, nodes, head_dim);
-  if (!p.combine) return 0;
-  const int64_t slots = p.flat * kv_heads;
-  return slots > INT32_MAX ? -1 : static_cast<int>(slots);
+  return p.combine ? static_cast<int>(p.flat * kv_heads) : 0;
 }
 
 extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, const void* v_cache,
@@ -1003,16 +1018,11 @@ extern "C" int tk_tree_decode(int dtype, const void* q, const void* k_cache, con
     return tk::fail("tree decode: null pointer");
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_len <= 0 || nodes <= 0)
     return tk::fail("tree decode: empty problem");
-  if (head_dim != 64 && head_dim != 128) return tk::fail("tree decode: head_dim must be 64 or 128");
   if (q_heads % kv_heads != 0) return tk::fail("tree decode: q_heads must be a multiple of kv_heads");
-  if (nodes > kMaxNodes) return tk::fail("tree decode: at most %d nodes", kMaxNodes);
-  if (batch > 65535 || q_heads > 65535 || max_len > INT32_MAX - 65536)
-    return tk::fail("tree decode: problem too large");
   const int64_t group = q_heads / kv_heads, rows = nodes * group;
-  const int64_t most = tk::cdiv(max_len, kTileKeys) + tk::cdiv(nodes, kTileKeys);
+  if (const char* why = unsupported(batch, kv_heads, group, max_len, nodes, head_dim))
+    return tk::fail("tree decode: %s", why);
   const Plan plan = make_plan(batch, kv_heads, rows, max_len, nodes, head_dim);
-  if (batch * most > INT32_MAX / 2 || plan.flat * kv_heads * plan.row_blocks > (1 << 22))
-    return tk::fail("tree decode: problem too large");
   if (plan.combine && workspace == nullptr) return tk::fail("tree decode: null pointer");
   for (const void* p : {q, k_cache, v_cache, k_tree, v_tree, static_cast<const void*>(o),
                         static_cast<const void*>(workspace)})
