@@ -402,3 +402,19 @@ def test_yarn_frequencies_keep_fast_pairs_and_slow_the_slow_ones() -> None:
 def test_refused_frequencies(kwargs, message) -> None:
     with pytest.raises(ValueError, match=message):
         rotary_frequencies(**kwargs)
+
+
+@pytest.mark.parametrize("q,k,positions,message", [
+    ((1, 65536, 1, 64), None, (1,), "65535 heads"),
+    ((1, 65000, 1, 64), (1, 600, 1, 64), (1,), "65535 heads"),
+    ((2, 65536, 64), None, (2,), "65535 heads"),
+    ((2 ** 31 - 65536, 1, 64), None, (2 ** 31 - 65536,), "tokens"),
+    ((2 ** 16, 1, 2 ** 15, 64), None, (2 ** 15,), "tokens"),
+])
+def test_sizes_past_the_librarys_counters_are_value_errors(q, k, positions, message) -> None:
+    def meta(shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    with pytest.raises(ValueError, match=message):
+        rotary_embedding(meta(q), None if k is None else meta(k), meta(positions, torch.int32),
+                         meta((32,), torch.float64))

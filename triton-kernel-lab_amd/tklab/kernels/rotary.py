@@ -22,6 +22,8 @@ from tklab import _hip
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _POSITION_DTYPES = (torch.int32, torch.int64)
 _MAX_HEAD_DIM = 1024
+_MAX_HEADS = 65535
+_MAX_TOKENS = 2**31 - 65537
 _SCALINGS = ("none", "linear", "ntk", "yarn")
 
 
@@ -106,7 +108,8 @@ def rotary_embedding(
     Args:
         q, k: ``[batch, heads, tokens, head_dim]``, or packed ``[tokens, heads, head_dim]``;
             float16, bfloat16 or float32, any strides with a contiguous last dimension, head
-            counts of their own. ``k`` may be ``None``. head_dim at most 1024.
+            counts of their own. ``k`` may be ``None``. head_dim at most 1024, 65535 heads in
+            all, 2**31 - 65537 tokens.
         positions: int32 or int64, ``[batch, tokens]`` or ``[tokens]`` (shared by the batch);
             ``[tokens]`` for packed tensors. Any value, negative ones included.
         frequencies: float64 ``[rotary_dim // 2]`` on the same device
@@ -256,7 +259,12 @@ def _validate(
             raise ValueError("q and k must share a dtype and a device")
     if dtype not in _DTYPES:
         raise ValueError("rotary_embedding supports float16, bfloat16 and float32 tensors")
-    wanted, given = (shape[0] if rank == 3 else shape[2],), positions.shape
+    tokens = shape[0] if rank == 3 else shape[2]
+    if shape[1] + (0 if k is None else k_shape[1]) > _MAX_HEADS:
+        raise ValueError(f"rotary_embedding supports at most {_MAX_HEADS} heads in all")
+    if tokens * (1 if rank == 3 else shape[0]) > _MAX_TOKENS:
+        raise ValueError(f"rotary_embedding supports at most {_MAX_TOKENS} tokens")
+    wanted, given = (tokens,), positions.shape
     if given != wanted and (rank == 3 or given != (shape[0], *wanted)):
         raise ValueError("positions must be [tokens]" + (" or [batch, tokens]" * (rank == 4)))
     if positions.dtype not in _POSITION_DTYPES:
