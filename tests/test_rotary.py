@@ -361,6 +361,23 @@ def test_forward_mode_is_refused_not_dropped(dual, grad) -> None:
     assert all(torch.equal(a, b) for a, b in zip(plain, again))
 
 
+@pytest.mark.gpu
+def test_more_token_runs_than_one_grid_dimension_holds() -> None:
+    """2^24 + 9 workgroups of a token each: rows of odd halves, which no vector divides. The input is
+    one token's row, the output 34 GB."""
+    tokens, period = 2 ** 24 + 9, 4096
+    q = torch.randn(1, 2, 514, device="cuda").bfloat16()
+    freq, _ = rotary_frequencies(514, device="cuda")
+    positions = torch.arange(tokens, dtype=torch.int32, device="cuda") % period
+    want = rotary_embedding(q.expand(period, -1, -1), None, positions[:period], freq)
+    out = rotary_embedding(q.expand(tokens, -1, -1), None, positions, freq)
+    assert out.shape == (tokens, 2, 514)
+    step = 64 * period
+    for t in range(0, tokens // step * step, step):
+        assert bool((out[t: t + step].view(64, period, 2, 514) == want).all())
+    assert torch.equal(out[-9:], want[:9])
+
+
 def test_plain_and_linear_frequencies() -> None:
     freq, magnitude = rotary_frequencies(8, base=10000.0)
     assert freq.dtype == torch.float64 and magnitude == 1.0

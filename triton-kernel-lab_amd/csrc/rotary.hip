@@ -135,7 +135,7 @@ struct Unit {
 template <typename T, int VEC, bool kInterleaved>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float table[];  // cos[block_tokens * half], then sin
-  const int t0 = blockIdx.x * a.block_tokens;
+  const int t0 = int(blockIdx.z * gridDim.x + blockIdx.x) * a.block_tokens;
   const int h0 = blockIdx.y * int(a.block_heads.d);
   const int angles = a.block_tokens * a.half;
   const uint32_t count = a.units.d * a.block_heads.d * uint32_t(a.block_tokens);
@@ -336,11 +336,15 @@ extern "C" int tk_rotary(int dtype, const void* q, void* q_out, const void* k, v
   a.magnitude = magnitude;
   a.pos64 = wide_positions;
   a.inverse = inverse;
-  const dim3 grid(static_cast<uint32_t>(tk::cdiv(total, block_tokens)),
-                  static_cast<uint32_t>(tk::cdiv(heads, block_heads)));
+  // A launch holds fewer than 2^32 threads in each dimension, so the runs of tokens spread over
+  // two. The last layer's last runs may lie past the tokens: fewer of them than layers, and two
+  // layers have runs of at most 2^7 tokens, so less than 2^10 tokens in all, within 32 bits.
+  const int64_t token_runs = tk::cdiv(total, block_tokens);
+  const int64_t layers = tk::cdiv(token_runs, (int64_t(1) << 24) - 1);
+  const dim3 grid(static_cast<uint32_t>(tk::cdiv(token_runs, layers)),
+                  static_cast<uint32_t>(tk::cdiv(heads, block_heads)),
+                  static_cast<uint32_t>(layers));
   const size_t lds = static_cast<size_t>(block_tokens) * half * 2 * sizeof(float);
-  // A launch holds fewer than 2^32 threads in each dimension.
-  if (grid.x >= (1u << 24)) return tk::fail("rotary: problem too large");
   hipStream_t s = tk::as_stream(stream);
   switch (dtype) {
     case TK_DTYPE_F32: launch_vec<float>(vec, a, interleaved != 0, grid, lds, s); break;
