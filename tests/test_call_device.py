@@ -49,3 +49,14 @@ def test_row_layout_packs_strides_and_refuses_rows_the_kernels_cannot_read() -> 
         _hip.row_layout(x[..., 1:], "x", -1)
     with pytest.raises(ValueError, match="16-byte aligned"):
         _hip.row_layout(torch.zeros(2, 3, 4, 60, dtype=torch.bfloat16), "x", -1)
+
+
+def test_row_layout_takes_any_stride_of_a_single_entry() -> None:
+    x = torch.zeros(4096, dtype=torch.bfloat16)
+    one = x.as_strided((1, 3, 1, 64), (1027, 128, 2 ** 24 + 8, 1))
+    address, strides = _hip.row_layout(one, "x", -1)
+    batch, head, row = memoryview(strides).cast("q")
+    assert address == x.data_ptr() and head == 128
+    assert batch % 8 == 0 and row % 8 == 0 and 0 <= batch < 2 ** 24 and 64 <= row < 2 ** 24
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        _hip.row_layout(x.as_strided((1, 3, 1, 64), (1027, 127, 5, 1)), "x", -1)

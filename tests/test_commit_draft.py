@@ -99,6 +99,14 @@ def test_a_captured_call_replays() -> None:
         assert torch.equal(ends, expected[2])
 
 
+@pytest.mark.gpu
+def test_strides_of_single_entries_do_not_matter() -> None:
+    """One sequence, head and node, as slices of wider tensors leave them."""
+    k, v, k_tree, v_tree = _problem(1, 1, 20, 1, 64, torch.bfloat16, 5)
+    odd = [t.as_strided(t.shape, (1027, 3, 64 if t.shape[2] > 1 else 77, 1)) for t in (k, v, k_tree, v_tree)]
+    _check(odd[0], odd[1], _ints([7]), odd[2], odd[3], _ints([[0]]), _ints([1]))
+
+
 # ------------------------------------------------------------------ without a GPU
 
 

@@ -296,6 +296,34 @@ def test_scales_of_nothing_and_next_to_nothing(scale, dim, nodes, group) -> None
     _check(q * far, k * far, v, kt * far, vt, mask, _ints([150, 0]), scale=scale)
 
 
+def _single(x, dim):
+    """x with an odd stride in a dimension of one entry, which no address uses."""
+    strides = list(x.stride())
+    assert x.shape[dim] == 1
+    strides[dim] = 2 ** 24 + 1027
+    return x.as_strided(x.shape, strides)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_strides_of_single_entries_do_not_matter(dim) -> None:
+    """One sequence, one head and one node, as slices of wider tensors leave them."""
+    mask = torch.ones(1, 1, dtype=torch.bool, device="cuda")
+    q, k, v, kt, vt = _problem(1, 4, 1, 1, 70, dim, torch.bfloat16, 15)
+    want, want_lse = _check(q, k, v, kt, vt, mask)
+    odd = [q, k, v, kt, vt]
+    for d in range(3):
+        odd = [_single(x, d) if x.shape[d] == 1 else x for x in odd]
+    out, lse = _check(*odd, mask)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    q, k, v, kt, vt = _problem(2, 4, 2, 3, 1, dim, torch.float16, 16)
+    _check(q, _single(k, 2), _single(v, 2), kt, vt, torch.ones(3, 3, dtype=torch.bool, device="cuda"), _ints([1, 0]))
+    # The output's memory order is still the queries'.
+    q, k, v, kt, vt = _problem(1, 4, 2, 3, 40, dim, torch.float16, 17)
+    out = tree_decode(_single(q, 0), k, v, kt, vt, torch.ones(3, 3, dtype=torch.bool, device="cuda"))
+    assert out.stride()[1:] == q.stride()[1:]
+
+
 # ------------------------------------------------------------------ without a GPU
 
 

@@ -260,12 +260,18 @@ def stream_on(device: int) -> int:
 
 def row_layout(tensor: torch.Tensor, name: str, device: int) -> tuple[int, bytes]:
     """Address and packed leading strides of a 4-D 16-bit tensor on GPU ``device``, whose rows must
-    be unit-stride and 16-byte aligned (``ValueError`` otherwise)."""
+    be unit-stride and 16-byte aligned (``ValueError`` otherwise).
+
+    No address uses the stride of a dimension with one entry, so any will do: one that the kernels
+    would refuse is replaced by the row length."""
     address, strides = tensor.data_ptr(), tensor.stride()
     if tensor.get_device() != device:
         raise ValueError(f"{name} must be on the other tensors' device")
     if strides[3] != 1:
         raise ValueError(f"{name} requires a contiguous final dimension")
+    if (strides[0] | strides[1] | strides[2]) & 7 or strides[2] >= 2**24:
+        shape = tensor.shape
+        strides = [shape[3] if shape[d] == 1 else strides[d] for d in range(3)]
     if (strides[0] | strides[1] | strides[2]) & 7 or address & 15:
         raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of 8)")
     return address, _PACKERS[3](strides[0], strides[1], strides[2])

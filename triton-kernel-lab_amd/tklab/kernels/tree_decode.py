@@ -94,10 +94,9 @@ def tree_decode(
     if slots < 0:
         raise ValueError("tree_decode: the problem is too large")
     out = torch.empty_like(q)
-    out_strides = out.stride()
-    if out_strides[3] != 1 or (out_strides[0] | out_strides[1] | out_strides[2]) & 7:
+    if out.stride(3) != 1:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        out_strides = out.stride()
+    out_ptr, out_strides = _hip.row_layout(out, "out", device)
     lse = workspace = None
     if return_lse:
         lse = torch.empty((batch, q_heads, nodes), dtype=torch.float32, device=q.device)
@@ -116,7 +115,7 @@ def tree_decode(
         vt_ptr,
         mask.data_ptr(),
         None if cache_seqlens is None else cache_seqlens.data_ptr(),
-        out.data_ptr(),
+        out_ptr,
         None if lse is None else lse.data_ptr(),
         None if workspace is None else workspace.data_ptr(),
         batch,
@@ -131,7 +130,7 @@ def tree_decode(
         kt_strides,
         vt_strides,
         _hip.int64_bytes((0 if len(mask_strides) == 2 else mask_strides[0], mask_strides[-2])),
-        _hip.int64_bytes(out_strides[:3]),
+        out_strides,
         head_dim ** -0.5 if scale is None else float(scale),
         _hip.stream_on(device),
     )
@@ -193,7 +192,7 @@ def _validate(
         raise ValueError("tree_decode requires CUDA (ROCm/HIP) tensors")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_tree", k_tree),
                     ("v_tree", v_tree)):
-        if t.stride(2) >= 2**24:
+        if t.stride(2) >= 2**24 and t.shape[2] > 1:
             raise ValueError(f"{name} key strides must be below 2**24 elements")
     device = q.get_device()
     if mask.get_device() != device or (nodes > 1 and mask.stride(-1) != 1):
