@@ -324,6 +324,54 @@ def test_strides_of_single_entries_do_not_matter(dim) -> None:
     assert out.stride()[1:] == q.stride()[1:]
 
 
+def _run_tiles(lengths, max_len, kv_heads, group, nodes, dim):
+    """Tiles of a run where one round of workgroups makes at least 8, from the library's plan."""
+    from tklab import _hip
+
+    batch = len(lengths)
+    slots = _hip.query("tk_tree_decode_slots", batch, kv_heads, group, max_len, nodes, dim)
+    runs = slots // kv_heads - batch
+    total = sum(-(-n // 32) + -(-nodes // 32) for n in lengths)
+    tiles = -(-total // runs)
+    assert tiles >= 8
+    return tiles
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("dim,nodes,group,lengths,kv_heads,tiles", [
+    # 256 rows at head_dim 128: two tiles a step, four steps in LDS.
+    (128, 64, 4, [9000], 8, 9),
+    (128, 64, 4, [11990], 8, 12),
+    (128, 64, 4, [17003], 8, 17),
+    (128, 64, 4, [33001], 8, 33),
+    # Waves without rows, and a second block with some.
+    (128, 33, 4, [20000], 8, 20),
+    (128, 48, 3, [14001], 8, 14),
+    (128, 65, 4, [9002], 8, 18),
+    # Runs that end a sequence, begin in its drafted tiles or hold nothing else.
+    (128, 64, 4, [30000, 0, 70000], 1, 13),
+    (128, 256, 1, [20001, 31, 40000, 1], 2, 16),
+    # The other shapes, past what their rings hold.
+    (64, 64, 4, [33001], 8, 17),
+    (64, 20, 4, [33001], 8, 17),
+    (64, 12, 4, [33001], 8, 17),
+    (128, 20, 4, [33001], 8, 17),
+    (128, 12, 4, [17003], 8, 9),
+    (128, 6, 4, [17003], 8, 9),
+    (128, 3, 4, [17003], 8, 9),
+])
+def test_runs_longer_than_the_ring(dtype, dim, nodes, group, lengths, kv_heads, tiles) -> None:
+    """Every slot of the ring in LDS is read, filled again and read again."""
+    max_len = max(lengths) + 5
+    assert _run_tiles(lengths, max_len, kv_heads, group, nodes, dim) == tiles
+    q, k, v, kt, vt = _problem(len(lengths), kv_heads * group, kv_heads, nodes, max_len, dim, dtype, 18)
+    k[0, :, lengths[0]:], v[0, :, lengths[0]:] = math.nan, math.nan
+    # A key of weight in every tile, so that a stale or missing tile shows.
+    v[:, :, ::32] += 4
+    _check(q, k, v, kt, vt, tree_mask(_tree(nodes).cuda()), _ints(lengths))
+
+
 # ------------------------------------------------------------------ without a GPU
 
 
