@@ -94,9 +94,14 @@ def tree_decode(
     if slots < 0:
         raise ValueError("tree_decode: the problem is too large")
     out = torch.empty_like(q)
-    if out.stride(3) != 1:
+    out_strides = out.stride()
+    if out_strides[3] != 1:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    out_ptr, out_strides = _hip.row_layout(out, "out", device)
+        out_strides = out.stride()
+    if (out_strides[0] | out_strides[1] | out_strides[2]) & 7:
+        out_strides = _hip.row_layout(out, "out", device)[1]
+    else:
+        out_strides = _hip.int64_bytes(out_strides[:3])
     lse = workspace = None
     if return_lse:
         lse = torch.empty((batch, q_heads, nodes), dtype=torch.float32, device=q.device)
@@ -115,7 +120,7 @@ def tree_decode(
         vt_ptr,
         mask.data_ptr(),
         None if cache_seqlens is None else cache_seqlens.data_ptr(),
-        out_ptr,
+        out.data_ptr(),
         None if lse is None else lse.data_ptr(),
         None if workspace is None else workspace.data_ptr(),
         batch,
