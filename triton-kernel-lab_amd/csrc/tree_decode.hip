@@ -16,7 +16,8 @@
 // the context or the tree lie outside the tile's buffer range and arrive as zeros.
 //
 // Softmax statistics and sums are float32, P is rounded to the storage dtype for the second
-// product (as in every attention of this library), O once at the end.
+// product (as in every attention of this library; bfloat16 results are 2.3e-3 from float64's instead
+// of 1.7e-3), O once at the end.
 //
 // Masked keys must not reach a row by way of 0 * inf or 0 * NaN in the second product. Past the
 // context's end V is zero; a drafted tile's V is checked, and if it holds an infinity or a NaN
@@ -31,10 +32,16 @@
 // short contexts the chain of latencies (2.5 us to find the run, 1.5 to the first tile, about 0.75
 // per tile, 1.5 and more for the partial results). B1 T8 G4 L2000 (32 rows): 9 + 4 us. B16 T16 G4
 // of lengths up to 8192 (64 rows, 304 MB): 57 + 6.4 us, 5.3 TB/s in the split kernel; equal lengths
-// of 8192 with 16 or 32 rows 6.3 to 6.5 TB/s. With 256 rows the matrix and vector work per tile:
-// B1 T64 G4 L131072 (538 MB, 137.5 GFLOP): 141 to 146 + 7.6 us, 0.95 PFLOP/s; of it 10 us before
-// the key loop and 6 to 10 behind it (33.5 MB of partial results). Half the LDS reads, or the same
-// tile read again and again, takes as long there; without the exponentials it is 8 % shorter.
+// of 8192 with 16 or 32 rows 6.3 to 6.5 TB/s. B1 T64 G4 L131072 (256 rows, 538 MB, 137.5 GFLOP):
+// 135 to 146 + 7.6 us, about 0.97 PFLOP/s; of it 10 us before the key loop (4 with fewer rows; what the
+// others consist of is not known) and 6 to 10 behind it (33.5 MB of partial results). No unit is full
+// there: of a wave's 269 k cycles the SIMD's matrix unit is busy 132 k, other vector instructions
+// issue for 95 k, and the wave stands ready but not issued 91 k and waits for reads or barriers 74 k.
+// Half the LDS reads, or the same tile read again and again, takes as long; without the exponentials
+// it is 8 % shorter. 129 to 192 rows take this shape too, idle waves multiplying zeros: 132 rows of
+// the same cache 131 to 138 + 6 us, 160 rows 134 to 139 + 6.3, 192 rows 138 to 142 + 6.9.
+// D64, same heads: B1 T64 L131072 (269 MB, 68.7 GFLOP) 88 to 91 + 8.2 us; B16 T16 L8192 (64 rows, 270 MB)
+// 52 + 6.1, ragged up to 8192 (152 MB) 34.6 + 5.6.
 // Measured and not kept: four waves of 64 rows, one per SIMD, with the exponentials of one tile
 // between the products of another (175 to 193 us: a wave issues in order, and its issue slots are
 // the bound); the DMA spread over the matrix phase (150 us against 147); default-policy loads
@@ -938,12 +945,16 @@ void launch(const TreeArgs& a, bool combine, hipStream_t s) {
                        dim3(64 * kCombineWaves), 0, s, a);
 }
 
-// A call of at most this many tiles per sequence is not split, by its pairs of a sequence's KV head
-// and a row block: writing and joining partial results costs more than the tiles that runs of their
+// A call whose caches hold at most this many tiles per sequence is not split, by its pairs of a
+// sequence's KV head and a row block (with 128 pairs and more no sequence of so few tiles is, however
+// long the cache): writing and joining partial results costs more than the tiles that runs of their
 // own would save. D128 Hkv8, whole against split + combine: B16 (128 pairs) L1024 64 rows 24 against
 // 30 us, 128 rows 32 against 40, 256 rows 45 against 55; L2048 39 against 39, 52 against 49, 70
 // against 67. B4 and B8 L512 16 against 15 to 18, 21 against 21 to 24, 29 against 29 to 35; L1024
 // 24 against 20, 31 against 28, 42 against 38. B1 L256 11 to 15 against as much; L512 14 against 11.
+// D64 B4 lengths 300 to 500, caches of 512 (whole) against 8192: 64 rows 11.8 against 8.2 + 4.0, 256
+// rows 24.3 against 19.8 + 5.8 (D128 13.8 against 10 + 4.4, 28 against 22.9 + 6.1). B16 is whole in
+// both: 12.6 against 12.7 + 3.4, the joining launch that finds nothing to join.
 int64_t whole_tiles(int64_t pairs) { return pairs >= 128 ? 40 : pairs >= 32 ? 18 : 10; }
 
 // How the call is cut: runs (the tiles of all sequences over `runs` give the run length), the

@@ -10,9 +10,11 @@
 //                     a token rejected once is not tried again).
 // The next token is then drawn from the current node's w = max(p - q, 0) after a rejection, p
 // without the rejected tokens, or p: the first v with w_0 + .. + w_v > u_0 sum(w). If w has no
-// mass, p stands in for it; if p has none either, the token is -1. All of it is float64 (a
-// difference or product of two float32 is exact there), so the result does not depend on how
-// the sums are split, except where a border lies within ~1e-15 of u_0 sum(w).
+// mass, p stands in for it; if p has none either, the token is -1. All of it is float64, where a
+// product of two float32 is exact and a difference is rounded once, by at most 2^-53 of it. The
+// sums' order depends on the splits: with c entries a split a sum passes through at most
+// c / 128 + 64 additions, so a border within (c / 128 + 64) 2^-52 sum(w) of u_0 sum(w) may fall to
+// either side (2^-45 of the sum where c is 8192).
 //
 // The children test a probability each, known from parents and tokens alone, so one wave
 // gathers all nodes' at once and walks in registers: the path costs two trips to memory. Then

@@ -67,7 +67,8 @@ def tree_decode(
         k_tree, v_tree: ``[batch, kv_heads, nodes, head_dim]``, the drafted tokens' own.
         mask: bool ``[nodes, nodes]`` or ``[batch, nodes, nodes]``: ``mask[i, j]`` lets node
             ``i`` see node ``j``. A key that a node does not see cannot reach its result, whatever
-            it holds (infinities and NaN included).
+            it holds (infinities and NaN included; cache positions that share memory with a seen
+            one must hold finite values).
         cache_seqlens: optional int32 ``[batch]`` context lengths, clamped to ``[0, max_len]``;
             ``None`` means every sequence has ``max_len`` keys.
         scale: score scale, default ``1 / sqrt(head_dim)``.
