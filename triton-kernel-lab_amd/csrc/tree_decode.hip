@@ -33,15 +33,16 @@
 // per tile, 1.5 and more for the partial results). B1 T8 G4 L2000 (32 rows): 9 + 4 us. B16 T16 G4
 // of lengths up to 8192 (64 rows, 304 MB): 57 + 6.4 us, 5.3 TB/s in the split kernel; equal lengths
 // of 8192 with 16 or 32 rows 6.3 to 6.5 TB/s. B1 T64 G4 L131072 (256 rows, 538 MB, 137.5 GFLOP):
-// 135 to 146 + 7.6 us, about 0.97 PFLOP/s; of it 10 us before the key loop (4 with fewer rows; what the
-// others consist of is not known) and 6 to 10 behind it (33.5 MB of partial results). No unit is full
-// there: of a wave's 269 k cycles the SIMD's matrix unit is busy 132 k, other vector instructions
-// issue for 95 k, and the wave stands ready but not issued 91 k and waits for reads or barriers 74 k.
-// Half the LDS reads, or the same tile read again and again, takes as long; without the exponentials
-// it is 8 % shorter. 129 to 192 rows take this shape too, idle waves multiplying zeros: 132 rows of
-// the same cache 131 to 138 + 6 us, 160 rows 134 to 139 + 6.3, 192 rows 138 to 142 + 6.9.
-// D64, same heads: B1 T64 L131072 (269 MB, 68.7 GFLOP) 88 to 91 + 8.2 us; B16 T16 L8192 (64 rows, 270 MB)
-// 52 + 6.1, ragged up to 8192 (152 MB) 34.6 + 5.6.
+// 135 to 146 + 7.6 us, about 0.97 PFLOP/s; of it 10 us before the key loop (4 with fewer rows; what
+// the others consist of is not known) and 6 to 10 behind it (33.5 MB of partial results). No unit is
+// full there: of a wave's 269 k cycles the SIMD's matrix unit is busy 132 k, other vector
+// instructions issue for 95 k, and the wave stands ready but not issued for 91 k and waits for reads
+// or barriers for 74 k. Half the LDS reads, or the same tile read again and again, takes as long;
+// without the exponentials it is 8 % shorter. 129 to 192 rows take this shape too, idle waves
+// multiplying zeros: 132 rows of the same cache 131 to 138 + 6 us, 160 rows 134 to 137 + 6.3, 192
+// rows 136 to 138 + 6.9.
+// D64, same heads: B1 T64 L131072 (269 MB, 68.7 GFLOP) 88 to 91 + 8.2 us; B16 T16 L8192 (64 rows,
+// 270 MB) 52 + 6, ragged up to 8192 (152 MB) 34.6 + 5.5.
 // Measured and not kept: four waves of 64 rows, one per SIMD, with the exponentials of one tile
 // between the products of another (175 to 193 us: a wave issues in order, and its issue slots are
 // the bound); the DMA spread over the matrix phase (150 us against 147); default-policy loads
