@@ -481,6 +481,34 @@ int tk_commit_draft(int dtype, void* k_cache, void* v_cache, const void* k_tree,
                     const int64_t* k_cache_strides, const int64_t* v_cache_strides,
                     const int64_t* k_tree_strides, const int64_t* v_tree_strides, void* stream);
 
+/* Norms of queries and keys for each head with rotary positions in the same pass. Every row (head of
+ * a token) becomes y = R z, z = x w / sqrt(mean(x^2) + eps), R the rotation of tk_rotary over the
+ * first rotary_dim features (z is copied behind them). Arguments as tk_rotary's; q_weight and
+ * k_weight hold head_dim entries of the storage dtype. k may be NULL (with what belongs to it);
+ * head_dim <= 512, heads <= 65535 a side. Statistics and angles as in tk_rotary: float32 and float64. */
+int tk_qk_norm_rotary(int dtype, const void* q, void* q_out, const void* k, void* k_out,
+                      const void* q_weight, const void* k_weight, const void* positions,
+                      const double* frequencies, int64_t batch, int64_t tokens, int64_t q_heads,
+                      int64_t kv_heads, int64_t head_dim, int64_t rotary_dim,
+                      const int64_t* q_strides, const int64_t* q_out_strides,
+                      const int64_t* k_strides, const int64_t* k_out_strides,
+                      const int64_t* position_strides, float eps, float magnitude, int interleaved,
+                      int wide_positions, void* stream);
+
+/* Its gradients from q, k and the outputs' gradients: dq, dk (strides of their own) and the weights'
+ * (head_dim entries of the storage dtype), summed in a fixed order. `partials`: float32
+ * [1024][head_dim], overwritten. Two launches. */
+int tk_qk_norm_rotary_bwd(int dtype, const void* q, const void* dq_out, void* dq, const void* k,
+                          const void* dk_out, void* dk, const void* q_weight, const void* k_weight,
+                          void* dq_weight, void* dk_weight, float* partials, const void* positions,
+                          const double* frequencies, int64_t batch, int64_t tokens,
+                          int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim,
+                          const int64_t* q_strides, const int64_t* dq_out_strides,
+                          const int64_t* dq_strides, const int64_t* k_strides,
+                          const int64_t* dk_out_strides, const int64_t* dk_strides,
+                          const int64_t* position_strides, float eps, float magnitude,
+                          int interleaved, int wide_positions, void* stream);
+
 /* ---- Calibration kernels (no counterpart in the reference). They measure the
  * roofs this GPU sustains, so that the kernels above can be priced against
  * measured ceilings beside the published peaks. */

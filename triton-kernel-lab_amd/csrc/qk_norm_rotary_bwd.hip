@@ -1,0 +1,220 @@
+// Gradients of the norms of queries and keys with rotary positions (qk_norm_rotary.hip). Per row,
+// with r = 1 / sqrt(mean(x^2) + eps) and dz = R^T dy (the rotation by the negative angle):
+//   dw += dz x r (over the side's rows),  g = dz w,  dx = r (g - x r^2 mean(g x)).
+// x and dy are read and dx written once; r is formed again from x rather than kept from the forward
+// (the row is there in any case), and both of a row's sums are reduced together.
+//
+// dw: every workgroup walks its side's runs in a fixed order, sums in registers (a lane's features
+// are the same in every row), folds its rows' lanes in LDS and writes one float32 row of partial
+// sums; a second kernel adds those rows in a fixed order. Results do not depend on timing.
+//
+// Bound by HBM.
+#include "qk_norm_rotary.hpp"
+
+namespace tk_qk_norm {
+
+template <typename T, int VEC, int NU, bool kInterleaved>
+__global__ __launch_bounds__(kThreads) void qk_norm_rotary_bwd_kernel(Args a) {
+  using R = Row<T, VEC, NU, kInterleaved>;
+  constexpr int PER = NU * R::N;    // sums per lane
+  extern __shared__ float shared[];  // cos, sin of a run; then the lanes' sums
+  const int w = blockIdx.x >= a.side[0].groups;
+  const uint32_t group = blockIdx.x - (w ? a.side[0].groups : 0);
+  const Side& s = a.side[w];
+  float* cosv = shared;
+  float* sinv = shared + s.block_tokens * a.half;
+
+  const int lanes = 1 << a.lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1);
+  const uint32_t step = kThreads >> a.lanes_log2;  // rows at a time
+  const typename R::Layout layout(a, lane);
+  float g[NU][R::N], sum[NU][R::N];
+  R::load_weight(s.weight, layout, g);
+#pragma unroll
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int k = 0; k < R::N; ++k) sum[i][k] = 0.f;
+
+  for (uint32_t j = group; j < s.runs; j += s.groups) {
+    const Run run(a, s, j);
+    uint32_t p = threadIdx.x >> a.lanes_log2;
+    Run::At here;
+    bool live = run.at(a, s, p, here);
+    typename R::Raw x, dy;
+    if (live) {
+      x.load(static_cast<const T*>(s.x) + offset(s.xs, here), layout);
+      dy.load(static_cast<const T*>(s.dy) + offset(s.ys, here), layout);
+    }
+    __syncthreads();  // the last run's angles have been read
+    fill_angles(a, s, run.t0, cosv, sinv);
+    __syncthreads();
+    while (p < run.count) {
+      Run::At next;
+      typename R::Raw x_ahead, dy_ahead;
+      const bool next_live = run.at(a, s, p + step, next);
+      if (next_live) {
+        x_ahead.load(static_cast<const T*>(s.x) + offset(s.xs, next), layout);
+        dy_ahead.load(static_cast<const T*>(s.dy) + offset(s.ys, next), layout);
+      }
+      float f[NU][R::N], d[NU][R::N];
+      x.expand(layout, f);
+      dy.expand(layout, d);
+      float square = 0.f, dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        if (layout.angle[i] >= 0 && live) {
+          const int at = here.token * a.half + layout.angle[i];
+#pragma unroll
+          for (int k = 0; k < R::PAIRS; ++k) {
+            const float c = cosv[at + k], sn = sinv[at + k];
+            const float d1 = d[i][R::first(k)], d2 = d[i][R::second(k)];
+            d[i][R::first(k)] = d1 * c + d2 * sn;
+            d[i][R::second(k)] = d2 * c - d1 * sn;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < R::N; ++k) {
+          square = fmaf(f[i][k], f[i][k], square);
+          dot = fmaf(d[i][k] * g[i][k], f[i][k], dot);
+        }
+      }
+      square = row_sum(square, a.lanes_log2);
+      dot = row_sum(dot, a.lanes_log2);
+      const float inverse = 1.0f / sqrtf(fmaf(square, a.inv_dim, a.eps));
+      const float share = dot * inverse * inverse * a.inv_dim;
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+          for (int k = 0; k < R::N; ++k) {
+            sum[i][k] = fmaf(d[i][k], f[i][k] * inverse, sum[i][k]);
+            f[i][k] = inverse * (d[i][k] * g[i][k] - f[i][k] * share);
+          }
+        R::store(static_cast<T*>(s.out) + offset(s.os, here), layout, f);
+      }
+      x = x_ahead;
+      dy = dy_ahead;
+      live = next_live;
+      here = next;
+      p += step;
+    }
+  }
+
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int k = 0; k < R::N; ++k) shared[threadIdx.x * PER + i * R::N + k] = sum[i][k];
+  __syncthreads();
+  float* out = a.partials + int64_t(blockIdx.x) * a.head_dim;
+  for (int e = threadIdx.x; e < lanes * PER; e += kThreads) {
+    const int owner = e / PER, i = e % PER / R::N, k = e % R::N;
+    const typename R::Layout at(a, owner);
+    int col = -1;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      if (n != i || at.col[n] < 0) continue;
+      if (!R::TWO || k < VEC)
+        col = at.col[n] + k;
+      else if (at.angle[n] >= 0)
+        col = at.col[n] + at.gap + k - VEC;
+    }
+    if (col < 0) continue;
+    float v = 0.f;
+    for (uint32_t row = 0; row < step; ++row) v += shared[row * lanes * PER + e];
+    out[col] = v;
+  }
+}
+
+// Sums of the partial rows: 32 features by 32 slices of the rows a workgroup.
+constexpr int kCols = 32, kSlices = 32;
+template <typename T>
+__global__ __launch_bounds__(kCols* kSlices) void qk_norm_weight_kernel(Args a) {
+  __shared__ float part[kSlices][kCols + 1];
+  const int w = blockIdx.y;
+  const Side& s = a.side[w];
+  const int col = blockIdx.x * kCols + threadIdx.x % kCols, slice = threadIdx.x / kCols;
+  const float* rows = a.partials + (w ? int64_t(a.side[0].groups) * a.head_dim : 0);
+  float v = 0.f;
+  if (col < a.head_dim)
+    for (uint32_t r = slice; r < s.groups; r += kSlices) v += rows[int64_t(r) * a.head_dim + col];
+  part[slice][threadIdx.x % kCols] = v;
+  __syncthreads();
+  if (slice == 0 && col < a.head_dim) {
+    for (int i = 1; i < kSlices; ++i) v += part[i][threadIdx.x];
+    static_cast<T*>(s.dweight)[col] = tk::from_f32<T>(v);
+  }
+}
+
+template <typename T, int VEC, int NU>
+static void launch(const Args& a, bool interleaved, hipStream_t s) {
+  const int block_tokens = a.side[0].block_tokens > a.side[1].block_tokens ? a.side[0].block_tokens
+                                                                           : a.side[1].block_tokens;
+  size_t lds = static_cast<size_t>(block_tokens) * a.half * 2 * sizeof(float);
+  const size_t sums = sizeof(float) * kThreads * NU * Row<T, VEC, NU, false>::N;
+  if (lds < sums) lds = sums;
+  const dim3 grid(a.side[0].groups + a.side[1].groups);
+  if (interleaved)
+    hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, VEC, NU, true>), grid, dim3(kThreads), lds, s, a);
+  else
+    hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, VEC, NU, false>), grid, dim3(kThreads), lds, s, a);
+}
+
+template <typename T>
+static void launch_all(int vec, int nu, const Args& a, bool interleaved, hipStream_t s) {
+#define TK_LAUNCH(T, V, N) launch<T, V, N>(a, interleaved, s)
+  TK_QK_NORM_VARIANTS(T, vec, nu, TK_LAUNCH)
+#undef TK_LAUNCH
+  hipLaunchKernelGGL((qk_norm_weight_kernel<T>),
+                     dim3(static_cast<uint32_t>(tk::cdiv(a.head_dim, kCols)), a.side[1].groups ? 2 : 1),
+                     dim3(kCols * kSlices), 0, s, a);
+}
+
+}  // namespace tk_qk_norm
+
+extern "C" int tk_qk_norm_rotary_bwd(
+    int dtype, const void* q, const void* dq_out, void* dq, const void* k, const void* dk_out,
+    void* dk, const void* q_weight, const void* k_weight, void* dq_weight, void* dk_weight,
+    float* partials, const void* positions, const double* frequencies, int64_t batch,
+    int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim,
+    const int64_t* q_strides, const int64_t* dq_out_strides, const int64_t* dq_strides,
+    const int64_t* k_strides, const int64_t* dk_out_strides, const int64_t* dk_strides,
+    const int64_t* position_strides, float eps, float magnitude, int interleaved,
+    int wide_positions, void* stream) {
+  using namespace tk_qk_norm;
+  const void* pointers[2][4] = {{q, dq_out, dq, q_weight}, {k, dk_out, dk, k_weight}};
+  const Tables tables[2] = {{q_strides, dq_out_strides, dq_strides},
+                            {k_strides, dk_out_strides, dk_strides}};
+  if (tk::valid_dtype(dtype) && (dq_out_strides == nullptr || partials == nullptr ||
+                                 dq_weight == nullptr || (k != nullptr && dk_weight == nullptr)))
+    return tk::fail("qk norm: null pointer");
+  Args a;
+  int vec, nu;
+  if (plan(dtype, pointers, tables, positions, frequencies, batch, tokens, q_heads, kv_heads,
+           head_dim, rotary_dim, position_strides, eps, magnitude, interleaved, wide_positions, a,
+           vec, nu))
+    return 1;
+  if (reinterpret_cast<uintptr_t>(partials) % 4 != 0)
+    return tk::fail("qk norm: tensors must be aligned to their dtype");
+  for (const void* p : {dq_weight, k != nullptr ? dk_weight : dq_weight})
+    if (reinterpret_cast<uintptr_t>(p) % tk::elem_size(dtype) != 0)
+      return tk::fail("qk norm: tensors must be aligned to their dtype");
+  a.partials = partials;
+  a.side[0].dweight = dq_weight;
+  a.side[1].dweight = k != nullptr ? dk_weight : dq_weight;
+  // The workgroups are shared out by the sides' runs.
+  const int64_t all = int64_t(a.side[0].runs) + a.side[1].runs;
+  for (int w = 0; w < 2; ++w) {
+    Side& s = a.side[w];
+    int64_t groups = all <= kGroups ? s.runs : int64_t(kGroups) * s.runs / all;
+    if (groups < 1 && s.runs > 0) groups = 1;
+    s.groups = static_cast<uint32_t>(groups);
+  }
+  hipStream_t s = tk::as_stream(stream);
+  switch (dtype) {
+    case TK_DTYPE_F32: launch_all<float>(vec, nu, a, interleaved != 0, s); break;
+    case TK_DTYPE_F16: launch_all<_Float16>(vec, nu, a, interleaved != 0, s); break;
+    default: launch_all<__bf16>(vec, nu, a, interleaved != 0, s); break;
+  }
+  return tk::check_launch("qk norm backward");
+}

@@ -16,6 +16,7 @@
 // Bound by HBM: q and k are read and written once. B2 N8192 Hq32 Hkv8 D128 bf16 (336 MB a pass):
 // 60 us, 5.6 TB/s, with about four units a thread and non-temporal accesses; two units 65 us, eight
 // 66, plain loads 64. One token of the same heads: 2.9 us.
+#include "rotary_angles.hpp"
 #include "tk_common.hpp"
 
 namespace {
@@ -39,24 +40,6 @@ struct RotaryArgs {
   float magnitude;
   int pos64, inverse;
 };
-
-// sin and cos of r in [-pi/4, pi/4] by their Taylor series (coefficients 1/n!).
-__device__ __forceinline__ void sincos_reduced(double r, double& s, double& c) {
-  const double z = r * r;
-  double p = -1.0 / 39916800.0;
-  p = fma(p, z, 1.0 / 362880.0);
-  p = fma(p, z, -1.0 / 5040.0);
-  p = fma(p, z, 1.0 / 120.0);
-  p = fma(p, z, -1.0 / 6.0);
-  s = fma(p * z, r, r);
-  double q = 1.0 / 479001600.0;
-  q = fma(q, z, -1.0 / 3628800.0);
-  q = fma(q, z, 1.0 / 40320.0);
-  q = fma(q, z, -1.0 / 720.0);
-  q = fma(q, z, 1.0 / 24.0);
-  q = fma(q, z, -0.5);
-  c = fma(q, z, 1.0);
-}
 
 // Features of one unit: a rotated unit of the halves layout is VEC pairs (two vectors), one of
 // the interleaved layout a vector of VEC / 2 pairs (a single pair for VEC 1); a unit past the
@@ -161,27 +144,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     const double pos = a.pos64 ? double(static_cast<const int64_t*>(a.positions)[at])
                                : double(static_cast<const int32_t*>(a.positions)[at]);
     const double x = pos * a.frequencies[pair];
-    // x = k pi/2 + r; pi/2 in two parts, the first with all 53 bits. Past 2^51 the rounding of
-    // x * 2/pi is off by whole quarter turns: the second pass takes off those that are left.
-    const double k = rint(x * 0.63661977236758134308);
-    double r = fma(k, -1.5707963267948965580, x);
-    r = fma(k, -6.1232339957367658e-17, r);
-    const double more = rint(r * 0.63661977236758134308);
-    r = fma(more, -1.5707963267948965580, r);
-    r = fma(more, -6.1232339957367658e-17, r);
     double s, c;
-    sincos_reduced(r, s, c);
-    // k modulo 4 is exact for every finite k.
-    const int quarter = int(k - 4.0 * floor(0.25 * k)) + int(more);
-    if (quarter & 1) {
-      const double swap = s;
-      s = c;
-      c = -swap;
-    }
-    if (quarter & 2) {
-      s = -s;
-      c = -c;
-    }
+    tk_rotary_angles::sincos_any(x, s, c);
     const double m = a.magnitude;
     cosv[i] = float(c * m);
     sinv[i] = float(a.inverse ? -s * m : s * m);

@@ -11,6 +11,7 @@ import ctypes
 import os
 import struct
 import threading
+from functools import lru_cache
 from pathlib import Path
 
 import torch
@@ -119,6 +120,10 @@ _SIGNATURES: dict[str, list[object]] = {
         _I64P, _P,
     ],
     "tk_tree_decode": [_I32] + [_P] * 10 + [_I64] * 6 + [_I64P] * 7 + [_F32, _P],
+    "tk_qk_norm_rotary": [_I32] + [_P] * 8 + [_I64] * 6 + [_I64P] * 5 + [_F32, _F32, _I32, _I32, _P],
+    "tk_qk_norm_rotary_bwd": (
+        [_I32] + [_P] * 13 + [_I64] * 6 + [_I64P] * 7 + [_F32, _F32, _I32, _I32, _P]
+    ),
     "tk_roof_copy": [_P, _P, _I64, _P],
     "tk_roof_stream": [_P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _P],
     "tk_roof_mfma": [_I32, _P, _I64, _I64, _P],
@@ -202,6 +207,12 @@ def int64_array(values: tuple[int, ...] | list[int]) -> ctypes.Array[ctypes.c_in
     """Pack integers into a C ``int64_t[]``."""
     n = len(values)
     return (_INT64_ARRAYS[n] if n < 5 else ctypes.c_int64 * n)(*values)
+
+
+@lru_cache(maxsize=4096)
+def int64_table(values: tuple[int, ...]) -> ctypes.Array[ctypes.c_int64]:
+    """:func:`int64_array` of the same integers, made once (entry points only read them)."""
+    return int64_array(values)
 
 
 _PACKERS = tuple(struct.Struct(f"{n}q").pack for n in range(5))
