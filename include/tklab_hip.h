@@ -509,6 +509,49 @@ int tk_qk_norm_rotary_bwd(int dtype, const void* q, const void* dq_out, void* dq
                           const int64_t* position_strides, float eps, float magnitude,
                           int interleaved, int wide_positions, void* stream);
 
+/* Keys and values appended to caches held in 8 bits (cache_type 0: float8 e4m3, finite; 1: int8). Row
+ * t < counts[b] (NULL: tokens) of every KV head becomes row seqlens[b] + t of the caches: with
+ * a = max(max |x|, 2^-100) and M = 448 or 127, codes round(x (M (1 / a))) to nearest even and the scale
+ * a / M (a row with an infinity or a NaN: codes 0, scale NaN), scales[b][h][l] = {key's, value's}.
+ * Rows past max_len are not written; new_seqlens[b] = min(seqlens[b] + counts[b], max_len), seqlens
+ * and counts clamped to [0, max_len] and [0, tokens]. Strides {batch, head, position} in elements;
+ * rows of k, v and the caches 16-byte aligned, pairs of scales 8-byte; head_dim a multiple of 16, at
+ * most 1024. */
+int tk_append_quantized(int dtype, void* k_cache, void* v_cache, float* scales,
+                        const int32_t* seqlens, const void* k, const void* v,
+                        const int32_t* counts, int32_t* new_seqlens, int64_t batch,
+                        int64_t kv_heads, int64_t max_len, int64_t tokens, int64_t head_dim,
+                        const int64_t* k_cache_strides, const int64_t* v_cache_strides,
+                        const int64_t* scale_strides, const int64_t* k_strides,
+                        const int64_t* v_strides, int cache_type, void* stream);
+
+/* Such caches read back: k and v, contiguous [batch][kv_heads][max_len][head_dim] of the dtype, get
+ * code * scale below seqlens[b] (NULL: max_len) and zeros from there on. */
+int tk_read_quantized(int dtype, const void* k_cache, const void* v_cache, const float* scales,
+                      const int32_t* seqlens, void* k, void* v, int64_t batch, int64_t kv_heads,
+                      int64_t max_len, int64_t head_dim, const int64_t* k_cache_strides,
+                      const int64_t* v_cache_strides, const int64_t* scale_strides, int cache_type,
+                      void* stream);
+
+/* tk_gqa_decode over such caches, any q_heads / kv_heads: q and o [batch][q_heads][head_dim] with
+ * strides {batch, head} in multiples of 8 elements, caches {batch, head, position} in multiples of
+ * 16, key strides below 2^24, bases 16-byte aligned; dtype F16 or BF16, head_dim 64 or 128. `lse`
+ * (nullable) float32 [batch][q_heads], base 2; a sequence without keys gets 0 and -inf.
+ * `workspace`: tk_quantized_decode_slots(...) * (q_heads / kv_heads) * (head_dim + 2) floats,
+ * 16-byte aligned, overwritten (NULL when that is 0). At most two launches. */
+int tk_quantized_decode(int dtype, const void* q, const void* k_cache, const void* v_cache,
+                        const float* scales, const int32_t* seqlens, void* o, float* lse,
+                        float* workspace, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                        int64_t max_len, int64_t head_dim, const int64_t* q_strides,
+                        const int64_t* k_strides, const int64_t* v_strides,
+                        const int64_t* scale_strides, const int64_t* o_strides, float scale,
+                        int cache_type, void* stream);
+
+/* Partial results that tk_quantized_decode keeps per head of a group for these sizes (group =
+ * q_heads / kv_heads); -1 for sizes it does not take. No launch, no GPU. */
+int tk_quantized_decode_slots(int64_t batch, int64_t kv_heads, int64_t group, int64_t max_len,
+                              int64_t head_dim);
+
 /* ---- Calibration kernels (no counterpart in the reference). They measure the
  * roofs this GPU sustains, so that the kernels above can be priced against
  * measured ceilings beside the published peaks. */

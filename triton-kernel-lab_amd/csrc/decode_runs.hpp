@@ -1,0 +1,132 @@
+// Runs of key tiles for the decode kernels over caches whose lengths only the device knows: the
+// tiles of all sequences are dealt in equal runs, found by every workgroup from the lengths, so a
+// ragged batch fills the chip; and the joining of the runs' partial results.
+#pragma once
+#include "attention_dma.hpp"
+#include "tk_common.hpp"
+
+namespace tk_runs {
+
+constexpr int kTileKeys = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+// The running maximum before any key: finite, so that a masked score (-inf) minus it stays
+// -inf, and below every score that carries weight.
+constexpr float kNoMax = -3.0e38f;
+
+struct Schedule {
+  const int32_t* seqlens;  // null: every sequence has max_len keys
+  int batch, max_len;
+  int runs;       // the tiles of all sequences over this many runs give the run length
+  int min_chunk;  // tiles of the shortest run of a sequence that is split
+  int whole;      // a sequence of at most this many tiles is one run
+};
+
+__device__ __forceinline__ int context_length(const Schedule& s, int b) {
+  const int n = s.seqlens != nullptr ? s.seqlens[b] : s.max_len;
+  return min(max(n, 0), s.max_len);
+}
+
+// At least one tile (an empty one writes the result of no keys).
+__device__ __forceinline__ int tiles_of(int length) {
+  return max((length + kTileKeys - 1) / kTileKeys, 1);
+}
+
+// Inclusive prefix sums over the wave's lanes: within rows of 16 lanes by shifts, then the rows'
+// and the halves' last sums broadcast to the next ones.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_part(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += dpp_part<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v += dpp_part<0x112, 0xF>(v);
+  v += dpp_part<0x114, 0xF>(v);
+  v += dpp_part<0x118, 0xF>(v);
+  v += dpp_part<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp_part<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+struct Lengths {
+  int first;  // this lane's sequence's length (sequence = lane)
+  int chunk;  // tiles per run
+};
+
+__device__ __forceinline__ Lengths read_lengths(const Schedule& s, int lane) {
+  Lengths r;
+  r.first = lane < s.batch ? context_length(s, lane) : 0;
+  int sum = lane < s.batch ? tiles_of(r.first) : 0;
+  for (int b = lane + 64; b < s.batch; b += 64) sum += tiles_of(context_length(s, b));
+  const int total = __builtin_amdgcn_readlane(wave_prefix(sum), 63);
+  r.chunk = max((total + s.runs - 1) / s.runs, s.min_chunk);
+  return r;
+}
+
+__device__ __forceinline__ int runs_of(const Schedule& s, int chunk, int tiles) {
+  return tiles <= s.whole ? 1 : (tiles + chunk - 1) / chunk;
+}
+
+struct Run {
+  int b, length, split, splits, flat0;  // flat0: the sequence's first flat run
+};
+
+// Sequence and split of flat run f (all wave-uniform); false past the last.
+__device__ __forceinline__ bool find_run(const Schedule& s, const Lengths& n, int f, int lane,
+                                         Run& out) {
+  int before = 0;
+  for (int b0 = 0; b0 < s.batch; b0 += 64) {
+    const int b = b0 + lane;
+    const int len = b0 == 0 ? n.first : (b < s.batch ? context_length(s, b) : 0);
+    const int mine = b < s.batch ? runs_of(s, n.chunk, tiles_of(len)) : 0;
+    const int upto = before + wave_prefix(mine);
+    const uint64_t hit = __ballot(upto > f);
+    if (hit != 0) {
+      const int at = __builtin_ctzll(hit);
+      out.b = b0 + at;
+      out.length = __builtin_amdgcn_readlane(len, at);
+      out.splits = __builtin_amdgcn_readlane(mine, at);
+      out.flat0 = __builtin_amdgcn_readlane(upto, at) - out.splits;
+      out.split = f - out.flat0;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// Splits and first flat run of sequence b (wave-uniform).
+__device__ __forceinline__ void sequence_runs(const Schedule& s, const Lengths& n, int b, int lane,
+                                              Run& out) {
+  int before = 0;
+  for (int b0 = 0; b0 <= b; b0 += 64) {
+    const int i = b0 + lane;
+    const int len = b0 == 0 ? n.first : (i < s.batch ? context_length(s, i) : 0);
+    const int mine = i < s.batch ? runs_of(s, n.chunk, tiles_of(len)) : 0;
+    const int upto = before + wave_prefix(mine);
+    if (b < b0 + 64) {
+      out.splits = __builtin_amdgcn_readlane(mine, b - b0);
+      out.flat0 = __builtin_amdgcn_readlane(upto, b - b0) - out.splits;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+
+// A wave-uniform address, asserted to the compiler, so that buffer descriptors built from it stay
+// in scalar registers.
+__device__ __forceinline__ void* uniform_ptr(const void* p) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(x >> 32));
+  return reinterpret_cast<void*>((uint64_t(hi) << 32) | lo);
+}
+
+// A buffer of `rows` rows of `row` bytes, `stride` bytes apart: what lies past the last row's end
+// reads as zero without an access.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* p, int rows,
+                                                              uint32_t stride, int row) {
+  const uint32_t range = rows > 0 ? uint32_t(rows - 1) * stride + row : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(p), (short)0,
+                                           __builtin_amdgcn_readfirstlane(range), 0x00020000);
+}
+
+}  // namespace tk_runs

@@ -124,6 +124,9 @@ _SIGNATURES: dict[str, list[object]] = {
     "tk_qk_norm_rotary_bwd": (
         [_I32] + [_P] * 13 + [_I64] * 6 + [_I64P] * 7 + [_F32, _F32, _I32, _I32, _P]
     ),
+    "tk_append_quantized": [_I32] + [_P] * 8 + [_I64] * 5 + [_I64P] * 5 + [_I32, _P],
+    "tk_read_quantized": [_I32] + [_P] * 6 + [_I64] * 4 + [_I64P] * 3 + [_I32, _P],
+    "tk_quantized_decode": [_I32] + [_P] * 8 + [_I64] * 5 + [_I64P] * 5 + [_F32, _I32, _P],
     "tk_roof_copy": [_P, _P, _I64, _P],
     "tk_roof_stream": [_P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _P],
     "tk_roof_mfma": [_I32, _P, _I64, _I64, _P],
@@ -137,6 +140,7 @@ _QUERIES: dict[str, list[object]] = {
     "tk_gemm_tile": [_P, _P] + [_I64] * 7,
     "tk_attn_fwd_rows": [_I64, _I64, _I64, _I64, _I64, _I64, _I32],
     "tk_tree_decode_slots": [_I64] * 6,
+    "tk_quantized_decode_slots": [_I64] * 5,
 }
 
 EXPORTED_SYMBOLS: tuple[str, ...] = ("tk_abi_version", "tk_last_error", *_QUERIES, *_SIGNATURES)
@@ -286,6 +290,23 @@ def row_layout(tensor: torch.Tensor, name: str, device: int) -> tuple[int, bytes
     if (strides[0] | strides[1] | strides[2]) & 7 or address & 15:
         raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of 8)")
     return address, _PACKERS[3](strides[0], strides[1], strides[2])
+
+
+def row_table(tensor: torch.Tensor, name: str, device: int, dims: int, unit: int):
+    """Address and table of the first ``dims`` strides of a tensor on GPU ``device`` whose rows must
+    be unit-stride and start on 16-byte boundaries, ``unit`` elements apart (``ValueError``
+    otherwise). Strides of dimensions with one entry address nothing, so any will do."""
+    address, strides, shape = tensor.data_ptr(), tensor.stride(), tensor.shape
+    if tensor.get_device() != device:
+        raise ValueError(f"{name} must be on the other tensors' device")
+    if strides[-1] != 1:
+        raise ValueError(f"{name} requires a contiguous final dimension")
+    strides = strides[:dims]
+    if 1 in shape[:dims]:
+        strides = tuple(shape[-1] if shape[d] == 1 else strides[d] for d in range(dims))
+    if address & 15 or any(s % unit for s in strides):
+        raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of {unit})")
+    return address, int64_table(strides)
 
 
 def query(name: str, *args: int | None) -> int:
