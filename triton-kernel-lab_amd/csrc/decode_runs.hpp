@@ -111,6 +111,22 @@ __device__ __forceinline__ void sequence_runs(const Schedule& s, const Lengths& 
   }
 }
 
+// LDS ring of 16-bit tiles: rows stored whole, chunks swizzled, as the DMA writes contiguous LDS.
+template <int D>
+struct Ring {
+  static constexpr int RB = D * 2;             // bytes per row
+  static constexpr int TILE = kTileKeys * RB;  // bytes per tensor tile
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int IPT = TILE / 1024;      // DMA instructions per tensor tile
+  static constexpr int RPI = 1024 / RB;        // rows per DMA instruction
+  static constexpr int CPR = RB / 16;          // 16-byte chunks per row
+  // K: chunk c of row r at slot c ^ kswz(r): a ds_read_b128 phase (16 lanes, one chunk of 16
+  // rows) touches 16 distinct bank groups. V: 32-byte granule g of row r at g ^ vswz(r): a
+  // transposing read's phase takes one granule of 8 rows, on distinct positions.
+  static __device__ __forceinline__ int kswz(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
+  static __device__ __forceinline__ int vswz(int r) { return D == 128 ? (r & 7) : ((r >> 1) & 3); }
+};
+
 // A wave-uniform address, asserted to the compiler, so that buffer descriptors built from it stay
 // in scalar registers.
 __device__ __forceinline__ void* uniform_ptr(const void* p) {

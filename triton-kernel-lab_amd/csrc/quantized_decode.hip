@@ -88,7 +88,7 @@ __device__ __forceinline__ i32x2 lds_read_tr8(uint32_t addr) {
 // LDS ring: NS stages of a 32-key tile of K, the same keys of V, and their scales. Rows are stored
 // whole with their 16-byte chunks swizzled (the DMA writes contiguous LDS).
 template <int D>
-struct Ring {
+struct Ring8 {
   static constexpr int RB = D;                 // bytes per row
   static constexpr int TILE = kTileKeys * RB;  // bytes per tensor tile
   static constexpr int SCALES = 2 * TILE;      // offset of the scales
@@ -111,7 +111,7 @@ struct Ring {
 // The stream of a run's tiles into the ring. All fields but the lane offsets are wave-uniform.
 template <int D>
 struct Fetcher {
-  using R = Ring<D>;
+  using R = Ring8<D>;
   const uint8_t *k, *v;  // first row of the next tile
   const char* scales;
   uint32_t k_row, v_row, s_row;  // bytes per row
@@ -159,7 +159,7 @@ struct Fetcher {
 
 template <typename T, int kType, int D, int MT>
 __global__ __launch_bounds__(64, 1) void quantized_split_kernel(DecodeArgs a) {
-  using R = Ring<D>;
+  using R = Ring8<D>;
   constexpr int DC = D / 64;  // 16-byte chunks of a key per lane, two products each
   constexpr int OC = D / 16;  // 16-dim output chunks
   constexpr int NS = R::NS, RB = R::RB;

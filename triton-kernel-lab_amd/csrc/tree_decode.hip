@@ -51,6 +51,7 @@
 #include <type_traits>
 
 #include "attention_dma.hpp"
+#include "decode_runs.hpp"
 #include "tk_common.hpp"
 
 namespace {
@@ -58,15 +59,16 @@ namespace {
 using tk_attn::f32x4;
 using tk_attn::i32x2;
 using tk_attn::i32x4;
+using tk_runs::kLog2e;
+using tk_runs::kNoMax;
+using tk_runs::kTileKeys;
+using tk_runs::Ring;
+using tk_runs::uniform_ptr;
+using tk_runs::wave_prefix;
 
-constexpr int kTileKeys = 32;
 constexpr int kMaxNodes = 256;
 constexpr int kMaskWords = kMaxNodes / 32;
 constexpr int kNonTemporal = 2;
-constexpr float kLog2e = 1.4426950408889634f;
-// The running maximum before any key: finite, so that a masked score (-inf) minus it stays
-// -inf, and below every score that carries weight.
-constexpr float kNoMax = -3.0e38f;
 
 struct TreeArgs {
   const void *q, *k, *v, *k_tree, *v_tree;
@@ -96,22 +98,6 @@ struct TreeArgs {
 __device__ __forceinline__ int context_length(const TreeArgs& a, int b) {
   const int n = a.seqlens != nullptr ? a.seqlens[b] : a.max_len;
   return min(max(n, 0), a.max_len);
-}
-
-// Inclusive prefix sums over the wave's lanes: within rows of 16 lanes by shifts, then the rows'
-// and the halves' last sums broadcast to the next ones.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_part(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
-}
-__device__ __forceinline__ int wave_prefix(int v) {
-  v += dpp_part<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
-  v += dpp_part<0x112, 0xF>(v);
-  v += dpp_part<0x114, 0xF>(v);
-  v += dpp_part<0x118, 0xF>(v);
-  v += dpp_part<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-  v += dpp_part<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-  return v;
 }
 
 // Tiles of the shortest run of a sequence that is split.
@@ -192,30 +178,6 @@ __device__ __forceinline__ void sequence_runs(const TreeArgs& a, const Lengths& 
     }
     before = __builtin_amdgcn_readlane(upto, 63);
   }
-}
-
-// ---- LDS ring (rows stored whole, chunks swizzled, as the DMA writes contiguous LDS)
-
-template <int D>
-struct Ring {
-  static constexpr int RB = D * 2;             // bytes per row
-  static constexpr int TILE = kTileKeys * RB;  // bytes per tensor tile
-  static constexpr int STAGE = 2 * TILE;
-  static constexpr int IPT = TILE / 1024;      // DMA instructions per tensor tile
-  static constexpr int RPI = 1024 / RB;        // rows per DMA instruction
-  static constexpr int CPR = RB / 16;          // 16-byte chunks per row
-  // K: chunk c of row r at slot c ^ kswz(r): a ds_read_b128 phase (16 lanes, one chunk of 16
-  // rows) touches 16 distinct bank groups. V: 32-byte granule g of row r at g ^ vswz(r): a
-  // transposing read's phase takes one granule of 8 rows, on distinct positions.
-  static __device__ __forceinline__ int kswz(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
-  static __device__ __forceinline__ int vswz(int r) { return D == 128 ? (r & 7) : ((r >> 1) & 3); }
-};
-
-__device__ __forceinline__ void* uniform_ptr(const void* p) {
-  const uint64_t x = reinterpret_cast<uintptr_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(x));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(x >> 32));
-  return reinterpret_cast<void*>((uint64_t(hi) << 32) | lo);
 }
 
 // The stream of a run's tiles into the ring: context rows, then the tree's. All fields but the
