@@ -552,6 +552,27 @@ int tk_quantized_decode(int dtype, const void* q, const void* k_cache, const voi
 int tk_quantized_decode_slots(int64_t batch, int64_t kv_heads, int64_t group, int64_t max_len,
                               int64_t head_dim);
 
+/* Decode for a batch behind a shared prefix: sequence b's query token (q, o: [batch][q_heads][head_dim],
+ * strides {batch, head}) sees the prefix_len keys of k_prefix (strides {head, position}) that all
+ * sequences share, and the first clamp(seqlens[b], 0, max_len) keys (all of them with NULL) of its own
+ * k_cache (strides {batch, head, position}). The prefix is read once for the whole batch. `lse`
+ * (nullable) float32 [batch][q_heads], base 2. Strides in elements, multiples of 8, key strides below
+ * 2^24, bases 16-byte aligned; dtype F16 or BF16, head_dim 64 or 128, any q_heads / kv_heads.
+ * `workspace`: tk_prefix_decode_slots(...) * (head_dim + 2) floats, 16-byte aligned, overwritten. Two
+ * launches. The head mapping is tk_gqa_decode's. */
+int tk_prefix_decode(int dtype, const void* q, const void* k_prefix, const void* v_prefix,
+                     const void* k_cache, const void* v_cache, const int32_t* seqlens, void* o,
+                     float* lse, float* workspace, int64_t batch, int64_t q_heads,
+                     int64_t kv_heads, int64_t prefix_len, int64_t max_len, int64_t head_dim,
+                     const int64_t* q_strides, const int64_t* k_prefix_strides,
+                     const int64_t* v_prefix_strides, const int64_t* k_strides,
+                     const int64_t* v_strides, const int64_t* o_strides, float scale, void* stream);
+
+/* Partial results that tk_prefix_decode keeps for these sizes (group = q_heads / kv_heads); -1 for
+ * sizes it does not take. No launch, no GPU. */
+int tk_prefix_decode_slots(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len,
+                           int64_t max_len, int64_t head_dim);
+
 /* ---- Calibration kernels (no counterpart in the reference). They measure the
  * roofs this GPU sustains, so that the kernels above can be priced against
  * measured ceilings beside the published peaks. */

@@ -1,0 +1,719 @@
+// Grouped-query attention decode for a batch behind a shared prefix: sequence b's one query token sees
+// the prefix_len keys that the whole batch shares and the first clamp(seqlens[b], 0, max_len) keys of
+// its own cache; G = q_heads / kv_heads query heads read a KV head.
+//
+// The prefix is attended once for all: the batch * G query rows of a KV head (row r = sequence r / G,
+// head r % G) form one matrix against its keys, so a key is read once for up to 64 or 128 rows instead
+// of once per sequence. Both parts are cut into runs of 32-key tiles, whose partial results (float32
+// sums, reference maximum and sum of the weights) a second kernel joins per row in a fixed order.
+//
+// Both products run on v_mfma_f32_16x16x32 with the keys as the first operand's rows, as in the other
+// decode kernels:
+//   S^T (16 keys x 16 rows) = K . Q^T, Q^T in registers; a row's maximum and sum are over a lane's
+//     values and lanes ^ 16, ^ 32.
+//   O^T (16 dims x 16 rows) += V^T . P^T, P^T from the score registers, V^T by transposing LDS reads.
+// K and V reach LDS by non-temporal buffer->LDS DMA. Rows past a run's end lie outside the buffer range
+// and arrive as zeros.
+//
+// One launch does both parts. A workgroup of W waves is either of the prefix (the waves share a ring of
+// tiles, each has 16 MT rows of its own) or of the sequences' own caches (each wave has a run and an
+// eighth or more of the ring to itself, and the G rows of its sequence): the first kind is bound by the
+// matrix units once there are many rows, the second by HBM, and side by side they share a CU. The work
+// is dealt on the device from the lengths: T, the work of all tiles over the workgroups that run at
+// once, with a prefix tile priced against an own one, sets the length of both kinds' runs.
+//
+// Softmax statistics and sums are float32, P is rounded to the storage dtype for the second product (as
+// in every attention of this library), O once at the end.
+#include "attention_dma.hpp"
+#include "decode_runs.hpp"
+#include "tk_common.hpp"
+
+namespace {
+
+using namespace tk_runs;
+using tk_attn::f32x4;
+using tk_attn::i32x2;
+using tk_attn::i32x4;
+
+constexpr int kNonTemporal = 2;
+constexpr int kMinRun = 4;  // tiles of the shortest run of a part that is cut
+
+struct PrefixArgs {
+  const void *q, *kp, *vp, *k, *v;
+  const int32_t* seqlens;
+  void* o;
+  float* lse;
+  float* part_o;   // [slot][D]: prefix [run][KV head][row], then own [flat run][KV head][head of G]
+  float2* part_ml; // [slot]
+  int64_t qb, qh, ob, oh, kph, kpl, vph, vpl, kb, kh, kl, vb, vh, vl;
+  tk::FastDiv by_group, by_kv_heads, by_row_blocks;
+  int batch, q_heads, kv_heads, group, rows, max_len, prefix_len, prefix_tiles, row_blocks;
+  int workgroups;           // that run at once
+  int price;                // of a prefix tile for a workgroup, in 1/16 of an own tile for a wave
+  int most_runs, most_own;  // bounds on the prefix's runs and the own flat runs
+  float scale_log2;         // positive
+  int flip;                 // Q's sign bits to turn (a negative scale)
+};
+
+__device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
+  const int n = a.seqlens != nullptr ? a.seqlens[b] : a.max_len;
+  return min(max(n, 0), a.max_len);
+}
+__device__ __forceinline__ int tiles_in(int length) { return (length + kTileKeys - 1) / kTileKeys; }
+
+// How the work is cut, the same for every workgroup of the call.
+struct Deal {
+  int first;         // this lane's sequence's length (sequence = lane)
+  int own_chunk;     // tiles of an own run
+  int prefix_chunk;  // and of a prefix run
+  int prefix_runs;
+};
+
+template <int W>
+__device__ __forceinline__ Deal make_deal(const PrefixArgs& a, int lane) {
+#pragma clang fp contract(off)  // both kernels have to come to the same numbers
+  Deal d;
+  d.first = lane < a.batch ? own_length(a, lane) : 0;
+  int sum = tiles_in(d.first);
+  for (int b = lane + 64; b < a.batch; b += 64) sum += tiles_in(own_length(a, b));
+  const int own = __builtin_amdgcn_readlane(wave_prefix(sum), 63);
+  const float prefix_work =
+      float(a.prefix_tiles) * float(a.kv_heads * a.row_blocks) * float(a.price) * (1.f / 16);
+  const float own_work = float(own) * float(a.kv_heads) * (1.f / W);
+  const float share = (prefix_work + own_work) / float(a.workgroups);
+  // The bounds hold whatever the rounding above did.
+  const int spare = max(a.most_own - a.batch, 1);
+  d.own_chunk = max(max(int(share) + 1, kMinRun), (own + spare - 1) / spare);
+  d.prefix_chunk = max(max(int(share * 16 / float(a.price)) + 1, kMinRun),
+                       (a.prefix_tiles + a.most_runs - 1) / a.most_runs);
+  d.prefix_runs = (a.prefix_tiles + d.prefix_chunk - 1) / d.prefix_chunk;
+  return d;
+}
+
+// Own flat run f: sequence, split and number of splits (wave-uniform); false past the last.
+struct OwnRun {
+  int b, length, split, splits, flat0;
+};
+__device__ __forceinline__ bool find_own(const PrefixArgs& a, const Deal& d, int f, int lane, OwnRun& out) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    const int len = b0 == 0 ? d.first : (b < a.batch ? own_length(a, b) : 0);
+    const int mine = (tiles_in(len) + d.own_chunk - 1) / d.own_chunk;
+    const int upto = before + wave_prefix(mine);
+    const uint64_t hit = __ballot(upto > f);
+    if (hit != 0) {
+      const int at = __builtin_ctzll(hit);
+      out.b = b0 + at;
+      out.length = __builtin_amdgcn_readlane(len, at);
+      out.splits = __builtin_amdgcn_readlane(mine, at);
+      out.flat0 = __builtin_amdgcn_readlane(upto, at) - out.splits;
+      out.split = f - out.flat0;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// A tensor's rows as a stream of 32-row tiles into LDS; PER DMA instructions of this wave per tile,
+// from instruction `wave` * PER on. All fields but the lane offsets are wave-uniform.
+template <int D, int PER>
+struct Stream {
+  using R = Ring<D>;
+  const char* p;  // first row of the next tile
+  uint32_t row;   // bytes per row
+  int left;       // rows from there to the end of the run
+  uint32_t off[PER];
+
+  // Instruction i covers rows RPI (wave PER + i) .. +RPI-1; the lane fetches the chunk that belongs at
+  // its LDS slot.
+  template <bool kValues>
+  __device__ __forceinline__ void start(const void* base, int64_t stride, int rows, int wave, int lane) {
+    p = static_cast<const char*>(base);
+    row = uint32_t(stride * 2);
+    left = rows;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = (wave * PER + i) * R::RPI + lane / R::CPR;
+      const int slot = lane % R::CPR;
+      const int chunk = kValues ? ((((slot >> 1) ^ R::vswz(r)) << 1) | (slot & 1)) : slot ^ R::kswz(r);
+      off[i] = r * row + chunk * 16;
+    }
+  }
+  // The next tile to `to`, this wave's share of the tile in LDS. Past the end (issued to keep the wait
+  // counts static) nothing is read and LDS gets zeros.
+  __device__ __forceinline__ void next(char* to) {
+    const __amdgpu_buffer_rsrc_t r = rows_buffer(p, min(max(left, 0), kTileKeys), row, D * 2);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (tk_attn::lds_void*)(to + i * 1024), 16, off[i], 0, 0,
+                                               kNonTemporal);
+    p += int64_t(kTileKeys) * row;
+    left -= kTileKeys;
+  }
+};
+
+// 16 MT query rows against tiles of keys.
+template <typename T, int D, int MT>
+struct Rows {
+  using R = Ring<D>;
+  static constexpr int DC = D / 32, OC = D / 16, RB = R::RB;
+  static constexpr int HB = 4;  // output chunks per batch of V reads
+  i32x4 qf[MT][DC];
+  f32x4 o[MT][OC];
+  float top[MT], sum[MT];  // reference maximum of row row16, this lane's share of its sum
+  uint32_t ka[DC], va[OC];
+
+  __device__ __forceinline__ void start(int row16, int quad) {
+#pragma unroll
+    for (int c = 0; c < DC; ++c) ka[c] = row16 * RB + (((4 * c + quad) ^ R::kswz(row16)) * 16);
+    const int trow = 4 * quad + (row16 >> 2);
+#pragma unroll
+    for (int c = 0; c < OC; ++c) va[c] = R::TILE + trow * RB + ((c ^ R::vswz(trow)) * 32) + 8 * (row16 & 3);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      top[m] = kNoMax;
+      sum[m] = 0.f;
+#pragma unroll
+      for (int c = 0; c < OC; ++c) o[m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // s[m][i][r]: product of row row16 of row tile m and key 16 i + 4 quad + r of the tile at LDS address
+  // `at`. The reads of four 32-feature steps are in flight at a time; `read` runs behind the last one.
+  template <typename F>
+  __device__ __forceinline__ void scores(uint32_t at, f32x4 (&s)[MT][2], F&& read) {
+    i32x4 kc[DC][2];
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      kc[c][0] = tk_attn::lds_read_b128<0>(at + ka[c]);
+      kc[c][1] = tk_attn::lds_read_b128<16 * RB>(at + ka[c]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      const int younger = DC - 1 - c;
+      if (younger >= 3)
+        tk_attn::wait_lgkm<6>();
+      else if (younger == 2)
+        tk_attn::wait_lgkm<4>();
+      else if (younger == 1)
+        tk_attn::wait_lgkm<2>();
+      else
+        tk_attn::wait_lgkm<0>();
+      tk_attn::pin(kc[c][0]);
+      tk_attn::pin(kc[c][1]);
+      if (c == DC - 1) read();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          s[m][i] = tk_attn::Mma16<T>::run(kc[c][i], qf[m][c], c == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[m][i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // The keys from `live` on are no keys.
+  __device__ __forceinline__ void cut(int live, int quad, f32x4 (&s)[MT][2]) {
+    if (__builtin_expect(live < kTileKeys, 0)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * i + 4 * quad + r >= live) s[m][i][r] = -INFINITY;
+    }
+  }
+
+  // P = exp2(scale s - top) into pf. The reference maximum moves only when the tile's exceeds it by
+  // more than 8 (base 2), so p <= 2^8 and o and sum are rescaled in few tiles: a lane whose
+  // exponentials sum to at most 2^8 has none above it, and then no maximum is formed.
+  __device__ __forceinline__ void softmax(const f32x4 (&s)[MT][2], float scale, i32x4 (&pf)[MT]) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      f32x4 p[2];
+      float part = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[m][i][r], scale, -top[m]));
+          part += p[i][r];
+        }
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(part <= 256.f)) != 0, 0)) {
+        float high = s[m][0][0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) high = fmaxf(high, s[m][i][r]);
+        high = tk_attn::max_over_column(high) * scale;
+        const float next = high > top[m] + 8.f ? high : top[m];
+        const float alpha = __builtin_amdgcn_exp2f(top[m] - next);
+        top[m] = next;
+        sum[m] *= alpha;
+#pragma unroll
+        for (int c = 0; c < OC; ++c) o[m][c] *= alpha;
+        part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[m][i][r], scale, -next));
+            part += p[i][r];
+          }
+      }
+      sum[m] += part;
+      pf[m] = tk_attn::acc_frag2<T>(p[0], p[1]);
+    }
+  }
+
+  // o += V^T P^T of the tile at `at`, whose first batch of V fragments has been requested; `read` runs
+  // behind the last read.
+  i32x2 lo[OC], hi[OC];
+  __device__ __forceinline__ void request_v(uint32_t at, int c0) {
+#pragma unroll
+    for (int c = c0; c < c0 + HB && c < OC; ++c) {
+      lo[c] = tk_attn::lds_read_tr16<0>(at + va[c]);
+      hi[c] = tk_attn::lds_read_tr16<16 * RB>(at + va[c]);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void accumulate(uint32_t at, const i32x4 (&pf)[MT], F&& read) {
+#pragma unroll
+    for (int c0 = 0; c0 < OC; c0 += HB) {
+      tk_attn::wait_lgkm<0>();
+      i32x4 vf[HB];
+#pragma unroll
+      for (int c = 0; c < HB; ++c) {
+        asm volatile("" : "+v"(lo[c0 + c]), "+v"(hi[c0 + c]));
+        vf[c] = i32x4{lo[c0 + c][0], lo[c0 + c][1], hi[c0 + c][0], hi[c0 + c][1]};
+      }
+      if (c0 + HB < OC)
+        request_v(at, c0 + HB);
+      else
+        read();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < HB; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m][c0 + c] = tk_attn::Mma16<T>::run(vf[c], pf[m], o[m][c0 + c]);
+    }
+  }
+
+  // Row row16 of row tile m into slot `slot`.
+  __device__ __forceinline__ void write(const PrefixArgs& a, int m, int64_t slot, bool mine, int quad) const {
+    const float l = tk_attn::sum_over_column(sum[m]);
+    if (!mine) return;
+#pragma unroll
+    for (int c = 0; c < OC; ++c)
+      *reinterpret_cast<f32x4*>(a.part_o + slot * D + 16 * c + 4 * quad) = o[m][c];
+    if (quad == 0) a.part_ml[slot] = float2{top[m], l};
+  }
+};
+
+// NS ring stages of a workgroup; an own run's wave has up to NS / W of them.
+template <typename T, int D, int W, int MT, int NS>
+__global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(PrefixArgs a) {
+  using R = Ring<D>;
+  constexpr int DC = D / 32;
+  __shared__ __attribute__((aligned(1024))) char ring[NS * R::STAGE];
+  const uint32_t ring_base = (uint32_t)(uintptr_t)(tk_attn::lds_void*)ring;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row16 = lane & 15;
+  const int quad = lane >> 4;
+  const Deal deal = make_deal<W>(a, lane);
+  const float scale = a.scale_log2;
+  auto nothing = []() {};
+  // The prefix's workgroups come first: the row blocks of a (run, KV head) are dealt to one XCD
+  // (workgroup index modulo 8), one after the other, so that they share its L2.
+  const int pairs = deal.prefix_runs * a.kv_heads;
+  const int prefix_groups = (pairs + 7) / 8 * 8 * a.row_blocks;
+
+  if (int(blockIdx.x) < prefix_groups) {
+    constexpr int PER = R::IPT / W;     // this wave's instructions per tensor tile
+    constexpr int STEP = 2 * PER, LA = NS - 1;
+    static_assert(LA * STEP < 64, "ring deeper than the vmcnt counter");
+    const int eighth = a.by_row_blocks.div(blockIdx.x / 8);
+    const int pair = eighth * 8 + blockIdx.x % 8;
+    const int rb = blockIdx.x / 8 - eighth * a.row_blocks;
+    if (pair >= pairs) return;
+    const int run = a.by_kv_heads.div(pair);
+    const int kvh = pair - run * a.kv_heads;
+    const int t0 = run * deal.prefix_chunk;
+    const int t1 = min(t0 + deal.prefix_chunk, a.prefix_tiles);
+    const int limit = min(a.prefix_len, t1 * kTileKeys);
+    const int w0 = rb * 16 * W * MT + wave * 16 * MT;  // this wave's first row
+    const bool busy = w0 < a.rows;                      // waves past the last row only fetch
+
+    Rows<T, D, MT> x;
+    // Q^T fragments: row w0 + 16 m + row16 (zero past the last), dims 32 c + 8 quad .. +7. A negative
+    // scale is taken into Q's signs (exact), so that the largest score is the largest product.
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = w0 + 16 * m + row16;
+      const int64_t b = a.by_group.div(r);
+      const int64_t h = kvh * a.group + (r - b * a.group);
+      const T* p = static_cast<const T*>(a.q) + b * a.qb + h * a.qh + 8 * quad;
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+        x.qf[m][c] = r < a.rows ? *reinterpret_cast<const i32x4*>(p + 32 * c) : i32x4{0, 0, 0, 0};
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    Stream<D, PER> ks, vs;
+    const int first = t0 * kTileKeys;
+    ks.template start<false>(static_cast<const T*>(a.kp) + kvh * a.kph + first * a.kpl, a.kpl, limit - first,
+                             wave, lane);
+    vs.template start<true>(static_cast<const T*>(a.vp) + kvh * a.vph + first * a.vpl, a.vpl, limit - first,
+                            wave, lane);
+    char* mine = ring + wave * PER * 1024;
+    auto fetch = [&](int stage) {
+      ks.next(mine + stage * R::STAGE);
+      vs.next(mine + stage * R::STAGE + R::TILE);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < LA; ++i) fetch(i);
+    x.start(row16, quad);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        x.qf[m][c] ^= a.flip;
+        tk_attn::pin(x.qf[m][c]);
+      }
+    int stage = 0;
+    for (int t = t0; t < t1; ++t) {
+      // A tile has landed (this wave's share) once only the LA - 1 younger tiles' loads are
+      // outstanding; behind the barrier every wave's share has, and every wave has read the tile
+      // before it, whose stage the tile fetched now takes.
+      tk_attn::wait_vmcnt<(LA - 1) * STEP>();
+      if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      fetch(stage == 0 ? NS - 1 : stage - 1);
+      const uint32_t at = ring_base + stage * R::STAGE;
+      stage = stage == NS - 1 ? 0 : stage + 1;
+      if (!busy) continue;
+      f32x4 s[MT][2];
+      i32x4 pf[MT];
+      x.scores(at, s, nothing);
+      x.request_v(at, 0);
+      x.cut(limit - t * kTileKeys, quad, s);
+      x.softmax(s, scale, pf);
+      x.accumulate(at, pf, nothing);
+    }
+    // The tiles issued past the end still write (zeros) into the ring.
+    tk_attn::wait_vmcnt<0>();
+    if (!busy) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = w0 + 16 * m + row16;
+      x.write(a, m, (int64_t(run) * a.kv_heads + kvh) * a.rows + r, r < a.rows, quad);
+    }
+    return;
+  }
+
+  // A run of a sequence's own cache for each wave. K and V of a stage are refilled apart, each as soon
+  // as it has been read, so that even a single stage keeps loads in flight.
+  // Stages of the slice: at most 63 loads may be outstanding, Q's among them.
+  constexpr int PER = R::IPT, SS = NS / W * 2 * PER + DC < 64 ? NS / W : NS / W - 1;
+  static_assert(SS >= 1 && SS * 2 * PER + DC < 64, "slice deeper than the vmcnt counter");
+  const int unit = (blockIdx.x - prefix_groups) * W + wave;
+  const int f = a.by_kv_heads.div(unit);
+  const int kvh = unit - f * a.kv_heads;
+  OwnRun run;
+  if (!find_own(a, deal, f, lane, run)) return;
+  const int64_t b = run.b;
+  const int t0 = run.split * deal.own_chunk;
+  const int t1 = min(t0 + deal.own_chunk, tiles_in(run.length));
+  const int limit = min(run.length, t1 * kTileKeys);
+  // Every run's rows are the G heads of its sequence, 16 at a time.
+  for (int r0 = 0; r0 < a.group; r0 += 16) {
+    Rows<T, D, 1> x;
+    const int r = r0 + row16;
+    const T* p = static_cast<const T*>(a.q) + b * a.qb + (kvh * a.group + r) * a.qh + 8 * quad;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+      x.qf[0][c] = r < a.group ? *reinterpret_cast<const i32x4*>(p + 32 * c) : i32x4{0, 0, 0, 0};
+    __builtin_amdgcn_sched_barrier(0);
+    Stream<D, PER> ks, vs;
+    const int first = t0 * kTileKeys;
+    ks.template start<false>(static_cast<const T*>(a.k) + b * a.kb + kvh * a.kh + first * a.kl, a.kl,
+                             limit - first, 0, lane);
+    vs.template start<true>(static_cast<const T*>(a.v) + b * a.vb + kvh * a.vh + first * a.vl, a.vl,
+                            limit - first, 0, lane);
+    char* slice = ring + wave * (NS / W) * R::STAGE;
+#pragma unroll
+    for (int i = 0; i < SS; ++i) {
+      ks.next(slice + i * R::STAGE);
+      vs.next(slice + i * R::STAGE + R::TILE);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    x.start(row16, quad);
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      x.qf[0][c] ^= a.flip;
+      tk_attn::pin(x.qf[0][c]);
+    }
+    int stage = 0;
+    for (int t = t0; t < t1; ++t) {
+      char* here = slice + stage * R::STAGE;
+      const uint32_t at = ring_base + uint32_t(here - ring);
+      stage = stage == SS - 1 ? 0 : stage + 1;
+      f32x4 s[1][2];
+      i32x4 pf[1];
+      // The tile's keys are followed by its values and SS - 1 tiles.
+      tk_attn::wait_vmcnt<(SS - 1) * 2 * PER + PER>();
+      x.scores(at, s, [&]() { ks.next(here); });
+      // And its values by SS - 1 tiles and the keys just sent for.
+      tk_attn::wait_vmcnt<(SS - 1) * 2 * PER + PER>();
+      x.request_v(at, 0);
+      x.cut(limit - t * kTileKeys, quad, s);
+      x.softmax(s, scale, pf);
+      x.accumulate(at, pf, [&]() { vs.next(here + R::TILE); });
+    }
+    // The tiles issued past the end still write (zeros) into the slice.
+    tk_attn::wait_vmcnt<0>();
+    const int64_t slot = int64_t(a.most_runs) * a.kv_heads * a.rows + (int64_t(f) * a.kv_heads + kvh) * a.group + r;
+    x.write(a, 0, slot, r < a.group, quad);
+  }
+}
+
+// One wave per row (sequence, head): L = D / 4 lanes hold a row of O as float4, 64 / L partial results
+// at a time, the prefix's first, folded in a fixed order.
+constexpr int kCombineWaves = 4;
+template <typename T, int D, int W>
+__global__ __launch_bounds__(64 * kCombineWaves) void prefix_combine_kernel(PrefixArgs a) {
+  constexpr int L = D / 4, S = 64 / L;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.x * kCombineWaves + wave;
+  const int b = blockIdx.y;
+  const Deal deal = make_deal<W>(a, lane);
+  // Runs and first flat run of sequence b.
+  int before = 0, splits = 0, flat0 = 0;
+  for (int b0 = 0; b0 <= b; b0 += 64) {
+    const int i = b0 + lane;
+    const int len = b0 == 0 ? deal.first : (i < a.batch ? own_length(a, i) : 0);
+    const int mine = (tiles_in(len) + deal.own_chunk - 1) / deal.own_chunk;
+    const int upto = before + wave_prefix(mine);
+    if (b < b0 + 64) {
+      splits = __builtin_amdgcn_readlane(mine, b - b0);
+      flat0 = __builtin_amdgcn_readlane(upto, b - b0) - splits;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (h >= a.q_heads) return;
+  const int kvh = a.by_group.div(h);
+  const int g = h - kvh * a.group;
+  const int parts = deal.prefix_runs + splits;
+  const int64_t prefix_step = int64_t(a.kv_heads) * a.rows, own_step = int64_t(a.kv_heads) * a.group;
+  const int64_t prefix0 = int64_t(kvh) * a.rows + int64_t(b) * a.group + g;
+  const int64_t own0 = int64_t(a.most_runs) * prefix_step + (int64_t(flat0) * a.kv_heads + kvh) * a.group + g;
+  auto slot = [&](int i) {
+    return i < deal.prefix_runs ? prefix0 + i * prefix_step : own0 + (i - deal.prefix_runs) * own_step;
+  };
+  float high = kNoMax;
+  for (int i = lane; i < parts; i += 64) high = fmaxf(high, a.part_ml[slot(i)].x);
+  high = tk::wave_allreduce(high, tk::MaxOp{});
+  float total = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int part = lane / L, d = (lane % L) * 4;
+#pragma unroll 4
+  for (int i = part; i < parts; i += S) {
+    const int64_t at = slot(i);
+    const float2 ml = a.part_ml[at];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
+    const float w = __builtin_amdgcn_exp2f(ml.x - high);
+    total += ml.y * w;
+    acc += v * w;
+  }
+#pragma unroll
+  for (int x = L; x < 64; x <<= 1) {
+    total += __shfl_xor(total, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], x);
+  }
+  if (part != 0) return;
+  float out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = acc[i] / total;
+  tk::store_vec<T, 4>(static_cast<T*>(a.o) + b * a.ob + h * a.oh + d, out);
+  if (lane == 0 && a.lse != nullptr) a.lse[int64_t(b) * a.q_heads + h] = high + log2f(total);
+}
+
+// Workgroup shapes by the rows a KV head has: 16 rows a wave up to four waves, then 32 rows a wave.
+// `price` of a prefix tile for a workgroup, in 1/16 of an own tile for a wave.
+struct Shape {
+  int waves, row_tiles, price;
+};
+Shape shape_for(int64_t rows) {
+  if (rows <= 16) return {1, 1, 16};
+  if (rows <= 32) return {2, 1, 10};
+  if (rows <= 64) return {4, 1, 6};
+  return {4, 2, 6};
+}
+constexpr int kWorkgroups = 512;  // two per CU, each with a 64 KiB ring
+
+// Instantiated here by name: left to the launches below, the host compiler leaves some of these
+// kernels' launch stubs undefined.
+#define TK_SPLIT(T, D, W, MT, NS) template __global__ void prefix_split_kernel<T, D, W, MT, NS>(PrefixArgs)
+#define TK_SPLITS(T)                                                                            \
+  TK_SPLIT(T, 128, 1, 1, 4); TK_SPLIT(T, 128, 2, 1, 4); TK_SPLIT(T, 128, 4, 1, 4);              \
+  TK_SPLIT(T, 128, 4, 2, 4); TK_SPLIT(T, 64, 1, 1, 8); TK_SPLIT(T, 64, 2, 1, 8);                \
+  TK_SPLIT(T, 64, 4, 1, 8); TK_SPLIT(T, 64, 4, 2, 8)
+TK_SPLITS(__bf16);
+TK_SPLITS(_Float16);
+
+template <typename T, int D, int W, int MT>
+void launch_shape(const PrefixArgs& a, uint32_t workgroups, hipStream_t s) {
+  hipLaunchKernelGGL((prefix_split_kernel<T, D, W, MT, D == 128 ? 4 : 8>), dim3(workgroups), dim3(64 * W), 0, s, a);
+  hipLaunchKernelGGL((prefix_combine_kernel<T, D, W>),
+                     dim3(static_cast<uint32_t>(tk::cdiv(a.q_heads, kCombineWaves)), a.batch),
+                     dim3(64 * kCombineWaves), 0, s, a);
+}
+
+template <typename T, int D>
+void launch(const PrefixArgs& a, uint32_t workgroups, hipStream_t s) {
+  const Shape shape = shape_for(a.rows);
+  if (shape.waves == 1)
+    launch_shape<T, D, 1, 1>(a, workgroups, s);
+  else if (shape.waves == 2)
+    launch_shape<T, D, 2, 1>(a, workgroups, s);
+  else if (shape.row_tiles == 1)
+    launch_shape<T, D, 4, 1>(a, workgroups, s);
+  else
+    launch_shape<T, D, 4, 2>(a, workgroups, s);
+}
+
+// Bounds on how the device cuts a call: prefix runs, own flat runs, workgroups.
+struct Plan {
+  int64_t row_blocks, most_runs, most_own, workgroups;
+};
+Plan make_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len, int64_t max_len) {
+  Plan p;
+  const Shape shape = shape_for(batch * group);
+  p.row_blocks = tk::cdiv(batch * group, 16 * shape.waves * shape.row_tiles);
+  const int64_t prefix_tiles = tk::cdiv(prefix_len, kTileKeys), own_tiles = tk::cdiv(max_len, kTileKeys);
+  // The prefix's runs if it were alone, and at most one for every kMinRun tiles.
+  p.most_runs = tk::cdiv(kWorkgroups, kv_heads * p.row_blocks);
+  if (p.most_runs > tk::cdiv(prefix_tiles, kMinRun)) p.most_runs = tk::cdiv(prefix_tiles, kMinRun);
+  // The own runs if they were alone, and one more per sequence, which ends in a shorter one.
+  p.most_own = tk::cdiv(kWorkgroups * shape.waves, kv_heads) + batch;
+  if (p.most_own > batch * tk::cdiv(own_tiles, kMinRun)) p.most_own = batch * tk::cdiv(own_tiles, kMinRun);
+  p.workgroups = tk::cdiv(p.most_runs * kv_heads, 8) * 8 * p.row_blocks + tk::cdiv(p.most_own * kv_heads, shape.waves);
+  return p;
+}
+
+// Why a problem of these (positive) sizes is not taken, or null. The grid holds at most 2^22
+// workgroups, and tiles and partial results are counted in 32 bits.
+const char* unsupported(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len, int64_t max_len,
+                        int64_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return "head_dim must be 64 or 128";
+  if (batch > 65535 || kv_heads > 65535 || group > 65535 || kv_heads * group > 65535 ||
+      prefix_len > (1 << 30) || max_len > (1 << 30) || batch * group > (1 << 22))
+    return "problem too large";
+  const Plan p = make_plan(batch, kv_heads, group, prefix_len, max_len);
+  if (batch * tk::cdiv(max_len, kTileKeys) > INT32_MAX / 2 || p.workgroups > (1 << 22) ||
+      p.most_runs * kv_heads * batch * group + p.most_own * kv_heads * group > INT32_MAX)
+    return "problem too large";
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" int tk_prefix_decode_slots(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len,
+                                      int64_t max_len, int64_t head_dim) {
+  if (batch <= 0 || kv_heads <= 0 || group <= 0 || prefix_len <= 0 || max_len <= 0) return -1;
+  if (unsupported(batch, kv_heads, group, prefix_len, max_len, head_dim) != nullptr) return -1;
+  const Plan p = make_plan(batch, kv_heads, group, prefix_len, max_len);
+  return static_cast<int>(p.most_runs * kv_heads * batch * group + p.most_own * kv_heads * group);
+}
+
+extern "C" int tk_prefix_decode(int dtype, const void* q, const void* k_prefix, const void* v_prefix,
+                                const void* k_cache, const void* v_cache, const int32_t* seqlens, void* o,
+                                float* lse, float* workspace, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                int64_t prefix_len, int64_t max_len, int64_t head_dim, const int64_t* q_strides,
+                                const int64_t* k_prefix_strides, const int64_t* v_prefix_strides,
+                                const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                                float scale, void* stream) {
+  if (dtype != TK_DTYPE_F16 && dtype != TK_DTYPE_BF16)
+    return tk::fail("prefix decode: dtype must be float16 or bfloat16");
+  if (q == nullptr || k_prefix == nullptr || v_prefix == nullptr || k_cache == nullptr || v_cache == nullptr ||
+      o == nullptr || workspace == nullptr || q_strides == nullptr || k_prefix_strides == nullptr ||
+      v_prefix_strides == nullptr || k_strides == nullptr || v_strides == nullptr || o_strides == nullptr)
+    return tk::fail("prefix decode: null pointer");
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || prefix_len <= 0 || max_len <= 0)
+    return tk::fail("prefix decode: empty problem");
+  if (q_heads % kv_heads != 0) return tk::fail("prefix decode: q_heads must be a multiple of kv_heads");
+  const int64_t group = q_heads / kv_heads;
+  if (const char* why = unsupported(batch, kv_heads, group, prefix_len, max_len, head_dim))
+    return tk::fail("prefix decode: %s", why);
+  const Plan plan = make_plan(batch, kv_heads, group, prefix_len, max_len);
+  for (const void* p : {q, k_prefix, v_prefix, k_cache, v_cache, static_cast<const void*>(o),
+                        static_cast<const void*>(workspace)})
+    if (!tk::aligned16(p)) return tk::fail("prefix decode: tensors must be 16-byte aligned");
+  struct {
+    const int64_t* strides;
+    int count;
+  } tables[] = {{q_strides, 2}, {o_strides, 2}, {k_prefix_strides, 2}, {v_prefix_strides, 2}, {k_strides, 3}, {v_strides, 3}};
+  for (const auto& t : tables)
+    for (int d = 0; d < t.count; ++d)
+      if (t.strides[d] < 0 || t.strides[d] % 8 != 0 || t.strides[d] >= (int64_t(1) << 40))
+        return tk::fail("prefix decode: strides must be non-negative multiples of 8 elements");
+  // The DMA addresses a tile's 32 rows through 32-bit buffer offsets.
+  for (int64_t stride : {k_prefix_strides[1], v_prefix_strides[1], k_strides[2], v_strides[2]})
+    if (stride >= (int64_t(1) << 24))
+      return tk::fail("prefix decode: key strides must be below 2^24 elements");
+  const Shape shape = shape_for(batch * group);
+  PrefixArgs a;
+  a.q = q, a.kp = k_prefix, a.vp = v_prefix, a.k = k_cache, a.v = v_cache;
+  a.seqlens = seqlens;
+  a.o = o;
+  a.lse = lse;
+  a.part_o = workspace;
+  const int64_t slots = plan.most_runs * kv_heads * batch * group + plan.most_own * kv_heads * group;
+  a.part_ml = reinterpret_cast<float2*>(workspace + slots * head_dim);
+  a.qb = q_strides[0], a.qh = q_strides[1];
+  a.ob = o_strides[0], a.oh = o_strides[1];
+  a.kph = k_prefix_strides[0], a.kpl = k_prefix_strides[1];
+  a.vph = v_prefix_strides[0], a.vpl = v_prefix_strides[1];
+  a.kb = k_strides[0], a.kh = k_strides[1], a.kl = k_strides[2];
+  a.vb = v_strides[0], a.vh = v_strides[1], a.vl = v_strides[2];
+  a.by_group = tk::FastDiv(static_cast<uint32_t>(group));
+  a.by_kv_heads = tk::FastDiv(static_cast<uint32_t>(kv_heads));
+  a.by_row_blocks = tk::FastDiv(static_cast<uint32_t>(plan.row_blocks));
+  a.batch = static_cast<int>(batch);
+  a.q_heads = static_cast<int>(q_heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.group = static_cast<int>(group);
+  a.rows = static_cast<int>(batch * group);
+  a.max_len = static_cast<int>(max_len);
+  a.prefix_len = static_cast<int>(prefix_len);
+  a.prefix_tiles = static_cast<int>(tk::cdiv(prefix_len, kTileKeys));
+  a.row_blocks = static_cast<int>(plan.row_blocks);
+  a.workgroups = kWorkgroups;
+  a.price = shape.price;
+  a.most_runs = static_cast<int>(plan.most_runs);
+  a.most_own = static_cast<int>(plan.most_own);
+  // Not 0, which would turn a masked score (-inf) into NaN: the least subnormal float (which the
+  // kernel's multiplications keep) leaves no score at or above 2^-149 * 2^128 = 2^-21, as good as 0
+  // to the hardware exponential.
+  a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 0x1p-149f);
+  a.flip = scale < 0.f ? int(0x80008000u) : 0;
+  hipStream_t s = tk::as_stream(stream);
+  const uint32_t workgroups = static_cast<uint32_t>(plan.workgroups);
+  if (dtype == TK_DTYPE_BF16) {
+    if (head_dim == 128)
+      launch<__bf16, 128>(a, workgroups, s);
+    else
+      launch<__bf16, 64>(a, workgroups, s);
+  } else {
+    if (head_dim == 128)
+      launch<_Float16, 128>(a, workgroups, s);
+    else
+      launch<_Float16, 64>(a, workgroups, s);
+  }
+  return tk::check_launch("prefix decode");
+}

@@ -127,6 +127,7 @@ _SIGNATURES: dict[str, list[object]] = {
     "tk_append_quantized": [_I32] + [_P] * 8 + [_I64] * 5 + [_I64P] * 5 + [_I32, _P],
     "tk_read_quantized": [_I32] + [_P] * 6 + [_I64] * 4 + [_I64P] * 3 + [_I32, _P],
     "tk_quantized_decode": [_I32] + [_P] * 8 + [_I64] * 5 + [_I64P] * 5 + [_F32, _I32, _P],
+    "tk_prefix_decode": [_I32] + [_P] * 9 + [_I64] * 6 + [_I64P] * 6 + [_F32, _P],
     "tk_roof_copy": [_P, _P, _I64, _P],
     "tk_roof_stream": [_P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _P],
     "tk_roof_mfma": [_I32, _P, _I64, _I64, _P],
@@ -141,6 +142,7 @@ _QUERIES: dict[str, list[object]] = {
     "tk_attn_fwd_rows": [_I64, _I64, _I64, _I64, _I64, _I64, _I32],
     "tk_tree_decode_slots": [_I64] * 6,
     "tk_quantized_decode_slots": [_I64] * 5,
+    "tk_prefix_decode_slots": [_I64] * 6,
 }
 
 EXPORTED_SYMBOLS: tuple[str, ...] = ("tk_abi_version", "tk_last_error", *_QUERIES, *_SIGNATURES)
