@@ -6,9 +6,10 @@
 // of its own. A row with an infinity or a NaN gets a scale of NaN and
 // codes of zero, so that every value read back of it is NaN.
 //
-// A lane holds 16 features (one 16-byte store of codes), the next power of two of head_dim / 16 lanes
-// a row; the same lanes take a token's key and its value, so both rows' loads are in flight together
-// and the pair of scales is one store.
+// A lane holds 16 bytes of tokens (8 features of 16 bits, 4 of 32), so that every wave reads and writes
+// whole lines of the wider tensors: with 16 features a lane, its two 16-byte accesses 32 bytes apart
+// from the next lane's, reading back ran at 2.4 TB/s. The same lanes take a token's key and its value,
+// so both rows' loads are in flight together and the pair of scales is one store.
 //
 // Bound by HBM: the tokens are read and the codes written once.
 #include "eight_bit.hpp"
@@ -17,8 +18,13 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;  // features per lane
 constexpr int kMaxHeadDim = 1024;
+
+// PER codes as one access.
+template <int kPer>
+struct alignas(kPer) Codes {
+  int c[kPer / 4];
+};
 
 struct AppendArgs {
   uint8_t* cache[2];
@@ -29,8 +35,8 @@ struct AppendArgs {
   int32_t* new_seqlens;
   int64_t cs[2][3], xs[2][3], ss[3];
   tk::FastDiv tokens, heads;
-  int batch, max_len, lanes, lanes_log2;
-  uint32_t rows;  // batch * heads * tokens
+  int max_len, units, lanes_log2;  // units: 16-byte parts of a row of tokens
+  uint32_t rows;                   // batch * heads * tokens
 };
 
 __device__ __forceinline__ uint32_t row_max(uint32_t v, int lanes_log2) {
@@ -38,8 +44,10 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, int lanes_log2) {
   return v;
 }
 
-template <typename T, int kType>
+// 2^lanes_log2 lanes a row (a power of two), lane l its parts l, l + lanes, ..: up to NU.
+template <typename T, int kType, int NU>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
+  constexpr int PER = 16 / sizeof(T);
   const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) >> a.lanes_log2;
   const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
   if (i >= a.rows) return;
@@ -52,15 +60,15 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
   const int count = a.counts != nullptr ? min(max(a.counts[b], 0), tokens) : tokens;
   if (h == 0 && t == 0 && lane == 0) a.new_seqlens[b] = start + min(count, a.max_len - start);
   if (t >= count || t >= a.max_len - start) return;
-  const bool mine = lane < a.lanes;  // head_dim / 16 may be no power of two
-  float x[2][kPer];
+  float x[2][NU][PER];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const T* p = static_cast<const T*>(a.x[w]) + b * a.xs[w][0] + h * a.xs[w][1] + t * a.xs[w][2] +
-                 lane * kPer;
+    const T* p = static_cast<const T*>(a.x[w]) + b * a.xs[w][0] + h * a.xs[w][1] + t * a.xs[w][2];
 #pragma unroll
-    for (int j = 0; j < kPer; j += 16 / int(sizeof(T)))
-      if (mine) tk::load_vec_stream<T, 16 / sizeof(T)>(p + j, x[w] + j);
+    for (int n = 0; n < NU; ++n) {
+      const int u = lane + (n << a.lanes_log2);
+      if (u < a.units) tk::load_vec_stream<T, PER>(p + u * PER, x[w][n]);
+    }
   }
   const int64_t at = int64_t(start) + t;
   float scale[2];
@@ -68,25 +76,30 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
   for (int w = 0; w < 2; ++w) {
     // Magnitudes compare as their bits, NaN above infinity above every number.
     uint32_t most = 0;
-    if (mine)
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) most = max(most, __float_as_uint(x[w][j]) & 0x7FFFFFFFu);
+    for (int n = 0; n < NU; ++n)
+      if (lane + (n << a.lanes_log2) < a.units)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) most = max(most, __float_as_uint(x[w][n][j]) & 0x7FFFFFFFu);
     most = row_max(most, a.lanes_log2);
     const bool sound = most < 0x7F800000u;
     const float top = fmaxf(__uint_as_float(most), 0x1p-100f);
     const float inverse = tk8::kMost<kType> * (1.0f / top);
     scale[w] = sound ? top / tk8::kMost<kType> : __uint_as_float(0x7FC00000u);
-    int codes[kPer / 4];
+    uint8_t* row = a.cache[w] + b * a.cs[w][0] + h * a.cs[w][1] + at * a.cs[w][2];
 #pragma unroll
-    for (int j = 0; j < kPer; j += 4) {
-      float v[4];
+    for (int n = 0; n < NU; ++n) {
+      Codes<PER> codes;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = x[w][j + k] * inverse;
-      codes[j / 4] = sound ? tk8::encode4<kType>(v) : 0;
+      for (int j = 0; j < PER; j += 4) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = x[w][n][j + k] * inverse;
+        codes.c[j / 4] = sound ? tk8::encode4<kType>(v) : 0;
+      }
+      const int u = lane + (n << a.lanes_log2);
+      if (u < a.units) *reinterpret_cast<Codes<PER>*>(row + u * PER) = codes;
     }
-    if (mine)
-      *reinterpret_cast<int4*>(a.cache[w] + b * a.cs[w][0] + h * a.cs[w][1] + at * a.cs[w][2] +
-                               lane * kPer) = make_int4(codes[0], codes[1], codes[2], codes[3]);
   }
   if (lane == 0)
     *reinterpret_cast<float2*>(a.scales + b * a.ss[0] + h * a.ss[1] + at * a.ss[2]) =
@@ -99,40 +112,37 @@ struct ReadArgs {
   const int32_t* seqlens;
   void* out[2];  // [batch][heads][max_len][head_dim]
   int64_t cs[2][3], ss[3];
-  tk::FastDiv lanes;  // head_dim / 16
+  tk::FastDiv units;  // 16-byte parts of a row of the output
   int max_len;
 };
 
 template <typename T, int kType>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
+  constexpr int PER = 16 / sizeof(T);
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
   const int64_t h = blockIdx.y, b = blockIdx.z;
-  const uint32_t row = a.lanes.div(i);
-  const int lane = int(i - row * a.lanes.d);
+  const uint32_t row = a.units.div(i);
+  const int u = int(i - row * a.units.d);
   if (row >= uint32_t(a.max_len)) return;
   const int length = a.seqlens != nullptr ? a.seqlens[b] : a.max_len;
-  const int64_t to = (((b * gridDim.y + h) * a.max_len + row) * a.lanes.d + lane) * kPer;
-  int4 codes[2] = {};
+  const int64_t to = (((b * gridDim.y + h) * a.max_len + row) * a.units.d + u) * PER;
+  Codes<PER> codes[2] = {};
   float2 scale = {};
   if (int(row) < length) {
 #pragma unroll
     for (int w = 0; w < 2; ++w)
-      codes[w] = *reinterpret_cast<const int4*>(a.cache[w] + b * a.cs[w][0] + h * a.cs[w][1] +
-                                                row * a.cs[w][2] + lane * kPer);
+      codes[w] = *reinterpret_cast<const Codes<PER>*>(a.cache[w] + b * a.cs[w][0] + h * a.cs[w][1] +
+                                                      row * a.cs[w][2] + u * PER);
     scale = *reinterpret_cast<const float2*>(a.scales + b * a.ss[0] + h * a.ss[1] + row * a.ss[2]);
   }
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const int c[4] = {codes[w].x, codes[w].y, codes[w].z, codes[w].w};
-    float x[kPer];
+    float x[PER];
 #pragma unroll
-    for (int j = 0; j < kPer; j += 4) tk8::decode4<kType>(c[j / 4], x + j);
+    for (int j = 0; j < PER; j += 4) tk8::decode4<kType>(codes[w].c[j / 4], x + j);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] *= w ? scale.y : scale.x;
-    T* out = static_cast<T*>(a.out[w]) + to;
-#pragma unroll
-    for (int j = 0; j < kPer; j += 16 / int(sizeof(T)))
-      tk::store_vec_stream<T, 16 / sizeof(T)>(out + j, x + j);
+    for (int j = 0; j < PER; ++j) x[j] *= w ? scale.y : scale.x;
+    tk::store_vec_stream<T, PER>(static_cast<T*>(a.out[w]) + to, x);
   }
 }
 
@@ -150,13 +160,23 @@ const char* bad_strides(const int64_t* s, int64_t unit, int64_t batch, int64_t h
   return last >= (static_cast<__int128>(1) << 52) ? "strides must keep rows in range" : nullptr;
 }
 
+template <typename T, int kType>
+void launch_append(const AppendArgs& a, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>(tk::cdiv(int64_t(a.rows) << a.lanes_log2, kThreads)));
+  if (a.units <= 64)
+    hipLaunchKernelGGL((append_kernel<T, kType, 1>), grid, dim3(kThreads), 0, s, a);
+  else if (sizeof(T) == 2 || a.units <= 128)
+    hipLaunchKernelGGL((append_kernel<T, kType, 2>), grid, dim3(kThreads), 0, s, a);
+  else if constexpr (sizeof(T) == 4)
+    hipLaunchKernelGGL((append_kernel<T, kType, 4>), grid, dim3(kThreads), 0, s, a);
+}
+
 template <typename T>
 void launch_append(const AppendArgs& a, int type, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>(tk::cdiv(int64_t(a.rows) << a.lanes_log2, kThreads)));
   if (type == tk8::kE4M3)
-    hipLaunchKernelGGL((append_kernel<T, tk8::kE4M3>), grid, dim3(kThreads), 0, s, a);
+    launch_append<T, tk8::kE4M3>(a, s);
   else
-    hipLaunchKernelGGL((append_kernel<T, tk8::kInt8>), grid, dim3(kThreads), 0, s, a);
+    launch_append<T, tk8::kInt8>(a, s);
 }
 
 template <typename T>
@@ -187,14 +207,14 @@ extern "C" int tk_append_quantized(int dtype, void* k_cache, void* v_cache, floa
     return tk::fail("append: unsupported cache type %d", cache_type);
   if (batch <= 0 || kv_heads <= 0 || max_len <= 0 || tokens <= 0 || head_dim <= 0)
     return tk::fail("append: empty problem");
-  if (head_dim % kPer != 0 || head_dim > kMaxHeadDim)
+  if (head_dim % 16 != 0 || head_dim > kMaxHeadDim)
     return tk::fail("append: head_dim must be a multiple of 16, at most %d", kMaxHeadDim);
   if (batch > 65535 || kv_heads > 65535 || max_len > (1 << 30) || tokens > (1 << 30))
     return tk::fail("append: problem too large");
   AppendArgs a;
-  a.lanes = static_cast<int>(head_dim / kPer);
+  a.units = static_cast<int>(head_dim * tk::elem_size(dtype) / 16);
   a.lanes_log2 = 0;
-  while ((1 << a.lanes_log2) < a.lanes) ++a.lanes_log2;
+  while ((1 << a.lanes_log2) < a.units && a.lanes_log2 < 6) ++a.lanes_log2;
   // A launch holds fewer than 2^32 threads, and rows are divided as numbers below 2^31.
   const __int128 rows = static_cast<__int128>(batch) * kv_heads * tokens;
   if ((rows << a.lanes_log2) >= (static_cast<__int128>(1) << 31))
@@ -229,7 +249,6 @@ extern "C" int tk_append_quantized(int dtype, void* k_cache, void* v_cache, floa
   a.new_seqlens = new_seqlens;
   a.tokens = tk::FastDiv(static_cast<uint32_t>(tokens));
   a.heads = tk::FastDiv(static_cast<uint32_t>(kv_heads));
-  a.batch = static_cast<int>(batch);
   a.max_len = static_cast<int>(max_len);
   a.rows = static_cast<uint32_t>(rows);
   hipStream_t s = tk::as_stream(stream);
@@ -256,11 +275,11 @@ extern "C" int tk_read_quantized(int dtype, const void* k_cache, const void* v_c
     return tk::fail("read: unsupported cache type %d", cache_type);
   if (batch <= 0 || kv_heads <= 0 || max_len <= 0 || head_dim <= 0)
     return tk::fail("read: empty problem");
-  if (head_dim % kPer != 0 || head_dim > kMaxHeadDim)
+  if (head_dim % 16 != 0 || head_dim > kMaxHeadDim)
     return tk::fail("read: head_dim must be a multiple of 16, at most %d", kMaxHeadDim);
-  const int64_t lanes = head_dim / kPer;
+  const int64_t units = head_dim * tk::elem_size(dtype) / 16;
   if (batch > 65535 || kv_heads > 65535 || max_len > (1 << 30) ||
-      max_len * lanes > INT32_MAX - kThreads)
+      max_len * units > INT32_MAX - kThreads)
     return tk::fail("read: problem too large");
   ReadArgs a;
   const int64_t* cache_strides[2] = {k_cache_strides, v_cache_strides};
@@ -282,9 +301,9 @@ extern "C" int tk_read_quantized(int dtype, const void* k_cache, const void* v_c
   a.seqlens = seqlens;
   a.out[0] = k;
   a.out[1] = v;
-  a.lanes = tk::FastDiv(static_cast<uint32_t>(lanes));
+  a.units = tk::FastDiv(static_cast<uint32_t>(units));
   a.max_len = static_cast<int>(max_len);
-  const dim3 grid(static_cast<uint32_t>(tk::cdiv(max_len * lanes, kThreads)),
+  const dim3 grid(static_cast<uint32_t>(tk::cdiv(max_len * units, kThreads)),
                   static_cast<uint32_t>(kv_heads), static_cast<uint32_t>(batch));
   hipStream_t s = tk::as_stream(stream);
   switch (dtype) {

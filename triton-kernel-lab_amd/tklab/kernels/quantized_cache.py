@@ -70,7 +70,7 @@ def append_quantized(
     batch, kv_heads, tokens, head_dim = shape
     if tokens == 0:
         raise ValueError("append_quantized does not support empty dimensions")
-    lanes = 1 << (head_dim // 16 - 1).bit_length()
+    lanes = min(1 << (head_dim * dtype.itemsize // 16 - 1).bit_length(), 64)
     if batch * kv_heads * tokens * lanes >= 2**31 or tokens > 2**30:
         raise ValueError("append_quantized: the problem is too large")
     device = k_cache.get_device()
@@ -141,7 +141,7 @@ def read_quantized(
     (k_ptr, k_strides), (v_ptr, v_strides), (s_ptr, s_strides), kind = _cache_layout(
         k_cache, v_cache, scales)
     batch, kv_heads, max_len, head_dim = shape = k_cache.shape
-    if max_len * head_dim // 16 > 2**31 - 257:
+    if max_len * head_dim * dtype.itemsize // 16 > 2**31 - 257:
         raise ValueError("read_quantized: the problem is too large")
     device = k_cache.get_device()
     if cache_seqlens is not None:
