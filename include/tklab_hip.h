@@ -497,7 +497,7 @@ int tk_qk_norm_rotary(int dtype, const void* q, void* q_out, const void* k, void
 
 /* Its gradients from q, k and the outputs' gradients: dq, dk (strides of their own) and the weights'
  * (head_dim entries of the storage dtype), summed in a fixed order. `partials`: float32
- * [1024][head_dim], overwritten. Two launches. */
+ * [768][head_dim], overwritten. Two launches. */
 int tk_qk_norm_rotary_bwd(int dtype, const void* q, const void* dq_out, void* dq, const void* k,
                           const void* dk_out, void* dk, const void* q_weight, const void* k_weight,
                           void* dq_weight, void* dk_weight, float* partials, const void* positions,

@@ -138,16 +138,15 @@ struct Run {
   }
   // Batch entry, token and head of row p, false where there is none.
   struct At {
-    int64_t b, n;
-    int h, token;  // token: within the run
+    int b, n, h, token;  // token: within the run
   };
   __device__ __forceinline__ bool at(const Args& a, const Side& s, uint32_t p, At& r) const {
     r.token = int(s.block_heads.div(p));
     r.h = h0 + int(p - uint32_t(r.token) * s.block_heads.d);
     const int t = t0 + r.token;
     if (p >= count || t >= a.total_tokens || r.h >= s.heads) return false;
-    r.b = a.tokens.div(t);
-    r.n = t - r.b * int64_t(a.tokens.d);
+    r.b = int(a.tokens.div(t));
+    r.n = t - r.b * int(a.tokens.d);
     return true;
   }
 };
@@ -198,8 +197,9 @@ int plan(int dtype, const void* const pointers[2][4], const Tables tables[2], co
          float eps, float magnitude, int interleaved, int wide_positions, Args& a, int& vec,
          int& units_per_lane);
 
-// Workgroups (float32 partial rows) of the backward for each side.
-constexpr int kGroups = 1024;
+// Workgroups (float32 partial rows) of the backward: three per CU, as many as its registers let run at
+// once for rows of 128 features (1024 had a second round: 122 us against 108).
+constexpr int kGroups = 768;
 
 // f(kernel's vector and units) for the variants that plan() picks.
 #define TK_QK_NORM_VARIANTS(T, vec, nu, F)                                \

@@ -28,8 +28,9 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rotary_bwd_kernel(Args a) {
   const int lane = threadIdx.x & (lanes - 1);
   const uint32_t step = kThreads >> a.lanes_log2;  // rows at a time
   const typename R::Layout layout(a, lane);
-  float g[NU][R::N], sum[NU][R::N];
-  R::load_weight(s.weight, layout, g);
+  typename R::Raw weight;
+  weight.load(static_cast<const T*>(s.weight), layout);
+  float sum[NU][R::N];
 #pragma unroll
   for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -49,16 +50,18 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rotary_bwd_kernel(Args a) {
     fill_angles(a, s, run.t0, cosv, sinv);
     __syncthreads();
     while (p < run.count) {
-      Run::At next;
-      typename R::Raw x_ahead, dy_ahead;
-      const bool next_live = run.at(a, s, p + step, next);
-      if (next_live) {
-        x_ahead.load(static_cast<const T*>(s.x) + offset(s.xs, next), layout);
-        dy_ahead.load(static_cast<const T*>(s.dy) + offset(s.ys, next), layout);
-      }
-      float f[NU][R::N], d[NU][R::N];
+      float f[NU][R::N], d[NU][R::N], g[NU][R::N];
       x.expand(layout, f);
       dy.expand(layout, d);
+      // The next row's loads take the registers that this one's have left.
+      __builtin_amdgcn_sched_barrier(0);
+      Run::At next;
+      const bool next_live = run.at(a, s, p + step, next);
+      if (next_live) {
+        x.load(static_cast<const T*>(s.x) + offset(s.xs, next), layout);
+        dy.load(static_cast<const T*>(s.dy) + offset(s.ys, next), layout);
+      }
+      weight.expand(layout, g);
       float square = 0.f, dot = 0.f;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
@@ -92,8 +95,6 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rotary_bwd_kernel(Args a) {
           }
         R::store(static_cast<T*>(s.out) + offset(s.os, here), layout, f);
       }
-      x = x_ahead;
-      dy = dy_ahead;
       live = next_live;
       here = next;
       p += step;
@@ -126,24 +127,27 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rotary_bwd_kernel(Args a) {
   }
 }
 
-// Sums of the partial rows: 32 features by 32 slices of the rows a workgroup.
-constexpr int kCols = 32, kSlices = 32;
+// Sums of the partial rows: 8 features by 128 slices of the rows a workgroup, so that a thread adds a
+// handful of rows (32 features by 32 slices: 9.9 us at 1023 rows, the loads one behind the other).
+constexpr int kCols = 8, kSlices = 128;
 template <typename T>
 __global__ __launch_bounds__(kCols* kSlices) void qk_norm_weight_kernel(Args a) {
-  __shared__ float part[kSlices][kCols + 1];
+  __shared__ float part[kSlices][kCols];
   const int w = blockIdx.y;
   const Side& s = a.side[w];
-  const int col = blockIdx.x * kCols + threadIdx.x % kCols, slice = threadIdx.x / kCols;
+  const int c = threadIdx.x % kCols, col = blockIdx.x * kCols + c, slice = threadIdx.x / kCols;
   const float* rows = a.partials + (w ? int64_t(a.side[0].groups) * a.head_dim : 0);
   float v = 0.f;
   if (col < a.head_dim)
+#pragma unroll 8
     for (uint32_t r = slice; r < s.groups; r += kSlices) v += rows[int64_t(r) * a.head_dim + col];
-  part[slice][threadIdx.x % kCols] = v;
-  __syncthreads();
-  if (slice == 0 && col < a.head_dim) {
-    for (int i = 1; i < kSlices; ++i) v += part[i][threadIdx.x];
-    static_cast<T*>(s.dweight)[col] = tk::from_f32<T>(v);
+  part[slice][c] = v;
+#pragma unroll
+  for (int half = kSlices / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (slice < half) part[slice][c] += part[slice + half][c];
   }
+  if (slice == 0 && col < a.head_dim) static_cast<T*>(s.dweight)[col] = tk::from_f32<T>(part[0][c]);
 }
 
 template <typename T, int VEC, int NU>
@@ -168,6 +172,33 @@ static void launch_all(int vec, int nu, const Args& a, bool interleaved, hipStre
   hipLaunchKernelGGL((qk_norm_weight_kernel<T>),
                      dim3(static_cast<uint32_t>(tk::cdiv(a.head_dim, kCols)), a.side[1].groups ? 2 : 1),
                      dim3(kCols * kSlices), 0, s, a);
+}
+
+// Workgroups of each side, kGroups in all at most: as few rounds of runs as that allows, where a run
+// costs its rows and, a quarter of a row for each, its angles per thread. (A run of 8 heads has four
+// times the angles of one of 32: B2 N8192 Hq32 Hkv8 106.6 us with workgroups by runs alone, 99.8 so.)
+static void share_groups(Args& a) {
+  int64_t cost[2], all = 0;
+  for (int w = 0; w < 2; ++w) {
+    const Side& s = a.side[w];
+    const int64_t step = kThreads >> a.lanes_log2;
+    cost[w] = 16 * tk::cdiv(int64_t(s.block_tokens) * s.block_heads.d, step) +
+              4 * int64_t(s.block_tokens) * a.half / kThreads;
+    all += cost[w] * s.runs;
+  }
+  int64_t most = all / kGroups;  // a workgroup's share, if it came out even
+  for (;;) {
+    int64_t groups = 0, next = INT64_MAX;
+    for (int w = 0; w < 2; ++w) {
+      Side& s = a.side[w];
+      const int64_t rounds = most / cost[w] > 1 ? most / cost[w] : 1;
+      s.groups = static_cast<uint32_t>(tk::cdiv(s.runs, rounds));
+      groups += s.groups;
+      if (next > (rounds + 1) * cost[w]) next = (rounds + 1) * cost[w];
+    }
+    if (groups <= kGroups) return;
+    most = next;
+  }
 }
 
 }  // namespace tk_qk_norm
@@ -202,14 +233,7 @@ extern "C" int tk_qk_norm_rotary_bwd(
   a.partials = partials;
   a.side[0].dweight = dq_weight;
   a.side[1].dweight = k != nullptr ? dk_weight : dq_weight;
-  // The workgroups are shared out by the sides' runs.
-  const int64_t all = int64_t(a.side[0].runs) + a.side[1].runs;
-  for (int w = 0; w < 2; ++w) {
-    Side& s = a.side[w];
-    int64_t groups = all <= kGroups ? s.runs : int64_t(kGroups) * s.runs / all;
-    if (groups < 1 && s.runs > 0) groups = 1;
-    s.groups = static_cast<uint32_t>(groups);
-  }
+  share_groups(a);
   hipStream_t s = tk::as_stream(stream);
   switch (dtype) {
     case TK_DTYPE_F32: launch_all<float>(vec, nu, a, interleaved != 0, s); break;

@@ -23,7 +23,7 @@ _POSITION_DTYPES = (torch.int32, torch.int64)
 _MAX_HEAD_DIM = 512
 _MAX_HEADS = 65535
 _MAX_TOKENS = 2**31 - 65537
-_PARTIAL_ROWS = 1024
+_PARTIAL_ROWS = 768
 
 
 def qk_norm_rotary(
