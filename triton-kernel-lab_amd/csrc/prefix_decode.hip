@@ -16,14 +16,26 @@
 // and arrive as zeros.
 //
 // One launch does both parts. A workgroup of W waves is either of the prefix (the waves share a ring of
-// tiles, each has 16 MT rows of its own) or of the sequences' own caches (each wave has a run and an
-// eighth or more of the ring to itself, and the G rows of its sequence): the first kind is bound by the
-// matrix units once there are many rows, the second by HBM, and side by side they share a CU. The work
-// is dealt on the device from the lengths: T, the work of all tiles over the workgroups that run at
-// once, with a prefix tile priced against an own one, sets the length of both kinds' runs.
+// tiles, each has 16 MT rows of its own) or of the sequences' own caches (each of up to two waves has a
+// run and a part of the ring to itself, and the G rows of its sequence): the first kind is bound by
+// issuing its instructions once there are many rows, the second by HBM, and side by side they share a CU.
+// The work is dealt on the device from the lengths: a share is the work of all tiles over the workgroups
+// that run at once, with a prefix tile priced against an own one; the prefix's runs are a share long and
+// come first, own ones half a share, so that none that starts late ends late.
 //
 // Softmax statistics and sums are float32, P is rounded to the storage dtype for the second product (as
-// in every attention of this library), O once at the end.
+// in every attention of this library; bfloat16 results are 2.3e-3 from float64's instead of 1.7e-3), O
+// once at the end.
+//
+// What bounds it (bf16 D128 Hq32 Hkv8, both kernels): B128, prefix 32768, own lengths up to 2048 (668 MB,
+// 71 GFLOP) 149 us: every CU has one workgroup of each kind, a prefix tile takes 0.92 us beside own runs
+// (0.78 with the CU to itself: about 200 instructions of one wave a SIMD, 32 of them matrix ones) and HBM
+// delivers 5 TB/s. The same with own lengths of 2048 216 us, 5.6 TB/s; own caches alone (1.07 GB) 177 us,
+// 6.1 TB/s; the prefix alone 91 us, 0.76 PFLOP/s. B4 behind 2048 keys: 6 + 4 us, latencies.
+// Measured and not kept: tile after tile without overlap 172 us (the prefix alone 101); four own waves of
+// one stage each instead of two of two: 163 us, and own caches alone 187; a fifth ring stage, scheduling
+// groups that alternate matrix and vector instructions (149 to 152 us both); the exponentials of both row
+// tiles behind one test of the maximum, which leaves no registers (180 us).
 #include "attention_dma.hpp"
 #include "decode_runs.hpp"
 #include "tk_common.hpp"
@@ -69,6 +81,10 @@ struct Deal {
   int prefix_runs;
 };
 
+// Waves of a workgroup of W that take own runs. With four, each with a stage of the ring, so many loads
+// are in flight that the prefix's waves wait for theirs: two stages each for two waves.
+__host__ __device__ constexpr int own_waves(int waves) { return waves < 2 ? waves : 2; }
+
 template <int W>
 __device__ __forceinline__ Deal make_deal(const PrefixArgs& a, int lane) {
 #pragma clang fp contract(off)  // both kernels have to come to the same numbers
@@ -79,13 +95,17 @@ __device__ __forceinline__ Deal make_deal(const PrefixArgs& a, int lane) {
   const int own = __builtin_amdgcn_readlane(wave_prefix(sum), 63);
   const float prefix_work =
       float(a.prefix_tiles) * float(a.kv_heads * a.row_blocks) * float(a.price) * (1.f / 16);
-  const float own_work = float(own) * float(a.kv_heads) * (1.f / W);
+  const float own_work = float(own) * float(a.kv_heads) * (1.f / own_waves(W));
   const float share = (prefix_work + own_work) / float(a.workgroups);
   // The bounds hold whatever the rounding above did.
   const int spare = max(a.most_own - a.batch, 1);
-  d.own_chunk = max(max(int(share) + 1, kMinRun), (own + spare - 1) / spare);
-  d.prefix_chunk = max(max(int(share * 16 / float(a.price)) + 1, kMinRun),
-                       (a.prefix_tiles + a.most_runs - 1) / a.most_runs);
+  const int own_share = __builtin_amdgcn_readfirstlane(int(share));
+  const int prefix_share = __builtin_amdgcn_readfirstlane(int(share * 16 / float(a.price)));
+  // Own runs are half a share, so that the last ones to start are not long ones.
+  d.own_chunk = max(max(own_share / 2 + 1, kMinRun), (own + spare - 1) / spare);
+  const int chunk = max(prefix_share + 1, kMinRun);
+  const int runs = min((a.prefix_tiles + chunk - 1) / chunk, a.most_runs);
+  d.prefix_chunk = (a.prefix_tiles + runs - 1) / runs;
   d.prefix_runs = (a.prefix_tiles + d.prefix_chunk - 1) / d.prefix_chunk;
   return d;
 }
@@ -230,42 +250,43 @@ struct Rows {
   // P = exp2(scale s - top) into pf. The reference maximum moves only when the tile's exceeds it by
   // more than 8 (base 2), so p <= 2^8 and o and sum are rescaled in few tiles: a lane whose
   // exponentials sum to at most 2^8 has none above it, and then no maximum is formed.
+  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], float scale, int m, f32x4 (&p)[2], float& part) const {
+    part = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, -top[m]));
+        part += p[i][r];
+      }
+  }
+  __device__ __forceinline__ void settle(const f32x4 (&s)[2], float scale, int m, f32x4 (&p)[2], float part,
+                                         i32x4& pf) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(part <= 256.f)) != 0, 0)) {
+      float high = s[0][0];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) high = fmaxf(high, s[i][r]);
+      high = tk_attn::max_over_column(high) * scale;
+      const float next = high > top[m] + 8.f ? high : top[m];
+      const float alpha = __builtin_amdgcn_exp2f(top[m] - next);
+      top[m] = next;
+      sum[m] *= alpha;
+#pragma unroll
+      for (int c = 0; c < OC; ++c) o[m][c] *= alpha;
+      weigh(s, scale, m, p, part);
+    }
+    sum[m] += part;
+    pf = tk_attn::acc_frag2<T>(p[0], p[1]);
+  }
   __device__ __forceinline__ void softmax(const f32x4 (&s)[MT][2], float scale, i32x4 (&pf)[MT]) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       f32x4 p[2];
-      float part = 0.f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[m][i][r], scale, -top[m]));
-          part += p[i][r];
-        }
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(part <= 256.f)) != 0, 0)) {
-        float high = s[m][0][0];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) high = fmaxf(high, s[m][i][r]);
-        high = tk_attn::max_over_column(high) * scale;
-        const float next = high > top[m] + 8.f ? high : top[m];
-        const float alpha = __builtin_amdgcn_exp2f(top[m] - next);
-        top[m] = next;
-        sum[m] *= alpha;
-#pragma unroll
-        for (int c = 0; c < OC; ++c) o[m][c] *= alpha;
-        part = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[m][i][r], scale, -next));
-            part += p[i][r];
-          }
-      }
-      sum[m] += part;
-      pf[m] = tk_attn::acc_frag2<T>(p[0], p[1]);
+      float part;
+      weigh(s[m], scale, m, p, part);
+      settle(s[m], scale, m, p, part, pf[m]);
     }
   }
 
@@ -302,6 +323,115 @@ struct Rows {
     }
   }
 
+  // The tiles t0 .. t1-1 of a run with the matrix units kept busy: while a tile's exponentials are
+  // formed, the next one's scores are; its output products follow with the reads of the keys after that.
+  // Keys are read two tiles ahead of values, so each have a ring of their own, NS tiles at `ring` and
+  // behind them; tile t is in stage (t - t0) % NS. One barrier in every step ends all waves' reads of
+  // keys t + 1 and values t, whose stages then take keys t + 1 + NS and values t + NS, and shows keys t + 2
+  // and values t + 1 to all of them, which were sent for NS - 1 steps before. Keys and values 0 .. NS-1
+  // have been sent for, PER instructions each, in turns.
+  template <int NS, int PER, typename FK, typename FV>
+  __device__ __forceinline__ void pipeline(uint32_t ring, int t0, int t1, int limit, int quad, float scale,
+                                           bool busy, FK&& fetch_k, FV&& fetch_v) {
+    static_assert(NS >= 4, "a stage is refilled while it is read");
+    auto arrive = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    auto after = [](int stage) { return stage == NS - 1 ? 0 : stage + 1; };
+    i32x4 kc[DC][2];
+    auto request_k = [&](int stage) {
+      const uint32_t at = ring + stage * R::TILE;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        kc[c][0] = tk_attn::lds_read_b128<0>(at + ka[c]);
+        kc[c][1] = tk_attn::lds_read_b128<16 * RB>(at + ka[c]);
+      }
+    };
+    auto pin_k = [&]() {
+      tk_attn::wait_lgkm<0>();
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        tk_attn::pin(kc[c][0]);
+        tk_attn::pin(kc[c][1]);
+      }
+    };
+    auto multiply = [&](int c0, int c1, f32x4(&s)[MT][2]) {
+#pragma unroll
+      for (int c = c0; c < c1; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            s[m][i] = tk_attn::Mma16<T>::run(kc[c][i], qf[m][c], c == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[m][i]);
+    };
+    f32x4 even[MT][2], odd[MT][2];
+    tk_attn::wait_vmcnt<(2 * NS - 1) * PER>();
+    arrive();
+    if (busy) {
+      request_k(0);
+      pin_k();
+      multiply(0, DC, even);
+    }
+    tk_attn::wait_vmcnt<(2 * NS - 3) * PER>();
+    arrive();
+    fetch_k(0);
+    int t = t0, stage = 0;
+    auto turn = [&]() {  // a step's barrier, and what it lets be sent for
+      tk_attn::wait_vmcnt<(2 * NS - 4) * PER>();
+      arrive();
+      fetch_k(after(stage));
+      fetch_v(stage);
+    };
+    if (!busy) {
+      for (; t < t1; ++t) {
+        turn();
+        stage = after(stage);
+      }
+      return;
+    }
+    request_k(1);
+    auto step = [&](f32x4(&s)[MT][2], f32x4(&next)[MT][2]) {
+      const uint32_t at = ring + (NS - 1 + stage) * R::TILE;  // va counts from a stage of both
+      cut(limit - t * kTileKeys, quad, s);
+      pin_k();
+      f32x4 p[MT][2];
+      float part[MT];
+      i32x4 pf[MT];
+      // Half of the next scores beside each row tile's exponentials, and half of the value reads.
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (m > 0) tk_attn::wait_lgkm<4>();  // lgkmcnt counts at most 15 outstanding reads
+#pragma unroll
+        for (int c = m * OC / MT; c < (m + 1) * OC / MT; ++c) {
+          lo[c] = tk_attn::lds_read_tr16<0>(at + va[c]);
+          hi[c] = tk_attn::lds_read_tr16<16 * RB>(at + va[c]);
+        }
+        multiply(m * DC / MT, (m + 1) * DC / MT, next);
+        weigh(s[m], scale, m, p[m], part[m]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) settle(s[m], scale, m, p[m], part[m], pf[m]);
+      turn();
+#pragma unroll
+      for (int c = 0; c < OC; ++c) asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
+      stage = after(stage);
+      request_k(after(stage));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < OC; ++c) {
+        const i32x4 vf = {lo[c][0], lo[c][1], hi[c][0], hi[c][1]};
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m][c] = tk_attn::Mma16<T>::run(vf, pf[m], o[m][c]);
+      }
+      return ++t == t1;
+    };
+    for (;;) {
+      if (step(even, odd)) break;
+      if (step(odd, even)) break;
+    }
+    pin_k();  // the keys past the end
+  }
+
   // Row row16 of row tile m into slot `slot`.
   __device__ __forceinline__ void write(const PrefixArgs& a, int m, int64_t slot, bool mine, int quad) const {
     const float l = tk_attn::sum_over_column(sum[m]);
@@ -313,7 +443,7 @@ struct Rows {
   }
 };
 
-// NS ring stages of a workgroup; an own run's wave has up to NS / W of them.
+// NS ring stages of a workgroup; an own run's wave has up to NS / own_waves(W) of them.
 template <typename T, int D, int W, int MT, int NS>
 __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(PrefixArgs a) {
   using R = Ring<D>;
@@ -335,7 +465,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(Pr
   if (int(blockIdx.x) < prefix_groups) {
     constexpr int PER = R::IPT / W;     // this wave's instructions per tensor tile
     constexpr int STEP = 2 * PER, LA = NS - 1;
-    static_assert(LA * STEP < 64, "ring deeper than the vmcnt counter");
+    static_assert((MT == 1 ? LA : NS) * STEP + MT * DC < 64, "ring deeper than the vmcnt counter");
     const int eighth = a.by_row_blocks.div(blockIdx.x / 8);
     const int pair = eighth * 8 + blockIdx.x % 8;
     const int rb = blockIdx.x / 8 - eighth * a.row_blocks;
@@ -374,8 +504,24 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(Pr
       vs.next(mine + stage * R::STAGE + R::TILE);
       __builtin_amdgcn_sched_barrier(0);
     };
+    auto fetch_k = [&](int stage) {
+      ks.next(mine + stage * R::TILE);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto fetch_v = [&](int stage) {
+      vs.next(mine + (NS + stage) * R::TILE);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (MT == 1) {
 #pragma unroll
-    for (int i = 0; i < LA; ++i) fetch(i);
+      for (int i = 0; i < LA; ++i) fetch(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        fetch_k(i);
+        fetch_v(i);
+      }
+    }
     x.start(row16, quad);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -384,24 +530,28 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(Pr
         x.qf[m][c] ^= a.flip;
         tk_attn::pin(x.qf[m][c]);
       }
-    int stage = 0;
-    for (int t = t0; t < t1; ++t) {
-      // A tile has landed (this wave's share) once only the LA - 1 younger tiles' loads are
-      // outstanding; behind the barrier every wave's share has, and every wave has read the tile
-      // before it, whose stage the tile fetched now takes.
-      tk_attn::wait_vmcnt<(LA - 1) * STEP>();
-      if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      fetch(stage == 0 ? NS - 1 : stage - 1);
-      const uint32_t at = ring_base + stage * R::STAGE;
-      stage = stage == NS - 1 ? 0 : stage + 1;
-      if (!busy) continue;
-      f32x4 s[MT][2];
-      i32x4 pf[MT];
-      x.scores(at, s, nothing);
-      x.request_v(at, 0);
-      x.cut(limit - t * kTileKeys, quad, s);
-      x.softmax(s, scale, pf);
-      x.accumulate(at, pf, nothing);
+    if constexpr (MT == 1) {
+      int stage = 0;
+      for (int t = t0; t < t1; ++t) {
+        // A tile has landed (this wave's share) once only the LA - 1 younger tiles' loads are
+        // outstanding; behind the barrier every wave's share has, and every wave has read the tile
+        // before it, whose stage the tile fetched now takes.
+        tk_attn::wait_vmcnt<(LA - 1) * STEP>();
+        if constexpr (W > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        fetch(stage == 0 ? NS - 1 : stage - 1);
+        const uint32_t at = ring_base + stage * R::STAGE;
+        stage = stage == NS - 1 ? 0 : stage + 1;
+        if (!busy) continue;
+        f32x4 s[MT][2];
+        i32x4 pf[MT];
+        x.scores(at, s, nothing);
+        x.request_v(at, 0);
+        x.cut(limit - t * kTileKeys, quad, s);
+        x.softmax(s, scale, pf);
+        x.accumulate(at, pf, nothing);
+      }
+    } else {
+      x.template pipeline<NS, PER>(ring_base, t0, t1, limit, quad, scale, busy, fetch_k, fetch_v);
     }
     // The tiles issued past the end still write (zeros) into the ring.
     tk_attn::wait_vmcnt<0>();
@@ -417,16 +567,21 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(Pr
   // A run of a sequence's own cache for each wave. K and V of a stage are refilled apart, each as soon
   // as it has been read, so that even a single stage keeps loads in flight.
   // Stages of the slice: at most 63 loads may be outstanding, Q's among them.
-  constexpr int PER = R::IPT, SS = NS / W * 2 * PER + DC < 64 ? NS / W : NS / W - 1;
+  constexpr int OW = own_waves(W), PER = R::IPT;
+  constexpr int SS = NS / OW * 2 * PER + DC < 64 ? NS / OW : NS / OW - 1;
   static_assert(SS >= 1 && SS * 2 * PER + DC < 64, "slice deeper than the vmcnt counter");
-  const int unit = (blockIdx.x - prefix_groups) * W + wave;
+  if (wave >= OW) return;
+  const int unit = (blockIdx.x - prefix_groups) * OW + wave;
   const int f = a.by_kv_heads.div(unit);
   const int kvh = unit - f * a.kv_heads;
   OwnRun run;
   if (!find_own(a, deal, f, lane, run)) return;
   const int64_t b = run.b;
-  const int t0 = run.split * deal.own_chunk;
-  const int t1 = min(t0 + deal.own_chunk, tiles_in(run.length));
+  // A sequence's runs are of one length, but for the last.
+  const int tiles = tiles_in(run.length);
+  const int per = (tiles + run.splits - 1) / run.splits;
+  const int t0 = min(run.split * per, tiles);
+  const int t1 = min(t0 + per, tiles);
   const int limit = min(run.length, t1 * kTileKeys);
   // Every run's rows are the G heads of its sequence, 16 at a time.
   for (int r0 = 0; r0 < a.group; r0 += 16) {
@@ -443,7 +598,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(Pr
                              limit - first, 0, lane);
     vs.template start<true>(static_cast<const T*>(a.v) + b * a.vb + kvh * a.vh + first * a.vl, a.vl,
                             limit - first, 0, lane);
-    char* slice = ring + wave * (NS / W) * R::STAGE;
+    char* slice = ring + wave * (NS / OW) * R::STAGE;
 #pragma unroll
     for (int i = 0; i < SS; ++i) {
       ks.next(slice + i * R::STAGE);
@@ -552,7 +707,7 @@ Shape shape_for(int64_t rows) {
   if (rows <= 16) return {1, 1, 16};
   if (rows <= 32) return {2, 1, 10};
   if (rows <= 64) return {4, 1, 6};
-  return {4, 2, 6};
+  return {4, 2, 7};
 }
 constexpr int kWorkgroups = 512;  // two per CU, each with a 64 KiB ring
 
@@ -600,9 +755,9 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_le
   p.most_runs = tk::cdiv(kWorkgroups, kv_heads * p.row_blocks);
   if (p.most_runs > tk::cdiv(prefix_tiles, kMinRun)) p.most_runs = tk::cdiv(prefix_tiles, kMinRun);
   // The own runs if they were alone, and one more per sequence, which ends in a shorter one.
-  p.most_own = tk::cdiv(kWorkgroups * shape.waves, kv_heads) + batch;
+  p.most_own = tk::cdiv(2 * kWorkgroups * own_waves(shape.waves), kv_heads) + batch;
   if (p.most_own > batch * tk::cdiv(own_tiles, kMinRun)) p.most_own = batch * tk::cdiv(own_tiles, kMinRun);
-  p.workgroups = tk::cdiv(p.most_runs * kv_heads, 8) * 8 * p.row_blocks + tk::cdiv(p.most_own * kv_heads, shape.waves);
+  p.workgroups = tk::cdiv(p.most_runs * kv_heads, 8) * 8 * p.row_blocks + tk::cdiv(p.most_own * kv_heads, own_waves(shape.waves));
   return p;
 }
 
