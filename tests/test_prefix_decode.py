@@ -313,3 +313,22 @@ def test_refused_layouts() -> None:
     ]:
         with pytest.raises(ValueError, match=message):
             prefix_decode(*args)
+
+
+def test_lengths_of_another_batch_are_refused() -> None:
+    """One length for several sequences, several for one, on whatever device the check sees."""
+    from tklab.kernels.prefix_decode import _plan
+
+    def alike(*shape):
+        x = _meta(*shape)
+        return x.shape, x.stride(), x.dtype, 0
+
+    def plan(batch, lengths, strides=(1,), dtype=torch.int32, device=0):
+        return _plan(*alike(batch, 8, 64), *alike(2, 9, 64), *alike(2, 9, 64), *alike(batch, 2, 10, 64),
+                     *alike(batch, 2, 10, 64), ((lengths,), strides, dtype, device))
+
+    assert plan(4, 4)[0] == (4, 8, 64) and plan(1, 1, strides=(7,))[0] == (1, 8, 64)
+    for wrong in (dict(batch=4, lengths=1), dict(batch=1, lengths=4), dict(batch=4, lengths=4, strides=(2,)),
+                  dict(batch=4, lengths=4, dtype=torch.int64), dict(batch=4, lengths=4, device=1)):
+        with pytest.raises(ValueError, match="cache_seqlens must be"):
+            plan(**wrong)

@@ -294,21 +294,24 @@ def row_layout(tensor: torch.Tensor, name: str, device: int) -> tuple[int, bytes
     return address, _PACKERS[3](strides[0], strides[1], strides[2])
 
 
-def row_table(tensor: torch.Tensor, name: str, device: int, dims: int, unit: int):
-    """Address and table of the first ``dims`` strides of a tensor on GPU ``device`` whose rows must
-    be unit-stride and start on 16-byte boundaries, ``unit`` elements apart (``ValueError``
-    otherwise). Strides of dimensions with one entry address nothing, so any will do."""
-    address, strides, shape = tensor.data_ptr(), tensor.stride(), tensor.shape
-    if tensor.get_device() != device:
-        raise ValueError(f"{name} must be on the other tensors' device")
+def row_strides(name: str, shape: tuple[int, ...], strides: tuple[int, ...], dims: int, unit: int):
+    """Table of the first ``dims`` strides of a tensor whose rows must be unit-stride and ``unit``
+    elements (16 bytes) apart, ``ValueError`` otherwise. Strides of dimensions with one entry address
+    nothing, so any will do. For the callers' checks of sizes and layouts, which are made once for
+    tensors alike (their addresses: :func:`check_aligned`)."""
     if strides[-1] != 1:
         raise ValueError(f"{name} requires a contiguous final dimension")
-    strides = strides[:dims]
-    if 1 in shape[:dims]:
-        strides = tuple(shape[-1] if shape[d] == 1 else strides[d] for d in range(dims))
-    if address & 15 or any(s % unit for s in strides):
+    strides = tuple(shape[-1] if shape[d] == 1 else strides[d] for d in range(dims))
+    if any(s % unit for s in strides):
         raise ValueError(f"{name} rows must be 16-byte aligned (strides multiples of {unit})")
-    return address, int64_table(strides)
+    return int64_table(strides)
+
+
+def check_aligned(**addresses: int) -> None:
+    """``ValueError`` naming the first address that is not on a 16-byte boundary."""
+    for name, address in addresses.items():
+        if address & 15:
+            raise ValueError(f"{name} rows must be 16-byte aligned")
 
 
 def query(name: str, *args: int | None) -> int:

@@ -53,25 +53,25 @@ def prefix_decode(
     Raises:
         ValueError: on an unsupported shape, dtype, layout or device.
     """
-    _validate(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, scale)
-    batch, q_heads, head_dim = q_shape = q.shape
-    _, kv_heads, max_len, _ = k_cache.shape
-    prefix_len = k_prefix.shape[1]
-    device = q.get_device()
-    q_ptr, q_strides = _hip.row_table(q, "q", device, 2, 8)
-    kp_ptr, kp_strides = _hip.row_table(k_prefix, "k_prefix", device, 2, 8)
-    vp_ptr, vp_strides = _hip.row_table(v_prefix, "v_prefix", device, 2, 8)
-    k_ptr, k_strides = _hip.row_table(k_cache, "k_cache", device, 3, 8)
-    v_ptr, v_strides = _hip.row_table(v_cache, "v_cache", device, 3, 8)
-    if max(kp_strides[1], vp_strides[1], k_strides[2], v_strides[2]) >= 2**24:
-        raise ValueError("key strides must be below 2**24 elements")
-    slots = _slots(batch, kv_heads, q_heads // kv_heads, prefix_len, max_len, head_dim)
-    if slots < 0:
-        raise ValueError("prefix_decode: the problem is too large")
-    out = torch.empty(q_shape, dtype=q.dtype, device=q.device)
+    if scale is not None and not abs(scale) < 2.0**126:
+        raise ValueError("scale must be finite and below 2**126")
+    q_shape = q.shape
+    (batch, q_heads, head_dim), kv_heads, prefix_len, max_len, device, slots, tables = _plan(
+        q_shape, q.stride(), q.dtype, q.get_device(),
+        k_prefix.shape, k_prefix.stride(), k_prefix.dtype, k_prefix.get_device(),
+        v_prefix.shape, v_prefix.stride(), v_prefix.dtype, v_prefix.get_device(),
+        k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device(),
+        v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device(),
+        None if cache_seqlens is None else (cache_seqlens.shape, cache_seqlens.stride(),
+                                            cache_seqlens.dtype, cache_seqlens.get_device()))
+    q_ptr, kp_ptr, vp_ptr = q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr()
+    k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
+    if (q_ptr | kp_ptr | vp_ptr | k_ptr | v_ptr) & 15:
+        _hip.check_aligned(q=q_ptr, k_prefix=kp_ptr, v_prefix=vp_ptr, k_cache=k_ptr, v_cache=v_ptr)
+    out = q.new_empty(q_shape)
     lse = None
     if return_lse:
-        lse = torch.empty((batch, q_heads), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((batch, q_heads), dtype=torch.float32)
     # Float32 partial results, as twice as many elements of q's type.
     workspace = q.new_empty(2 * slots * (head_dim + 2))
     _hip.call_on(
@@ -93,39 +93,32 @@ def prefix_decode(
         prefix_len,
         max_len,
         head_dim,
-        q_strides,
-        kp_strides,
-        vp_strides,
-        k_strides,
-        v_strides,
-        _hip.int64_table((q_heads * head_dim, head_dim)),
+        *tables,
         head_dim ** -0.5 if scale is None else float(scale),
         _hip.stream_on(device),
     )
     return (out, lse) if return_lse else out
 
 
-@lru_cache(maxsize=256)
-def _slots(batch: int, kv_heads: int, group: int, prefix_len: int, max_len: int, head_dim: int) -> int:
-    """Partial results that the library asks for (a function of the sizes alone)."""
-    return _hip.query("tk_prefix_decode_slots", batch, kv_heads, group, prefix_len, max_len, head_dim)
-
-
-def _validate(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, scale) -> None:
-    """Check the contract, up to the rows' layout."""
-    q_shape, prefix_shape, cache_shape = q.shape, k_prefix.shape, k_cache.shape
+@lru_cache(maxsize=1024)
+def _plan(q_shape, q_strides, dtype, device, prefix_shape, kp_strides, kp_dtype, kp_device, vp_shape, vp_strides,
+          vp_dtype, vp_device, cache_shape, k_strides, k_dtype, k_device, v_shape, v_strides, v_dtype, v_device,
+          seqlens):
+    """Check the contract but for addresses and values: sizes, partial results that the library asks
+    for, and stride tables, made once for tensors alike."""
     if len(q_shape) != 3 or len(prefix_shape) != 3 or len(cache_shape) != 4:
         raise ValueError("prefix_decode expects q [batch, q_heads, head_dim], a prefix [kv_heads, "
                          "prefix_len, head_dim] and caches [batch, kv_heads, max_len, head_dim]")
-    if v_prefix.shape != prefix_shape or v_cache.shape != cache_shape:
+    if vp_shape != prefix_shape or v_shape != cache_shape:
         raise ValueError("keys and values must have identical shapes")
     batch, q_heads, head_dim = q_shape
     kv_heads, prefix_len, prefix_dim = prefix_shape
+    max_len = cache_shape[2]
     if cache_shape[0] != batch or cache_shape[3] != head_dim:
         raise ValueError("q and the caches disagree on batch or head_dim")
     if cache_shape[1] != kv_heads or prefix_dim != head_dim:
         raise ValueError("the prefix and the caches disagree on kv_heads or head_dim")
-    if not (batch and q_heads and kv_heads and prefix_len and cache_shape[2] and head_dim):
+    if not (batch and q_heads and kv_heads and prefix_len and max_len and head_dim):
         raise ValueError("prefix_decode does not support empty dimensions")
     if batch > 65535 or q_heads > 65535:
         raise ValueError("prefix_decode supports at most 65535 sequences and heads")
@@ -133,15 +126,27 @@ def _validate(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, scale) -> 
         raise ValueError("q_heads must be a multiple of kv_heads")
     if head_dim not in _HEAD_DIMS:
         raise ValueError("prefix_decode supports head_dim 64 and 128")
-    dtype = q.dtype
-    if dtype not in _DTYPES or not (
-            dtype == k_prefix.dtype == v_prefix.dtype == k_cache.dtype == v_cache.dtype):
+    if dtype not in _DTYPES or not dtype == kp_dtype == vp_dtype == k_dtype == v_dtype:
         raise ValueError("q, prefix and caches must share a float16 or bfloat16 dtype")
-    if scale is not None and not abs(scale) < 2.0**126:
-        raise ValueError("scale must be finite and below 2**126")
-    if not q.is_cuda:
+    if device < 0:
         raise ValueError("prefix_decode requires CUDA (ROCm/HIP) tensors")
-    if cache_seqlens is not None and (
-            cache_seqlens.shape != (batch,) or cache_seqlens.dtype != torch.int32
-            or cache_seqlens.get_device() != q.get_device() or not cache_seqlens.is_contiguous()):
+    for name, other in (("k_prefix", kp_device), ("v_prefix", vp_device), ("k_cache", k_device),
+                        ("v_cache", v_device)):
+        if other != device:
+            raise ValueError(f"{name} must be on q's device")
+    if seqlens is not None and (seqlens[0] != (batch,) or seqlens[2] != torch.int32 or seqlens[3] != device
+                                or (batch > 1 and seqlens[1][0] != 1)):
         raise ValueError("cache_seqlens must be a contiguous int32 [batch] tensor on q's device")
+    tables = (_hip.row_strides("q", q_shape, q_strides, 2, 8),
+              _hip.row_strides("k_prefix", prefix_shape, kp_strides, 2, 8),
+              _hip.row_strides("v_prefix", prefix_shape, vp_strides, 2, 8),
+              _hip.row_strides("k_cache", cache_shape, k_strides, 3, 8),
+              _hip.row_strides("v_cache", cache_shape, v_strides, 3, 8),
+              _hip.int64_table((q_heads * head_dim, head_dim)))
+    if max(tables[1][1], tables[2][1], tables[3][2], tables[4][2]) >= 2**24:
+        raise ValueError("key strides must be below 2**24 elements")
+    slots = _hip.query("tk_prefix_decode_slots", batch, kv_heads, q_heads // kv_heads, prefix_len, max_len,
+                       head_dim)
+    if slots < 0:
+        raise ValueError("prefix_decode: the problem is too large")
+    return tuple(q_shape), kv_heads, prefix_len, max_len, device, slots, tables

@@ -9,6 +9,7 @@ outputs' gradients.
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Any
 
 import torch
@@ -64,7 +65,11 @@ def qk_norm_rotary(
         ValueError: on an unsupported shape, dtype, layout or device.
         RuntimeError: on a forward-mode tangent.
     """
-    _validate(q, k, q_weight, k_weight, positions, frequencies)
+    plan = _plan(q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
+                 q_weight.shape, q_weight.stride(), q_weight.dtype, q_weight.get_device(),
+                 k_weight.shape, k_weight.stride(), k_weight.dtype, k_weight.get_device(),
+                 positions.shape, positions.stride(), positions.dtype, positions.get_device(),
+                 frequencies.shape, frequencies.stride(), frequencies.dtype, frequencies.get_device())
     validate_epsilon(eps)
     if not 2.0**-126 <= eps < 2.0**127:
         raise ValueError("eps must be a normal float32")
@@ -72,20 +77,20 @@ def qk_norm_rotary(
     # Within a forward-mode level the inputs may carry tangents, which autograd's function refuses.
     if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
             q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
-        return _QkNormRotaryFunction.apply(q, k, q_weight, k_weight, positions, frequencies, how)
-    return _forward(q, k, q_weight, k_weight, positions, frequencies, how)
+        return _QkNormRotaryFunction.apply(q, k, q_weight, k_weight, positions, frequencies, how, plan)
+    return _forward(q, k, q_weight, k_weight, positions, frequencies, how, plan)
 
 
 class _QkNormRotaryFunction(torch.autograd.Function):
     """Autograd bridge; the inputs are kept, no statistics."""
 
     @staticmethod
-    def forward(ctx: Any, q, k, q_weight, k_weight, positions, frequencies, how):
+    def forward(ctx: Any, q, k, q_weight, k_weight, positions, frequencies, how, plan):
         """Norm and turn."""
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
-        ctx.how = how
-        return _forward(q, k, q_weight, k_weight, positions, frequencies, how)
+        ctx.how = how, plan
+        return _forward(q, k, q_weight, k_weight, positions, frequencies, how, plan)
 
     @staticmethod
     @once_differentiable
@@ -95,22 +100,19 @@ class _QkNormRotaryFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         sides = [(0, q, q_weight, dq_out), (1, k, k_weight, dk_out)]
         sides = [s for s in sides if s[3] is not None and (need[s[0]] or need[s[0] + 2])]
-        grads: list[torch.Tensor | None] = [None] * 7
+        grads: list[torch.Tensor | None] = [None] * 8
         if sides:
-            results = _backward([s[1:] for s in sides], positions, frequencies, ctx.how)
+            results = _backward(sides, positions, frequencies, *ctx.how)
             for (which, *_), (dx, dw) in zip(sides, results):
                 grads[which] = dx if need[which] else None
                 grads[which + 2] = dw if need[which + 2] else None
         return tuple(grads)
 
 
-def _forward(q, k, q_weight, k_weight, positions, frequencies, how):
+def _forward(q, k, q_weight, k_weight, positions, frequencies, how, plan):
     """Allocate the outputs and enqueue the pass over tensors already checked."""
-    q_out, q_out_strides = _like(q)
-    k_out, k_out_strides = _like(k)
-    shape = q.shape
-    packed = len(shape) == 3
-    device = q.get_device()
+    device, sizes, (q_strides, q_out_strides), (k_strides, k_out_strides), position_strides, wide = plan
+    q_out, k_out = _like(q), _like(k)
     _hip.call_on(
         device,
         "tk_qk_norm_rotary",
@@ -123,95 +125,83 @@ def _forward(q, k, q_weight, k_weight, positions, frequencies, how):
         k_weight.data_ptr(),
         positions.data_ptr(),
         frequencies.data_ptr(),
-        1 if packed else shape[0],
-        shape[0] if packed else shape[2],
-        shape[1],
-        k.shape[1],
-        shape[-1],
-        2 * frequencies.shape[0],
-        _strides(q.stride()),
-        _strides(q_out_strides),
-        _strides(k.stride()),
-        _strides(k_out_strides),
-        _position_strides(positions),
+        *sizes,
+        q_strides,
+        q_out_strides,
+        k_strides,
+        k_out_strides,
+        position_strides,
         *how,
-        int(positions.dtype == torch.int64),
+        wide,
         _hip.stream_on(device),
     )
     return q_out, k_out
 
 
-def _backward(sides, positions, frequencies, how):
-    """(dx, dweight) of each side (x, weight, dy), one or two of them."""
-    arguments, tables, weights, grads = [], [], [], []
-    x0 = sides[0][0]
-    packed = x0.ndim == 3
-    for x, weight, dy in sides:
+def _backward(sides, positions, frequencies, how, plan):
+    """(dx, dweight) of each side (which, x, weight, dy), one or two of them."""
+    device, sizes, *tables_of, position_strides, wide = plan
+    pointers, tables, weights, grads, held = [], [], [], [], []
+    for which, x, weight, dy in sides:
         if dy.stride(-1) != 1:  # a broadcast gradient has stride 0
             dy = dy.contiguous()
-        dx, dx_strides = _like(x)
-        dw = torch.empty_like(weight)
-        arguments += [x, dy, dx]
-        tables += [_strides(x.stride()), _strides(dy.stride()), _strides(dx_strides)]
-        weights.append(weight)
+        dx, dw = _like(x), torch.empty_like(weight)
+        x_strides, out_strides = tables_of[which]
+        pointers += (x.data_ptr(), dy.data_ptr(), dx.data_ptr())
+        tables += (x_strides, _strides(dy.stride()), out_strides)
+        weights.append(weight.data_ptr())
         grads.append((dx, dw))
-    pad = [None] * (2 - len(sides))
-    partials = torch.empty((_PARTIAL_ROWS, x0.shape[-1]), dtype=torch.float32, device=x0.device)
-    device = x0.get_device()
+        held.append(dy)  # until the call below: a copy's memory would be handed out again
+    pad = () if len(sides) == 2 else (None,)
+    batch, tokens, q_heads, kv_heads, *dims = sizes
+    heads = (q_heads, kv_heads)
+    partials = torch.empty((_PARTIAL_ROWS, dims[0]), dtype=torch.float32, device=positions.device)
     _hip.call_on(
         device,
         "tk_qk_norm_rotary_bwd",
-        _hip.DTYPE_CODES[x0.dtype],
-        *(t.data_ptr() for t in arguments),
+        _hip.DTYPE_CODES[sides[0][1].dtype],
+        *pointers,
         *(pad * 3),
-        *(w.data_ptr() for w in weights),
+        *weights,
         *pad,
         *(dw.data_ptr() for _, dw in grads),
         *pad,
         partials.data_ptr(),
         positions.data_ptr(),
         frequencies.data_ptr(),
-        1 if packed else x0.shape[0],
-        x0.shape[0] if packed else x0.shape[2],
-        x0.shape[1],
-        0 if pad else sides[1][0].shape[1],
-        x0.shape[-1],
-        2 * frequencies.shape[0],
+        batch,
+        tokens,
+        heads[sides[0][0]],
+        0 if pad else kv_heads,
+        *dims,
         *tables,
         *(pad * 3),
-        _position_strides(positions),
+        position_strides,
         *how,
-        int(positions.dtype == torch.int64),
+        wide,
         _hip.stream_on(device),
     )
     return grads
 
 
-def _like(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
-    """A tensor of x's shape, and order where that leaves the last dimension contiguous, and its
-    strides."""
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A tensor of x's shape, and order where that leaves the last dimension contiguous."""
     out = torch.empty_like(x)
-    strides = out.stride()
-    if strides[-1] != 1:
+    if out.stride(-1) != 1:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        strides = out.stride()
-    return out, strides
+    return out
 
 
 def _strides(strides: tuple[int, ...]):
-    """``{batch, head, token}`` strides."""
-    return _hip.int64_table((0, strides[1], strides[0]) if len(strides) == 3 else strides[:3])
+    """Table of ``{batch, head, token}`` strides."""
+    return _hip.int64_table((0, strides[1], strides[0]) if len(strides) == 3 else tuple(strides[:3]))
 
 
-def _position_strides(positions: torch.Tensor):
-    """``{batch, token}`` strides."""
-    strides = positions.stride()
-    return _hip.int64_table(strides if len(strides) == 2 else (0, strides[0]))
-
-
-def _validate(q, k, q_weight, k_weight, positions, frequencies) -> None:
-    """Check the contract."""
-    shape, k_shape, dtype = q.shape, k.shape, q.dtype
+@lru_cache(maxsize=1024)
+def _plan(shape, q_strides, dtype, device, k_shape, k_strides, k_dtype, k_device, qw_shape, qw_strides, qw_dtype,
+          qw_device, kw_shape, kw_strides, kw_dtype, kw_device, pos_shape, pos_strides, pos_dtype, pos_device,
+          freq_shape, freq_strides, freq_dtype, freq_device):
+    """Check the contract; device, sizes and stride tables, made once for tensors alike."""
     rank = len(shape)
     if rank != 3 and rank != 4:
         raise ValueError("qk_norm_rotary expects q [batch, heads, tokens, head_dim] or packed "
@@ -224,36 +214,40 @@ def _validate(q, k, q_weight, k_weight, positions, frequencies) -> None:
         raise ValueError("q and k may differ only in their head counts")
     if dtype not in _DTYPES:
         raise ValueError("qk_norm_rotary supports float16, bfloat16 and float32 tensors")
-    if not dtype == k.dtype == q_weight.dtype == k_weight.dtype:
+    if not dtype == k_dtype == qw_dtype == kw_dtype:
         raise ValueError("q, k and their weights must share a dtype")
     tokens, dim = shape[0] if rank == 3 else shape[2], shape[-1]
-    if q_weight.shape != (dim,) or k_weight.shape != (dim,):
+    batch = 1 if rank == 3 else shape[0]
+    if qw_shape != (dim,) or kw_shape != (dim,):
         raise ValueError("q_weight and k_weight must be [head_dim]")
-    if dim > 1 and (q_weight.stride(0) != 1 or k_weight.stride(0) != 1):
+    if dim > 1 and (qw_strides[0] != 1 or kw_strides[0] != 1):
         raise ValueError("q_weight and k_weight must be contiguous")
     if shape[1] > _MAX_HEADS or k_shape[1] > _MAX_HEADS:
         raise ValueError(f"qk_norm_rotary supports at most {_MAX_HEADS} heads each")
-    if tokens * (1 if rank == 3 else shape[0]) > _MAX_TOKENS:
+    if tokens * batch > _MAX_TOKENS:
         raise ValueError(f"qk_norm_rotary supports at most {_MAX_TOKENS} tokens")
-    wanted, given = (tokens,), positions.shape
-    if given != wanted and (rank == 3 or given != (shape[0], *wanted)):
+    if pos_shape != (tokens,) and (rank == 3 or pos_shape != (batch, tokens)):
         raise ValueError("positions must be [tokens]" + (" or [batch, tokens]" * (rank == 4)))
-    if positions.dtype not in _POSITION_DTYPES:
+    if pos_dtype not in _POSITION_DTYPES:
         raise ValueError("positions must be int32 or int64")
-    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+    if freq_dtype != torch.float64 or len(freq_shape) != 1:
         raise ValueError("frequencies must be a float64 [rotary_dim // 2] tensor")
-    pairs = frequencies.shape[0]
+    pairs = freq_shape[0]
     if pairs == 0 or 2 * pairs > dim:
         raise ValueError("frequencies must cover at least one pair and at most head_dim features")
-    if pairs > 1 and frequencies.stride(0) != 1:
+    if pairs > 1 and freq_strides[0] != 1:
         raise ValueError("frequencies must be contiguous")
     if dim > _MAX_HEAD_DIM:
         raise ValueError(f"qk_norm_rotary supports head_dim up to {_MAX_HEAD_DIM}")
-    if not q.is_cuda:
+    if device < 0:
         raise ValueError("qk_norm_rotary requires CUDA (ROCm/HIP) tensors")
-    device = q.get_device()
-    if not (k.get_device() == device == positions.get_device() == frequencies.get_device()
-            == q_weight.get_device() == k_weight.get_device()):
+    if not device == k_device == qw_device == kw_device == pos_device == freq_device:
         raise ValueError("q, k, their weights, positions and frequencies must be on one device")
-    if q.stride(-1) != 1 or k.stride(-1) != 1:
+    if q_strides[-1] != 1 or k_strides[-1] != 1:
         raise ValueError("q and k require a contiguous final dimension")
+    outs = [_like(torch.empty_strided(s, t, device="meta")).stride() for s, t in ((shape, q_strides),
+                                                                                  (k_shape, k_strides))]
+    sizes = (batch, tokens, shape[1], k_shape[1], dim, 2 * pairs)
+    position_strides = _hip.int64_table(tuple(pos_strides) if len(pos_strides) == 2 else (0, pos_strides[0]))
+    return (device, sizes, (_strides(q_strides), _strides(outs[0])), (_strides(k_strides), _strides(outs[1])),
+            position_strides, int(pos_dtype == torch.int64))

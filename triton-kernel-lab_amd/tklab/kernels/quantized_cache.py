@@ -14,6 +14,8 @@ Inference only: autograd does not know of these calls.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from tklab import _hip
@@ -55,37 +57,20 @@ def append_quantized(
     Raises:
         ValueError: on an unsupported shape, dtype, layout or device.
     """
-    cache_shape, shape = k_cache.shape, k.shape
-    if len(cache_shape) != 4 or len(shape) != 4:
-        raise ValueError("append_quantized expects caches [batch, kv_heads, max_len, head_dim] and "
-                         "tokens [batch, kv_heads, tokens, head_dim]")
-    if v.shape != shape:
-        raise ValueError("k and v must have identical shapes")
-    if shape[0] != cache_shape[0] or shape[1] != cache_shape[1] or shape[3] != cache_shape[3]:
-        raise ValueError("the caches and the tokens disagree on batch, kv_heads or head_dim")
-    dtype = k.dtype
-    if dtype not in _DTYPES or v.dtype != dtype:
-        raise ValueError("k and v must share a float16, bfloat16 or float32 dtype")
-    caches = _cache_layout(k_cache, v_cache, scales, written=True)
-    batch, kv_heads, tokens, head_dim = shape
-    if tokens == 0:
-        raise ValueError("append_quantized does not support empty dimensions")
-    lanes = min(1 << (head_dim * dtype.itemsize // 16 - 1).bit_length(), 64)
-    if batch * kv_heads * tokens * lanes >= 2**31 or tokens > 2**30:
-        raise ValueError("append_quantized: the problem is too large")
-    device = k_cache.get_device()
-    _check_lengths(cache_seqlens, "cache_seqlens", batch, device)
-    if counts is not None:
-        _check_lengths(counts, "counts", batch, device)
-    unit = 16 // dtype.itemsize
-    k_ptr, k_strides = _hip.row_table(k, "k", device, 3, unit)
-    v_ptr, v_strides = _hip.row_table(v, "v", device, 3, unit)
+    device, kind, sizes, tables = _append_plan(
+        *cache_meta(k_cache, v_cache, scales), lengths_meta(cache_seqlens),
+        (k.shape, k.stride(), k.dtype, k.get_device()), (v.shape, v.stride(), v.dtype, v.get_device()),
+        None if counts is None else lengths_meta(counts))
+    k_cache_ptr, v_cache_ptr, s_ptr = k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr()
+    k_ptr, v_ptr = k.data_ptr(), v.data_ptr()
+    if (k_cache_ptr | v_cache_ptr | k_ptr | v_ptr) & 15 or s_ptr & 7:
+        _hip.check_aligned(k_cache=k_cache_ptr, v_cache=v_cache_ptr, k=k_ptr, v=v_ptr)
+        raise ValueError("pairs of scales must be 8-byte aligned")
     lengths = torch.empty_like(cache_seqlens)
-    (k_cache_ptr, k_cache_strides), (v_cache_ptr, v_cache_strides), (s_ptr, s_strides), kind = caches
     _hip.call_on(
         device,
         "tk_append_quantized",
-        _hip.DTYPE_CODES[dtype],
+        _hip.DTYPE_CODES[k.dtype],
         k_cache_ptr,
         v_cache_ptr,
         s_ptr,
@@ -94,16 +79,8 @@ def append_quantized(
         v_ptr,
         None if counts is None else counts.data_ptr(),
         lengths.data_ptr(),
-        batch,
-        kv_heads,
-        cache_shape[2],
-        tokens,
-        head_dim,
-        k_cache_strides,
-        v_cache_strides,
-        s_strides,
-        k_strides,
-        v_strides,
+        *sizes,
+        *tables,
         kind,
         _hip.stream_on(device),
     )
@@ -134,19 +111,14 @@ def read_quantized(
     Raises:
         ValueError: on an unsupported shape, dtype, layout or device.
     """
-    if dtype not in _DTYPES:
-        raise ValueError("read_quantized gives float16, bfloat16 or float32")
-    if k_cache.ndim != 4:
-        raise ValueError("read_quantized expects caches [batch, kv_heads, max_len, head_dim]")
-    (k_ptr, k_strides), (v_ptr, v_strides), (s_ptr, s_strides), kind = _cache_layout(
-        k_cache, v_cache, scales)
-    batch, kv_heads, max_len, head_dim = shape = k_cache.shape
-    if max_len * head_dim * dtype.itemsize // 16 > 2**31 - 257:
-        raise ValueError("read_quantized: the problem is too large")
-    device = k_cache.get_device()
-    if cache_seqlens is not None:
-        _check_lengths(cache_seqlens, "cache_seqlens", batch, device)
-    k, v = (torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in "kv")
+    device, kind, sizes, tables = _read_plan(
+        dtype, *cache_meta(k_cache, v_cache, scales),
+        None if cache_seqlens is None else lengths_meta(cache_seqlens))
+    k_ptr, v_ptr, s_ptr = k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr()
+    if (k_ptr | v_ptr) & 15 or s_ptr & 7:
+        _hip.check_aligned(k_cache=k_ptr, v_cache=v_ptr)
+        raise ValueError("pairs of scales must be 8-byte aligned")
+    k, v = (torch.empty(sizes, dtype=dtype, device=k_cache.device) for _ in "kv")
     _hip.call_on(
         device,
         "tk_read_quantized",
@@ -157,25 +129,37 @@ def read_quantized(
         None if cache_seqlens is None else cache_seqlens.data_ptr(),
         k.data_ptr(),
         v.data_ptr(),
-        batch,
-        kv_heads,
-        max_len,
-        head_dim,
-        k_strides,
-        v_strides,
-        s_strides,
+        *sizes,
+        *tables,
         kind,
         _hip.stream_on(device),
     )
     return k, v
 
 
-def _cache_layout(k_cache, v_cache, scales, *, written: bool = False):
-    """(address, strides) of the caches and their scales, checked, and the type's code."""
-    shape, kind = k_cache.shape, CACHE_TYPES.get(k_cache.dtype)
-    if v_cache.shape != shape:
+# Checks of sizes, types and layouts, made once for tensors alike: they see a tensor as (shape, strides,
+# dtype, device index).
+
+
+def cache_meta(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor):
+    """What the checks see of a cache's three tensors."""
+    return ((k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device()),
+            (v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device()),
+            (scales.shape, scales.stride(), scales.dtype, scales.get_device()))
+
+
+def lengths_meta(lengths: torch.Tensor):
+    """What the checks see of a tensor of lengths."""
+    return lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device()
+
+
+def check_cache(k_meta, v_meta, scales_meta):
+    """Check a cache; its type's code and the stride tables of its three tensors."""
+    shape, k_strides, dtype, device = k_meta
+    kind = CACHE_TYPES.get(dtype)
+    if v_meta[0] != shape:
         raise ValueError("k_cache and v_cache must have identical shapes")
-    if kind is None or v_cache.dtype != k_cache.dtype:
+    if kind is None or v_meta[2] != dtype:
         raise ValueError("k_cache and v_cache must share a float8_e4m3fn or int8 dtype")
     if 0 in shape:
         raise ValueError("a cache may not have empty dimensions")
@@ -184,29 +168,72 @@ def _cache_layout(k_cache, v_cache, scales, *, written: bool = False):
         raise ValueError(f"head_dim must be a multiple of 16, at most {_MAX_HEAD_DIM}")
     if batch > 65535 or kv_heads > 65535 or max_len > 2**30:
         raise ValueError("a cache holds at most 65535 sequences and heads and 2**30 positions")
-    if scales.shape != (batch, kv_heads, max_len, 2) or scales.dtype != torch.float32:
+    scales_shape, s_strides, scales_dtype, scales_device = scales_meta
+    if scales_shape != (batch, kv_heads, max_len, 2) or scales_dtype != torch.float32:
         raise ValueError("scales must be a float32 [batch, kv_heads, max_len, 2] tensor")
-    if not k_cache.is_cuda:
+    if device < 0:
         raise ValueError("an 8-bit cache requires CUDA (ROCm/HIP) tensors")
-    device = k_cache.get_device()
-    k = _hip.row_table(k_cache, "k_cache", device, 3, 16)
-    v = _hip.row_table(v_cache, "v_cache", device, 3, 16)
-    s_ptr, s_strides = scales.data_ptr(), scales.stride()
-    if scales.get_device() != device or s_strides[3] != 1:
+    if v_meta[3] != device:
+        raise ValueError("k_cache and v_cache must be on one device")
+    if scales_device != device or s_strides[3] != 1:
         raise ValueError("scales must be on the caches' device with a contiguous final dimension")
-    if 1 in shape:
-        s_strides = tuple(2 if shape[d] == 1 else s_strides[d] for d in range(3))
-    if s_ptr & 7 or (s_strides[0] | s_strides[1] | s_strides[2]) & 1:
+    s_strides = tuple(2 if shape[d] == 1 else s_strides[d] for d in range(3))
+    if (s_strides[0] | s_strides[1] | s_strides[2]) & 1:
         raise ValueError("pairs of scales must be 8-byte aligned")
-    if written:
-        for name, tensor in (("k_cache", k_cache), ("v_cache", v_cache), ("scales", scales)):
-            strides = tensor.stride()
-            if 0 in strides and any(strides[d] == 0 and shape[d] > 1 for d in range(3)):
-                raise ValueError(f"{name} is written: its rows may not share memory")
-    return k, v, (s_ptr, _hip.int64_table(s_strides[:3])), kind
+    return kind, (_hip.row_strides("k_cache", shape, k_strides, 3, 16),
+                  _hip.row_strides("v_cache", shape, v_meta[1], 3, 16), _hip.int64_table(s_strides))
 
 
-def _check_lengths(lengths: torch.Tensor, name: str, batch: int, device: int) -> None:
-    if (lengths.shape != (batch,) or lengths.dtype != torch.int32
-            or lengths.get_device() != device or not lengths.is_contiguous()):
+def check_lengths(meta, name: str, batch: int, device: int) -> None:
+    """Check a tensor of lengths (of one entry, whose stride addresses nothing, or contiguous)."""
+    shape, strides, dtype, where = meta
+    if shape != (batch,) or dtype != torch.int32 or where != device or (batch > 1 and strides[0] != 1):
         raise ValueError(f"{name} must be a contiguous int32 [batch] tensor on the caches' device")
+
+
+@lru_cache(maxsize=1024)
+def _append_plan(k_cache, v_cache, scales, seqlens, k, v, counts):
+    cache_shape, shape, dtype = k_cache[0], k[0], k[2]
+    if len(cache_shape) != 4 or len(shape) != 4:
+        raise ValueError("append_quantized expects caches [batch, kv_heads, max_len, head_dim] and "
+                         "tokens [batch, kv_heads, tokens, head_dim]")
+    if v[0] != shape:
+        raise ValueError("k and v must have identical shapes")
+    if shape[0] != cache_shape[0] or shape[1] != cache_shape[1] or shape[3] != cache_shape[3]:
+        raise ValueError("the caches and the tokens disagree on batch, kv_heads or head_dim")
+    if dtype not in _DTYPES or v[2] != dtype:
+        raise ValueError("k and v must share a float16, bfloat16 or float32 dtype")
+    kind, tables = check_cache(k_cache, v_cache, scales)
+    for name, meta in (("k_cache", k_cache), ("v_cache", v_cache), ("scales", scales)):
+        if any(meta[1][d] == 0 and cache_shape[d] > 1 for d in range(3)):
+            raise ValueError(f"{name} is written: its rows may not share memory")
+    batch, kv_heads, tokens, head_dim = shape
+    if tokens == 0:
+        raise ValueError("append_quantized does not support empty dimensions")
+    lanes = min(1 << (head_dim * dtype.itemsize // 16 - 1).bit_length(), 64)
+    if batch * kv_heads * tokens * lanes >= 2**31 or tokens > 2**30:
+        raise ValueError("append_quantized: the problem is too large")
+    device = k_cache[3]
+    if k[3] != device or v[3] != device:
+        raise ValueError("k and v must be on the caches' device")
+    check_lengths(seqlens, "cache_seqlens", batch, device)
+    if counts is not None:
+        check_lengths(counts, "counts", batch, device)
+    unit = 16 // dtype.itemsize
+    tables += (_hip.row_strides("k", shape, k[1], 3, unit), _hip.row_strides("v", shape, v[1], 3, unit))
+    return device, kind, (batch, kv_heads, cache_shape[2], tokens, head_dim), tables
+
+
+@lru_cache(maxsize=1024)
+def _read_plan(dtype, k_cache, v_cache, scales, seqlens):
+    if dtype not in _DTYPES:
+        raise ValueError("read_quantized gives float16, bfloat16 or float32")
+    shape, device = tuple(k_cache[0]), k_cache[3]
+    if len(shape) != 4:
+        raise ValueError("read_quantized expects caches [batch, kv_heads, max_len, head_dim]")
+    kind, tables = check_cache(k_cache, v_cache, scales)
+    if shape[2] * shape[3] * dtype.itemsize // 16 > 2**31 - 257:
+        raise ValueError("read_quantized: the problem is too large")
+    if seqlens is not None:
+        check_lengths(seqlens, "cache_seqlens", shape[0], device)
+    return device, kind, shape, tables

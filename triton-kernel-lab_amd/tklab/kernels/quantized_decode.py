@@ -16,7 +16,7 @@ from functools import lru_cache
 import torch
 
 from tklab import _hip
-from tklab.kernels.quantized_cache import _cache_layout, _check_lengths
+from tklab.kernels.quantized_cache import cache_meta, check_cache, check_lengths, lengths_meta
 
 _DTYPES = (torch.float16, torch.bfloat16)
 _HEAD_DIMS = (64, 128)
@@ -50,7 +50,53 @@ def quantized_decode(
     Raises:
         ValueError: on an unsupported shape, dtype, layout or device.
     """
-    q_shape, cache_shape = q.shape, k_cache.shape
+    if scale is not None and not abs(scale) < 2.0**126:
+        raise ValueError("scale must be finite and below 2**126")
+    q_shape = q.shape
+    (batch, q_heads, head_dim), kv_heads, max_len, device, kind, slots, tables = _plan(
+        q_shape, q.stride(), q.dtype, q.get_device(), *cache_meta(k_cache, v_cache, scales),
+        None if cache_seqlens is None else lengths_meta(cache_seqlens))
+    q_ptr, k_ptr, v_ptr, s_ptr = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr()
+    if (q_ptr | k_ptr | v_ptr) & 15 or s_ptr & 7:
+        _hip.check_aligned(q=q_ptr, k_cache=k_ptr, v_cache=v_ptr)
+        raise ValueError("pairs of scales must be 8-byte aligned")
+    out = q.new_empty(q_shape)
+    lse = workspace = None
+    if return_lse:
+        lse = q.new_empty((batch, q_heads), dtype=torch.float32)
+    if slots:
+        # Float32 partial results, as twice as many elements of q's type.
+        workspace = q.new_empty(2 * slots * (q_heads // kv_heads) * (head_dim + 2))
+    _hip.call_on(
+        device,
+        "tk_quantized_decode",
+        _hip.DTYPE_CODES[q.dtype],
+        q_ptr,
+        k_ptr,
+        v_ptr,
+        s_ptr,
+        None if cache_seqlens is None else cache_seqlens.data_ptr(),
+        out.data_ptr(),
+        None if lse is None else lse.data_ptr(),
+        None if workspace is None else workspace.data_ptr(),
+        batch,
+        q_heads,
+        kv_heads,
+        max_len,
+        head_dim,
+        *tables,
+        head_dim ** -0.5 if scale is None else float(scale),
+        kind,
+        _hip.stream_on(device),
+    )
+    return (out, lse) if return_lse else out
+
+
+@lru_cache(maxsize=1024)
+def _plan(q_shape, q_strides, dtype, device, k_meta, v_meta, scales_meta, seqlens):
+    """Check the contract but for addresses and values: sizes, partial results that the library asks
+    for, and stride tables, made once for tensors alike."""
+    cache_shape = k_meta[0]
     if len(q_shape) != 3 or len(cache_shape) != 4:
         raise ValueError("quantized_decode expects q [batch, q_heads, head_dim] and caches [batch, "
                          "kv_heads, max_len, head_dim]")
@@ -66,60 +112,18 @@ def quantized_decode(
         raise ValueError("q_heads must be a multiple of kv_heads")
     if head_dim not in _HEAD_DIMS:
         raise ValueError("quantized_decode supports head_dim 64 and 128")
-    dtype = q.dtype
     if dtype not in _DTYPES:
         raise ValueError("q must be float16 or bfloat16")
-    if scale is not None and not abs(scale) < 2.0**126:
-        raise ValueError("scale must be finite and below 2**126")
-    (k_ptr, k_strides), (v_ptr, v_strides), (s_ptr, s_strides), kind = _cache_layout(
-        k_cache, v_cache, scales)
-    if max(k_strides[2], v_strides[2], s_strides[2]) >= 2**24:
+    kind, tables = check_cache(k_meta, v_meta, scales_meta)
+    if max(table[2] for table in tables) >= 2**24:
         raise ValueError("key strides must be below 2**24 elements")
-    device = k_cache.get_device()
-    q_ptr, q_strides = _hip.row_table(q, "q", device, 2, 8)
-    if cache_seqlens is not None:
-        _check_lengths(cache_seqlens, "cache_seqlens", batch, device)
-    group = q_heads // kv_heads
-    slots = _slots(batch, kv_heads, group, max_len, head_dim)
+    if k_meta[3] != device:
+        raise ValueError("q must be on the caches' device")
+    if seqlens is not None:
+        check_lengths(seqlens, "cache_seqlens", batch, device)
+    slots = _hip.query("tk_quantized_decode_slots", batch, kv_heads, q_heads // kv_heads, max_len, head_dim)
     if slots < 0:
         raise ValueError("quantized_decode: the problem is too large")
-    out = torch.empty(q_shape, dtype=dtype, device=q.device)
-    lse = workspace = None
-    if return_lse:
-        lse = torch.empty((batch, q_heads), dtype=torch.float32, device=q.device)
-    if slots:
-        # Float32 partial results, as twice as many elements of q's type.
-        workspace = q.new_empty(2 * slots * group * (head_dim + 2))
-    _hip.call_on(
-        device,
-        "tk_quantized_decode",
-        _hip.DTYPE_CODES[dtype],
-        q_ptr,
-        k_ptr,
-        v_ptr,
-        s_ptr,
-        None if cache_seqlens is None else cache_seqlens.data_ptr(),
-        out.data_ptr(),
-        None if lse is None else lse.data_ptr(),
-        None if workspace is None else workspace.data_ptr(),
-        batch,
-        q_heads,
-        kv_heads,
-        max_len,
-        head_dim,
-        q_strides,
-        k_strides,
-        v_strides,
-        s_strides,
-        _hip.int64_table((q_heads * head_dim, head_dim)),
-        head_dim ** -0.5 if scale is None else float(scale),
-        kind,
-        _hip.stream_on(device),
-    )
-    return (out, lse) if return_lse else out
-
-
-@lru_cache(maxsize=256)
-def _slots(batch: int, kv_heads: int, group: int, max_len: int, head_dim: int) -> int:
-    """Partial results per head of a group that the library asks for (a function of the sizes)."""
-    return _hip.query("tk_quantized_decode_slots", batch, kv_heads, group, max_len, head_dim)
+    tables = (_hip.row_strides("q", q_shape, q_strides, 2, 8), *tables,
+              _hip.int64_table((q_heads * head_dim, head_dim)))
+    return tuple(q_shape), kv_heads, max_len, device, kind, slots, tables
