@@ -16,10 +16,11 @@ constexpr float kNoMax = -3.0e38f;
 struct Schedule {
   const int32_t* seqlens;  // null: every sequence has max_len keys
   int batch, max_len;
-  int runs;       // the tiles of all sequences over this many runs give the run length
-  int min_chunk;  // tiles of the shortest run of a sequence that is split
-  int whole;      // a sequence of at most this many tiles is one run
+  int runs;   // the tiles of all sequences over this many runs give the run length
+  int fewer;  // and over this many where that makes runs of less than kLongRun tiles
+  int whole;  // a sequence of at most this many tiles is one run
 };
+constexpr int kMinRun = 2, kLongRun = 8;  // tiles
 
 __device__ __forceinline__ int context_length(const Schedule& s, int b) {
   const int n = s.seqlens != nullptr ? s.seqlens[b] : s.max_len;
@@ -58,7 +59,11 @@ __device__ __forceinline__ Lengths read_lengths(const Schedule& s, int lane) {
   int sum = lane < s.batch ? tiles_of(r.first) : 0;
   for (int b = lane + 64; b < s.batch; b += 64) sum += tiles_of(context_length(s, b));
   const int total = __builtin_amdgcn_readlane(wave_prefix(sum), 63);
-  r.chunk = max((total + s.runs - 1) / s.runs, s.min_chunk);
+  // One round of workgroups, unless that makes short runs: then half as many, as a workgroup's start and
+  // its partial results cost as much as some tiles (D128 e4m3, both kernels: B8 Hkv1 G32 L16384 25.3 ->
+  // 21.8 us, G8 16.7 -> 15.4; B1 Hkv8 G4 L2000 with 4 tiles 10.7, 2 tiles 9.6).
+  r.chunk = max((total + s.runs - 1) / s.runs, kMinRun);
+  if (r.chunk < kLongRun) r.chunk = max(r.chunk, min((total + s.fewer - 1) / s.fewer, kLongRun));
   return r;
 }
 
@@ -143,6 +148,82 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* p, int
   const uint32_t range = rows > 0 ? uint32_t(rows - 1) * stride + row : 0;
   return __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(p), (short)0,
                                            __builtin_amdgcn_readfirstlane(range), 0x00020000);
+}
+
+// ---- Joining partial results. One wave a row, or, for rows that leave CUs idle (at most kFewRows), a
+// workgroup of four: the parts are shared out among them (8 rows of 128 parts 21.3 -> 16.4 us for both
+// kernels, 1024 rows of few parts 92.5 -> 98.8). L = D / 4 lanes hold a partial row of O as float4, 64 / L
+// of them at a time in a wave, each slice of the lanes with a running maximum of its own; slices are
+// joined by exchanges, waves through LDS. The order is fixed.
+constexpr int kJoinWaves = 4;
+constexpr int64_t kFewRows = 256;
+
+template <int D>
+struct JoinScratch {
+  tk_attn::f32x4 acc[kJoinWaves][D / 4];
+  float top[kJoinWaves], sum[kJoinWaves];
+};
+
+// slot(i): index of part i of `parts`, i of which part_ml holds (reference maximum, sum) and part_o D
+// unnormalized floats. Writes the row of the output and, where `lse` is not null, its base-2 LSE; no
+// weight at all gives 0 and -inf. WAVES of the workgroup's waves, `wave` among them, join the row.
+template <typename T, int D, int WAVES, typename Slot>
+__device__ __forceinline__ void join_parts(const float* part_o, const float2* part_ml, int parts, Slot slot, T* out,
+                                           float* lse, int wave, JoinScratch<D>& shared) {
+  using tk_attn::f32x4;
+  constexpr int L = D / 4, S = 64 / L;
+  const int lane = threadIdx.x & 63;
+  const int d = lane % L;
+  float top = kNoMax, sum = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = (WAVES == 1 ? 0 : wave * S) + lane / L; i < parts; i += WAVES * S) {
+    const int64_t at = slot(i);
+    const float2 ml = part_ml[at];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(part_o + at * D + 4 * d);
+    const float next = fmaxf(top, ml.x);
+    const float old = __builtin_amdgcn_exp2f(top - next), fresh = __builtin_amdgcn_exp2f(ml.x - next);
+    top = next;
+    sum = sum * old + ml.y * fresh;
+    acc = acc * old + v * fresh;
+  }
+#pragma unroll
+  for (int x = L; x < 64; x <<= 1) {
+    const float other = __shfl_xor(top, x);
+    const float next = fmaxf(top, other);
+    const float mine = __builtin_amdgcn_exp2f(top - next), theirs = __builtin_amdgcn_exp2f(other - next);
+    top = next;
+    sum = sum * mine + __shfl_xor(sum, x) * theirs;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * mine + __shfl_xor(acc[i], x) * theirs;
+  }
+  if constexpr (WAVES > 1) {
+    if (lane < L) shared.acc[wave][d] = acc;
+    if (lane == 0) {
+      shared.top[wave] = top;
+      shared.sum[wave] = sum;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    float high = kNoMax;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) high = fmaxf(high, shared.top[i]);
+    sum = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      const float w = __builtin_amdgcn_exp2f(shared.top[i] - high);
+      sum += shared.sum[i] * w;
+      acc += shared.acc[i][d] * w;
+    }
+    top = high;
+  }
+  if (lane >= L) return;
+  float row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row[i] = sum == 0.f ? 0.f : acc[i] / sum;
+  tk::store_vec<T, 4>(out + 4 * d, row);
+  if (lane == 0 && lse != nullptr) *lse = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
 }  // namespace tk_runs

@@ -48,7 +48,7 @@ using tk_attn::i32x2;
 using tk_attn::i32x4;
 
 constexpr int kNonTemporal = 2;
-constexpr int kMinRun = 4;  // tiles of the shortest run of a part that is cut
+constexpr int kLeastRun = 4;  // tiles of the shortest run of a part that is cut
 
 struct PrefixArgs {
   const void *q, *kp, *vp, *k, *v;
@@ -102,8 +102,8 @@ __device__ __forceinline__ Deal make_deal(const PrefixArgs& a, int lane) {
   const int own_share = __builtin_amdgcn_readfirstlane(int(share));
   const int prefix_share = __builtin_amdgcn_readfirstlane(int(share * 16 / float(a.price)));
   // Own runs are half a share, so that the last ones to start are not long ones.
-  d.own_chunk = max(max(own_share / 2 + 1, kMinRun), (own + spare - 1) / spare);
-  const int chunk = max(prefix_share + 1, kMinRun);
+  d.own_chunk = max(max(own_share / 2 + 1, kLeastRun), (own + spare - 1) / spare);
+  const int chunk = max(prefix_share + 1, kLeastRun);
   const int runs = min((a.prefix_tiles + chunk - 1) / chunk, a.most_runs);
   d.prefix_chunk = (a.prefix_tiles + runs - 1) / runs;
   d.prefix_runs = (a.prefix_tiles + d.prefix_chunk - 1) / d.prefix_chunk;
@@ -635,15 +635,13 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(Pr
   }
 }
 
-// One wave per row (sequence, head): L = D / 4 lanes hold a row of O as float4, 64 / L partial results
-// at a time, the prefix's first, folded in a fixed order.
-constexpr int kCombineWaves = 4;
-template <typename T, int D, int W>
-__global__ __launch_bounds__(64 * kCombineWaves) void prefix_combine_kernel(PrefixArgs a) {
-  constexpr int L = D / 4, S = 64 / L;
+// A row's partial results, the prefix's first.
+template <typename T, int D, int W, int WAVES>
+__global__ __launch_bounds__(64 * kJoinWaves) void prefix_combine_kernel(PrefixArgs a) {
+  __shared__ JoinScratch<D> shared;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.x * kCombineWaves + wave;
+  const int h = WAVES == 1 ? blockIdx.x * kJoinWaves + wave : blockIdx.x;
   const int b = blockIdx.y;
   const Deal deal = make_deal<W>(a, lane);
   // Runs and first flat run of sequence b.
@@ -662,40 +660,16 @@ __global__ __launch_bounds__(64 * kCombineWaves) void prefix_combine_kernel(Pref
   if (h >= a.q_heads) return;
   const int kvh = a.by_group.div(h);
   const int g = h - kvh * a.group;
-  const int parts = deal.prefix_runs + splits;
   const int64_t prefix_step = int64_t(a.kv_heads) * a.rows, own_step = int64_t(a.kv_heads) * a.group;
   const int64_t prefix0 = int64_t(kvh) * a.rows + int64_t(b) * a.group + g;
   const int64_t own0 = int64_t(a.most_runs) * prefix_step + (int64_t(flat0) * a.kv_heads + kvh) * a.group + g;
-  auto slot = [&](int i) {
-    return i < deal.prefix_runs ? prefix0 + i * prefix_step : own0 + (i - deal.prefix_runs) * own_step;
-  };
-  float high = kNoMax;
-  for (int i = lane; i < parts; i += 64) high = fmaxf(high, a.part_ml[slot(i)].x);
-  high = tk::wave_allreduce(high, tk::MaxOp{});
-  float total = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const int part = lane / L, d = (lane % L) * 4;
-#pragma unroll 4
-  for (int i = part; i < parts; i += S) {
-    const int64_t at = slot(i);
-    const float2 ml = a.part_ml[at];
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
-    const float w = __builtin_amdgcn_exp2f(ml.x - high);
-    total += ml.y * w;
-    acc += v * w;
-  }
-#pragma unroll
-  for (int x = L; x < 64; x <<= 1) {
-    total += __shfl_xor(total, x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], x);
-  }
-  if (part != 0) return;
-  float out[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = acc[i] / total;
-  tk::store_vec<T, 4>(static_cast<T*>(a.o) + b * a.ob + h * a.oh + d, out);
-  if (lane == 0 && a.lse != nullptr) a.lse[int64_t(b) * a.q_heads + h] = high + log2f(total);
+  join_parts<T, D, WAVES>(a.part_o, a.part_ml, deal.prefix_runs + splits,
+                          [&](int i) {
+                            return i < deal.prefix_runs ? prefix0 + i * prefix_step
+                                                        : own0 + (i - deal.prefix_runs) * own_step;
+                          },
+                          static_cast<T*>(a.o) + b * a.ob + h * a.oh,
+                          a.lse == nullptr ? nullptr : a.lse + int64_t(b) * a.q_heads + h, wave, shared);
 }
 
 // Workgroup shapes by the rows a KV head has: 16 rows a wave up to four waves, then 32 rows a wave.
@@ -724,9 +698,13 @@ TK_SPLITS(_Float16);
 template <typename T, int D, int W, int MT>
 void launch_shape(const PrefixArgs& a, uint32_t workgroups, hipStream_t s) {
   hipLaunchKernelGGL((prefix_split_kernel<T, D, W, MT, D == 128 ? 4 : 8>), dim3(workgroups), dim3(64 * W), 0, s, a);
-  hipLaunchKernelGGL((prefix_combine_kernel<T, D, W>),
-                     dim3(static_cast<uint32_t>(tk::cdiv(a.q_heads, kCombineWaves)), a.batch),
-                     dim3(64 * kCombineWaves), 0, s, a);
+  if (int64_t(a.q_heads) * a.batch <= kFewRows)
+    hipLaunchKernelGGL((prefix_combine_kernel<T, D, W, kJoinWaves>), dim3(a.q_heads, a.batch),
+                       dim3(64 * kJoinWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL((prefix_combine_kernel<T, D, W, 1>),
+                       dim3(static_cast<uint32_t>(tk::cdiv(a.q_heads, kJoinWaves)), a.batch),
+                       dim3(64 * kJoinWaves), 0, s, a);
 }
 
 template <typename T, int D>
@@ -751,12 +729,12 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_le
   const Shape shape = shape_for(batch * group);
   p.row_blocks = tk::cdiv(batch * group, 16 * shape.waves * shape.row_tiles);
   const int64_t prefix_tiles = tk::cdiv(prefix_len, kTileKeys), own_tiles = tk::cdiv(max_len, kTileKeys);
-  // The prefix's runs if it were alone, and at most one for every kMinRun tiles.
+  // The prefix's runs if it were alone, and at most one for every kLeastRun tiles.
   p.most_runs = tk::cdiv(kWorkgroups, kv_heads * p.row_blocks);
-  if (p.most_runs > tk::cdiv(prefix_tiles, kMinRun)) p.most_runs = tk::cdiv(prefix_tiles, kMinRun);
+  if (p.most_runs > tk::cdiv(prefix_tiles, kLeastRun)) p.most_runs = tk::cdiv(prefix_tiles, kLeastRun);
   // The own runs if they were alone, and one more per sequence, which ends in a shorter one.
   p.most_own = tk::cdiv(2 * kWorkgroups * own_waves(shape.waves), kv_heads) + batch;
-  if (p.most_own > batch * tk::cdiv(own_tiles, kMinRun)) p.most_own = batch * tk::cdiv(own_tiles, kMinRun);
+  if (p.most_own > batch * tk::cdiv(own_tiles, kLeastRun)) p.most_own = batch * tk::cdiv(own_tiles, kLeastRun);
   p.workgroups = tk::cdiv(p.most_runs * kv_heads, 8) * 8 * p.row_blocks + tk::cdiv(p.most_own * kv_heads, own_waves(shape.waves));
   return p;
 }

@@ -45,7 +45,7 @@ struct DecodeArgs {
   float* part_o;   // [slot][head of the group][D], slot = (flat run, KV head)
   float2* part_ml; // [slot][head of the group]: reference maximum, sum
   int64_t qb, qh, ob, oh, kb, kh, kl, vb, vh, vl, sb, sh, sl;
-  tk::FastDiv by_kv_heads, by_row_blocks;
+  tk::FastDiv by_group, by_kv_heads, by_row_blocks;
   int q_heads, kv_heads, group, row_blocks, flat;
   float scale_log2;
 };
@@ -451,54 +451,27 @@ __global__ __launch_bounds__(64, 1) void quantized_split_kernel(DecodeArgs a) {
   }
 }
 
-// One wave per (sequence, KV head, head of the group): D / 4 lanes hold a row of O as float4, the
-// others other splits, folded in a fixed order.
-constexpr int kCombineWaves = 4;
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kCombineWaves) void quantized_combine_kernel(DecodeArgs a) {
-  constexpr int L = D / 4, S = 64 / L;
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * kJoinWaves) void quantized_combine_kernel(DecodeArgs a) {
+  __shared__ JoinScratch<D> shared;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = blockIdx.x * kCombineWaves + wave;
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int h = WAVES == 1 ? blockIdx.x * kJoinWaves + wave : blockIdx.x;
+  const int b = blockIdx.y;
   const Lengths lengths = read_lengths(a.schedule, lane);
   Run run;
   sequence_runs(a.schedule, lengths, b, lane, run);
-  if (run.splits == 1 || r >= a.group) return;
-  const int64_t step = int64_t(a.kv_heads) * a.group;  // rows between a head's splits
-  const int64_t at0 = (int64_t(run.flat0) * a.kv_heads + kvh) * a.group + r;
-  float high = kNoMax;
-  for (int i = lane; i < run.splits; i += 64) high = fmaxf(high, a.part_ml[at0 + i * step].x);
-  high = tk::wave_allreduce(high, tk::MaxOp{});
-  float total = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const int part = lane / L, d = (lane % L) * 4;
-#pragma unroll 4
-  for (int i = part; i < run.splits; i += S) {
-    const float2 ml = a.part_ml[at0 + i * step];
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + (at0 + i * step) * D + d);
-    const float w = __builtin_amdgcn_exp2f(ml.x - high);
-    total += ml.y * w;
-    acc += v * w;
-  }
-#pragma unroll
-  for (int x = L; x < 64; x <<= 1) {
-    total += __shfl_xor(total, x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], x);
-  }
-  if (part != 0) return;
-  const int h = kvh * a.group + r;
-  float out[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = total == 0.f ? 0.f : acc[i] / total;
-  tk::store_vec<T, 4>(static_cast<T*>(a.o) + b * a.ob + h * a.oh + d, out);
-  if (lane == 0 && a.lse != nullptr)
-    a.lse[int64_t(b) * a.q_heads + h] = total == 0.f ? -INFINITY : high + log2f(total);
+  if (run.splits == 1 || h >= a.q_heads) return;  // (one run: written by the split kernel)
+  const int kvh = a.by_group.div(h);
+  const int64_t step = int64_t(a.kv_heads) * a.group;  // between a head's splits
+  const int64_t at0 = (int64_t(run.flat0) * a.kv_heads + kvh) * a.group + (h - kvh * a.group);
+  join_parts<T, D, WAVES>(a.part_o, a.part_ml, run.splits, [&](int i) { return at0 + i * step; },
+                          static_cast<T*>(a.o) + b * a.ob + h * a.oh,
+                          a.lse == nullptr ? nullptr : a.lse + int64_t(b) * a.q_heads + h, wave, shared);
 }
 
 constexpr int kResident = 1024;  // workgroups that run at once: four per CU
-constexpr int kMinChunk = 4;
+constexpr int kWhole = 4;         // tiles of a sequence that is not split
 
 // Instantiated here by name: left to the launches below, the host compiler leaves some of these
 // kernels' launch stubs undefined.
@@ -517,18 +490,21 @@ void launch(const DecodeArgs& a, bool combine, hipStream_t s) {
     hipLaunchKernelGGL((quantized_split_kernel<T, kType, D, 1>), grid, dim3(64), 0, s, a);
   else
     hipLaunchKernelGGL((quantized_split_kernel<T, kType, D, 2>), grid, dim3(64), 0, s, a);
-  if (combine)
-    hipLaunchKernelGGL((quantized_combine_kernel<T, D>),
-                       dim3(static_cast<uint32_t>(tk::cdiv(a.group, kCombineWaves)), a.kv_heads,
-                            a.schedule.batch),
-                       dim3(64 * kCombineWaves), 0, s, a);
+  if (!combine) return;
+  if (int64_t(a.q_heads) * a.schedule.batch <= kFewRows)
+    hipLaunchKernelGGL((quantized_combine_kernel<T, D, kJoinWaves>), dim3(a.q_heads, a.schedule.batch),
+                       dim3(64 * kJoinWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL((quantized_combine_kernel<T, D, 1>),
+                       dim3(static_cast<uint32_t>(tk::cdiv(a.q_heads, kJoinWaves)), a.schedule.batch),
+                       dim3(64 * kJoinWaves), 0, s, a);
 }
 
 // How the call is cut: runs (the tiles of all sequences over `runs` give the run length), the bound
 // on their number, blocks of heads. The sequences' last runs are shorter, so `runs` leaves room for
 // one more per sequence where that keeps the launch to one round of workgroups.
 struct Plan {
-  int64_t row_blocks, runs, flat, whole;
+  int64_t row_blocks, runs, fewer, flat, whole;
   bool combine;
 };
 Plan make_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t max_len) {
@@ -537,10 +513,11 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t max_len) 
   const int64_t most = tk::cdiv(max_len, kTileKeys);
   const int64_t base = kResident / (kv_heads * p.row_blocks);
   p.runs = base > 2 * batch ? base - batch + 1 : base > 1 ? base : 1;
-  p.whole = kMinChunk;
+  p.fewer = base > 1 ? tk::cdiv(base, 2) : 1;
+  p.whole = kWhole;
   p.combine = most > p.whole;
   p.flat = p.runs + batch;
-  const int64_t bound = p.combine ? batch * tk::cdiv(most, kMinChunk) : batch;
+  const int64_t bound = p.combine ? batch * tk::cdiv(most, kMinRun) : batch;
   if (p.flat > bound) p.flat = bound;
   return p;
 }
@@ -620,7 +597,7 @@ extern "C" int tk_quantized_decode(int dtype, const void* q, const void* k_cache
   a.schedule.batch = static_cast<int>(batch);
   a.schedule.max_len = static_cast<int>(max_len);
   a.schedule.runs = static_cast<int>(plan.runs);
-  a.schedule.min_chunk = kMinChunk;
+  a.schedule.fewer = static_cast<int>(plan.fewer);
   a.schedule.whole = static_cast<int>(plan.whole);
   a.q = q;
   a.k = static_cast<const uint8_t*>(k_cache);
@@ -635,6 +612,7 @@ extern "C" int tk_quantized_decode(int dtype, const void* q, const void* k_cache
   a.kb = k_strides[0], a.kh = k_strides[1], a.kl = k_strides[2];
   a.vb = v_strides[0], a.vh = v_strides[1], a.vl = v_strides[2];
   a.sb = scale_strides[0], a.sh = scale_strides[1], a.sl = scale_strides[2];
+  a.by_group = tk::FastDiv(static_cast<uint32_t>(group));
   a.by_kv_heads = tk::FastDiv(static_cast<uint32_t>(kv_heads));
   a.by_row_blocks = tk::FastDiv(static_cast<uint32_t>(plan.row_blocks));
   a.q_heads = static_cast<int>(q_heads);
