@@ -326,3 +326,37 @@ def test_refused_layouts() -> None:
     ]:
         with pytest.raises(ValueError, match=message):
             append_quantized(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float32, 64), (torch.float16, 80)])
+def test_many_tokens_of_many_sequences(kind, dtype, dim) -> None:
+    """Several tokens a lane: calls of more workgroups than that needs, counts that end inside one."""
+    gen = torch.Generator("cuda").manual_seed(9)
+    batch, kv, tokens = 9, 5, 1203
+    cache = _cache(batch, kv, 1300, dim, kind)
+    k, v = (_rows(gen, batch, tokens, kv, dim, dtype=dtype).transpose(1, 2) for _ in "kv")
+    lens = torch.tensor([0, 97, 98, 500, 1299, 1300, 3, 64, 1], dtype=torch.int32, device="cuda")
+    counts = torch.tensor([1203, 1203, 1203, 7, 9, 9, 0, 1025, 17], dtype=torch.int32, device="cuda")
+    _check_append(*cache, lens, k, v, counts)
+    _check_append(*cache, lens, k, v)
+
+
+def test_append_refuses_more_rows_than_a_launch_holds() -> None:
+    from tklab.kernels.quantized_cache import _append_plan
+
+    def alike(*shape, dtype):
+        x = _meta(*shape, dtype=dtype)
+        return x.shape, x.stride(), x.dtype, 0
+
+    def plan(batch, kv, tokens, dim):
+        cache = alike(batch, kv, 64, dim, dtype=F8)
+        one = alike(batch, kv, tokens, dim, dtype=torch.float32)
+        return _append_plan(cache, cache, alike(batch, kv, 64, 2, dtype=torch.float32), alike(batch, dtype=I32), one,
+                            one, None)
+
+    assert plan(65535, 1024, 1, 64)[2] == (65535, 1024, 64, 1, 64)
+    for sizes in [(65535, 8192, 1, 64), (60000, 1, 60000, 1024), (1, 1, 2 ** 30 + 1, 16), (65535, 65535, 1, 16)]:
+        with pytest.raises(ValueError, match="too large"):
+            plan(*sizes)

@@ -11,7 +11,10 @@
 // from the next lane's, reading back ran at 2.4 TB/s. The same lanes take a token's key and its value,
 // so both rows' loads are in flight together and the pair of scales is one store.
 //
-// Bound by HBM: the tokens are read and the codes written once.
+// Bound by HBM: the tokens are read and the codes written once. 8 x 4096 tokens of 8 KV heads, D128, from
+// bf16: 38.6 us, 5.3 TB/s; padded to that from 0 to 4096 (120 MB) 25.7 us, 4.7 TB/s. With one token a
+// lane, heads apart and default stores of codes 42 to 45 and 32 us; four or eight tokens a lane 41 and 45.
+// Reading back 8 x 8192 positions 66.5 us, 6.1 TB/s.
 #include "eight_bit.hpp"
 #include "tk_common.hpp"
 
@@ -19,6 +22,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHeadDim = 1024;
+constexpr int kSteps = 2;  // tokens that a lane takes where this many workgroups are left
+constexpr int kManyWorkgroups = 1024;
 
 // PER codes as one access.
 template <int kPer>
@@ -34,9 +39,10 @@ struct AppendArgs {
   const int32_t* counts;  // null: every token
   int32_t* new_seqlens;
   int64_t cs[2][3], xs[2][3], ss[3];
-  tk::FastDiv tokens, heads;
-  int max_len, units, lanes_log2;  // units: 16-byte parts of a row of tokens
-  uint32_t rows;                   // batch * heads * tokens
+  tk::FastDiv head_blocks, token_blocks;
+  int tokens, heads, max_len;
+  int units, lanes_log2;       // 16-byte parts of a row of tokens; lanes a row
+  int tokens_log2, heads_log2; // rows side by side in a workgroup
 };
 
 __device__ __forceinline__ uint32_t row_max(uint32_t v, int lanes_log2) {
@@ -44,66 +50,90 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, int lanes_log2) {
   return v;
 }
 
-// 2^lanes_log2 lanes a row (a power of two), lane l its parts l, l + lanes, ..: up to NU.
-template <typename T, int kType, int NU>
+// 2^lanes_log2 lanes a row (a power of two), lane l its parts l, l + lanes, ..: up to NU. A workgroup
+// takes 2^tokens_log2 * STEPS tokens of 2^heads_log2 heads; neighbouring workgroups take the heads of
+// the same tokens, which lie side by side in a projection's output.
+template <typename T, int kType, int NU, int STEPS>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
   constexpr int PER = 16 / sizeof(T);
-  const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) >> a.lanes_log2;
+  typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+  const uint32_t tokens_of = a.head_blocks.div(blockIdx.x);
+  const int64_t b = a.token_blocks.div(tokens_of);
   const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
-  if (i >= a.rows) return;
-  const uint32_t pair = a.tokens.div(i);  // (batch entry, head)
-  const int t = int(i - pair * a.tokens.d);
-  const int64_t b = a.heads.div(pair);
-  const int64_t h = pair - b * int64_t(a.heads.d);
+  const int row = threadIdx.x >> a.lanes_log2;
+  const int t0 = (int(tokens_of - b * a.token_blocks.d) * STEPS << a.tokens_log2) +
+                 (row & ((1 << a.tokens_log2) - 1));
+  const int64_t h = ((blockIdx.x - tokens_of * a.head_blocks.d) << a.heads_log2) + (row >> a.tokens_log2);
   const int start = min(max(a.seqlens[b], 0), a.max_len);
-  const int tokens = int(a.tokens.d);
-  const int count = a.counts != nullptr ? min(max(a.counts[b], 0), tokens) : tokens;
-  if (h == 0 && t == 0 && lane == 0) a.new_seqlens[b] = start + min(count, a.max_len - start);
-  if (t >= count || t >= a.max_len - start) return;
-  float x[2][NU][PER];
+  const int given = a.counts != nullptr ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
+  const int count = min(given, a.max_len - start);
+  if (h == 0 && t0 == 0 && lane == 0) a.new_seqlens[b] = start + count;
+  if (t0 >= count || h >= a.heads) return;
+  u32x4v raw[STEPS][2][NU];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const T* p = static_cast<const T*>(a.x[w]) + b * a.xs[w][0] + h * a.xs[w][1] + t * a.xs[w][2];
+  for (int i = 0; i < STEPS; ++i) {
+    const int t = t0 + (i << a.tokens_log2);
 #pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      const int u = lane + (n << a.lanes_log2);
-      if (u < a.units) tk::load_vec_stream<T, PER>(p + u * PER, x[w][n]);
-    }
-  }
-  const int64_t at = int64_t(start) + t;
-  float scale[2];
+    for (int w = 0; w < 2; ++w) {
+      const T* p = static_cast<const T*>(a.x[w]) + b * a.xs[w][0] + h * a.xs[w][1] + t * a.xs[w][2];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    // Magnitudes compare as their bits, NaN above infinity above every number.
-    uint32_t most = 0;
-#pragma unroll
-    for (int n = 0; n < NU; ++n)
-      if (lane + (n << a.lanes_log2) < a.units)
-#pragma unroll
-        for (int j = 0; j < PER; ++j) most = max(most, __float_as_uint(x[w][n][j]) & 0x7FFFFFFFu);
-    most = row_max(most, a.lanes_log2);
-    const bool sound = most < 0x7F800000u;
-    const float top = fmaxf(__uint_as_float(most), 0x1p-100f);
-    const float inverse = tk8::kMost<kType> * (1.0f / top);
-    scale[w] = sound ? top / tk8::kMost<kType> : __uint_as_float(0x7FC00000u);
-    uint8_t* row = a.cache[w] + b * a.cs[w][0] + h * a.cs[w][1] + at * a.cs[w][2];
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      Codes<PER> codes;
-#pragma unroll
-      for (int j = 0; j < PER; j += 4) {
-        float v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = x[w][n][j + k] * inverse;
-        codes.c[j / 4] = sound ? tk8::encode4<kType>(v) : 0;
+      for (int n = 0; n < NU; ++n) {
+        const int u = lane + (n << a.lanes_log2);
+        raw[i][w][n] = t < count && u < a.units
+                           ? __builtin_nontemporal_load(reinterpret_cast<const u32x4v*>(p + u * PER))
+                           : u32x4v{0u, 0u, 0u, 0u};
       }
-      const int u = lane + (n << a.lanes_log2);
-      if (u < a.units) *reinterpret_cast<Codes<PER>*>(row + u * PER) = codes;
     }
   }
-  if (lane == 0)
-    *reinterpret_cast<float2*>(a.scales + b * a.ss[0] + h * a.ss[1] + at * a.ss[2]) =
-        make_float2(scale[0], scale[1]);
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int t = t0 + (i << a.tokens_log2);
+    const int64_t at = int64_t(start) + t;
+    float scale[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float x[NU][PER];
+      // Magnitudes compare as their bits, NaN above infinity above every number.
+      uint32_t most = 0;
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+        const auto v = __builtin_bit_cast(tk::Vec<T, PER>, raw[i][w][n]);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          x[n][j] = tk::to_f32(v.v[j]);
+          most = max(most, __float_as_uint(x[n][j]) & 0x7FFFFFFFu);
+        }
+      }
+      most = row_max(most, a.lanes_log2);
+      const bool sound = most < 0x7F800000u;
+      const float top = fmaxf(__uint_as_float(most), 0x1p-100f);
+      const float inverse = tk8::kMost<kType> * (1.0f / top);
+      scale[w] = sound ? top / tk8::kMost<kType> : __uint_as_float(0x7FC00000u);
+      uint8_t* out = a.cache[w] + b * a.cs[w][0] + h * a.cs[w][1] + at * a.cs[w][2];
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+        Codes<PER> codes;
+#pragma unroll
+        for (int j = 0; j < PER; j += 4) {
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = x[n][j + k] * inverse;
+          codes.c[j / 4] = sound ? tk8::encode4<kType>(v) : 0;
+        }
+        const int u = lane + (n << a.lanes_log2);
+        if (t >= count || u >= a.units) continue;
+        // Many tokens' codes pass through the caches; a few tokens' are read next.
+        if constexpr (STEPS > 1 && PER == 8)
+          __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, codes),
+                                      reinterpret_cast<uint64_t*>(out + u * PER));
+        else
+          *reinterpret_cast<Codes<PER>*>(out + u * PER) = codes;
+      }
+    }
+    if (t < count && lane == 0)
+      *reinterpret_cast<float2*>(a.scales + b * a.ss[0] + h * a.ss[1] + at * a.ss[2]) =
+          make_float2(scale[0], scale[1]);
+  }
 }
 
 struct ReadArgs {
@@ -161,22 +191,24 @@ const char* bad_strides(const int64_t* s, int64_t unit, int64_t batch, int64_t h
 }
 
 template <typename T, int kType>
-void launch_append(const AppendArgs& a, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>(tk::cdiv(int64_t(a.rows) << a.lanes_log2, kThreads)));
-  if (a.units <= 64)
-    hipLaunchKernelGGL((append_kernel<T, kType, 1>), grid, dim3(kThreads), 0, s, a);
+void launch_append(const AppendArgs& a, int steps, uint32_t workgroups, hipStream_t s) {
+  const dim3 grid(workgroups), block(kThreads);
+  if (a.units <= 64 && steps > 1)
+    hipLaunchKernelGGL((append_kernel<T, kType, 1, kSteps>), grid, block, 0, s, a);
+  else if (a.units <= 64)
+    hipLaunchKernelGGL((append_kernel<T, kType, 1, 1>), grid, block, 0, s, a);
   else if (sizeof(T) == 2 || a.units <= 128)
-    hipLaunchKernelGGL((append_kernel<T, kType, 2>), grid, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((append_kernel<T, kType, 2, 1>), grid, block, 0, s, a);
   else if constexpr (sizeof(T) == 4)
-    hipLaunchKernelGGL((append_kernel<T, kType, 4>), grid, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((append_kernel<T, kType, 4, 1>), grid, block, 0, s, a);
 }
 
 template <typename T>
-void launch_append(const AppendArgs& a, int type, hipStream_t s) {
+void launch_append(const AppendArgs& a, int type, int steps, uint32_t workgroups, hipStream_t s) {
   if (type == tk8::kE4M3)
-    launch_append<T, tk8::kE4M3>(a, s);
+    launch_append<T, tk8::kE4M3>(a, steps, workgroups, s);
   else
-    launch_append<T, tk8::kInt8>(a, s);
+    launch_append<T, tk8::kInt8>(a, steps, workgroups, s);
 }
 
 template <typename T>
@@ -215,10 +247,22 @@ extern "C" int tk_append_quantized(int dtype, void* k_cache, void* v_cache, floa
   a.units = static_cast<int>(head_dim * tk::elem_size(dtype) / 16);
   a.lanes_log2 = 0;
   while ((1 << a.lanes_log2) < a.units && a.lanes_log2 < 6) ++a.lanes_log2;
-  // A launch holds fewer than 2^32 threads, and rows are divided as numbers below 2^31.
-  const __int128 rows = static_cast<__int128>(batch) * kv_heads * tokens;
-  if ((rows << a.lanes_log2) >= (static_cast<__int128>(1) << 31))
-    return tk::fail("append: problem too large");
+  // Rows side by side: as many tokens as there are, then heads. Lanes take several tokens where enough
+  // workgroups are left.
+  const int rows_log2 = 8 - a.lanes_log2;
+  a.tokens_log2 = 0;
+  while (a.tokens_log2 < rows_log2 && (int64_t(1) << a.tokens_log2) < tokens) ++a.tokens_log2;
+  a.heads_log2 = rows_log2 - a.tokens_log2;
+  const int64_t head_blocks = tk::cdiv(kv_heads, int64_t(1) << a.heads_log2);
+  int64_t token_blocks = tk::cdiv(tokens, int64_t(1) << a.tokens_log2);
+  int steps = 1;
+  if (a.units <= 64 && batch * head_blocks * token_blocks >= kSteps * kManyWorkgroups) {
+    steps = kSteps;
+    token_blocks = tk::cdiv(tokens, int64_t(kSteps) << a.tokens_log2);
+  }
+  // A launch holds fewer than 2^32 threads, and workgroups are divided as numbers below 2^31.
+  const __int128 workgroups = static_cast<__int128>(batch) * head_blocks * token_blocks;
+  if (workgroups >= (static_cast<__int128>(1) << 24)) return tk::fail("append: problem too large");
   const int64_t* cache_strides[2] = {k_cache_strides, v_cache_strides};
   const int64_t* x_strides[2] = {k_strides, v_strides};
   for (int w = 0; w < 2; ++w) {
@@ -247,15 +291,17 @@ extern "C" int tk_append_quantized(int dtype, void* k_cache, void* v_cache, floa
   a.seqlens = seqlens;
   a.counts = counts;
   a.new_seqlens = new_seqlens;
-  a.tokens = tk::FastDiv(static_cast<uint32_t>(tokens));
-  a.heads = tk::FastDiv(static_cast<uint32_t>(kv_heads));
+  a.head_blocks = tk::FastDiv(static_cast<uint32_t>(head_blocks));
+  a.token_blocks = tk::FastDiv(static_cast<uint32_t>(token_blocks));
+  a.tokens = static_cast<int>(tokens);
+  a.heads = static_cast<int>(kv_heads);
   a.max_len = static_cast<int>(max_len);
-  a.rows = static_cast<uint32_t>(rows);
+  const uint32_t grid = static_cast<uint32_t>(workgroups);
   hipStream_t s = tk::as_stream(stream);
   switch (dtype) {
-    case TK_DTYPE_F32: launch_append<float>(a, cache_type, s); break;
-    case TK_DTYPE_F16: launch_append<_Float16>(a, cache_type, s); break;
-    default: launch_append<__bf16>(a, cache_type, s); break;
+    case TK_DTYPE_F32: launch_append<float>(a, cache_type, steps, grid, s); break;
+    case TK_DTYPE_F16: launch_append<_Float16>(a, cache_type, steps, grid, s); break;
+    default: launch_append<__bf16>(a, cache_type, steps, grid, s); break;
   }
   return tk::check_launch("append");
 }

@@ -210,8 +210,11 @@ def _append_plan(k_cache, v_cache, scales, seqlens, k, v, counts):
     batch, kv_heads, tokens, head_dim = shape
     if tokens == 0:
         raise ValueError("append_quantized does not support empty dimensions")
-    lanes = min(1 << (head_dim * dtype.itemsize // 16 - 1).bit_length(), 64)
-    if batch * kv_heads * tokens * lanes >= 2**31 or tokens > 2**30:
+    # Workgroups of 256 lanes, of which a row takes the power of two above its 16-byte parts.
+    rows = 256 // min(1 << (head_dim * dtype.itemsize // 16 - 1).bit_length(), 64)
+    side_by_side = min(1 << (tokens - 1).bit_length(), rows)
+    workgroups = batch * -(-tokens // side_by_side) * -(-kv_heads // (rows // side_by_side))
+    if workgroups >= 2**24 or tokens > 2**30:
         raise ValueError("append_quantized: the problem is too large")
     device = k_cache[3]
     if k[3] != device or v[3] != device:
