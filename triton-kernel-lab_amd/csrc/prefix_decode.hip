@@ -27,15 +27,20 @@
 // in every attention of this library; bfloat16 results are 2.3e-3 from float64's instead of 1.7e-3), O
 // once at the end.
 //
+// Rows past a workgroup's 128 make further row blocks, which read the same keys at about the same time:
+// they run on one XCD, and the prefix's loads are then ordinary ones, so that its L2 keeps a tile for all
+// of them (with non-temporal loads 845 MB came from HBM where 668 do: 149 -> 133 us; where one row block
+// reads the prefix, non-temporal ones are faster: 24.3 us against 26.0).
+//
 // What bounds it (bf16 D128 Hq32 Hkv8, both kernels): B128, prefix 32768, own lengths up to 2048 (668 MB,
-// 71 GFLOP) 149 us: every CU has one workgroup of each kind, a prefix tile takes 0.92 us beside own runs
+// 71 GFLOP) 133 us: every CU has one workgroup of each kind, a prefix tile takes 0.92 us beside own runs
 // (0.78 with the CU to itself: about 200 instructions of one wave a SIMD, 32 of them matrix ones) and HBM
-// delivers 5 TB/s. The same with own lengths of 2048 216 us, 5.6 TB/s; own caches alone (1.07 GB) 177 us,
-// 6.1 TB/s; the prefix alone 91 us, 0.76 PFLOP/s. B4 behind 2048 keys: 6 + 4 us, latencies.
-// Measured and not kept: tile after tile without overlap 172 us (the prefix alone 101); four own waves of
-// one stage each instead of two of two: 163 us, and own caches alone 187; a fifth ring stage, scheduling
-// groups that alternate matrix and vector instructions (149 to 152 us both); the exponentials of both row
-// tiles behind one test of the maximum, which leaves no registers (180 us).
+// delivers 5.3 TB/s. The same with own lengths of 2048 195 us, 6.2 TB/s; own caches alone (1.07 GB) 177 us,
+// 6.1 TB/s; the prefix alone 85 us, 0.8 PFLOP/s. B4 behind 2048 keys: 6.5 + 4.3 us, latencies.
+// Measured and not kept (against the 149 us): tile after tile without overlap 172 us (the prefix alone
+// 101); four own waves of one stage each instead of two of two: 163 us, and own caches alone 187; a fifth
+// ring stage, scheduling groups that alternate matrix and vector instructions (149 to 152 us both); the
+// exponentials of both row tiles behind one test of the maximum, which leaves no registers (180 us).
 #include "attention_dma.hpp"
 #include "decode_runs.hpp"
 #include "tk_common.hpp"
@@ -137,8 +142,9 @@ __device__ __forceinline__ bool find_own(const PrefixArgs& a, const Deal& d, int
 }
 
 // A tensor's rows as a stream of 32-row tiles into LDS; PER DMA instructions of this wave per tile,
-// from instruction `wave` * PER on. All fields but the lane offsets are wave-uniform.
-template <int D, int PER>
+// from instruction `wave` * PER on. All fields but the lane offsets are wave-uniform. POLICY 0 is for rows
+// that other workgroups read at about the same time.
+template <int D, int PER, int POLICY = kNonTemporal>
 struct Stream {
   using R = Ring<D>;
   const char* p;  // first row of the next tile
@@ -168,7 +174,7 @@ struct Stream {
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (tk_attn::lds_void*)(to + i * 1024), 16, off[i], 0, 0,
-                                               kNonTemporal);
+                                               POLICY);
     p += int64_t(kTileKeys) * row;
     left -= kTileKeys;
   }
@@ -443,8 +449,9 @@ struct Rows {
   }
 };
 
-// NS ring stages of a workgroup; an own run's wave has up to NS / own_waves(W) of them.
-template <typename T, int D, int W, int MT, int NS>
+// NS ring stages of a workgroup; an own run's wave has up to NS / own_waves(W) of them. kShared: there are
+// several row blocks, which share the prefix's tiles in L2.
+template <typename T, int D, int W, int MT, int NS, bool kShared>
 __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(PrefixArgs a) {
   using R = Ring<D>;
   constexpr int DC = D / 32;
@@ -492,7 +499,7 @@ __global__ __launch_bounds__(64 * W, W >= 4 ? 2 : 1) void prefix_split_kernel(Pr
         x.qf[m][c] = r < a.rows ? *reinterpret_cast<const i32x4*>(p + 32 * c) : i32x4{0, 0, 0, 0};
     }
     __builtin_amdgcn_sched_barrier(0);
-    Stream<D, PER> ks, vs;
+    Stream<D, PER, kShared ? 0 : kNonTemporal> ks, vs;
     const int first = t0 * kTileKeys;
     ks.template start<false>(static_cast<const T*>(a.kp) + kvh * a.kph + first * a.kpl, a.kpl, limit - first,
                              wave, lane);
@@ -687,17 +694,23 @@ constexpr int kWorkgroups = 512;  // two per CU, each with a 64 KiB ring
 
 // Instantiated here by name: left to the launches below, the host compiler leaves some of these
 // kernels' launch stubs undefined.
-#define TK_SPLIT(T, D, W, MT, NS) template __global__ void prefix_split_kernel<T, D, W, MT, NS>(PrefixArgs)
-#define TK_SPLITS(T)                                                                            \
-  TK_SPLIT(T, 128, 1, 1, 4); TK_SPLIT(T, 128, 2, 1, 4); TK_SPLIT(T, 128, 4, 1, 4);              \
-  TK_SPLIT(T, 128, 4, 2, 4); TK_SPLIT(T, 64, 1, 1, 8); TK_SPLIT(T, 64, 2, 1, 8);                \
-  TK_SPLIT(T, 64, 4, 1, 8); TK_SPLIT(T, 64, 4, 2, 8)
+#define TK_SPLIT(T, D, W, MT, NS, SHARED) \
+  template __global__ void prefix_split_kernel<T, D, W, MT, NS, SHARED>(PrefixArgs)
+#define TK_SPLITS(T)                                                                                  \
+  TK_SPLIT(T, 128, 1, 1, 4, false); TK_SPLIT(T, 128, 2, 1, 4, false); TK_SPLIT(T, 128, 4, 1, 4, false); \
+  TK_SPLIT(T, 128, 4, 2, 4, false); TK_SPLIT(T, 128, 4, 2, 4, true);                                  \
+  TK_SPLIT(T, 64, 1, 1, 8, false); TK_SPLIT(T, 64, 2, 1, 8, false); TK_SPLIT(T, 64, 4, 1, 8, false);  \
+  TK_SPLIT(T, 64, 4, 2, 8, false); TK_SPLIT(T, 64, 4, 2, 8, true)
 TK_SPLITS(__bf16);
 TK_SPLITS(_Float16);
 
 template <typename T, int D, int W, int MT>
 void launch_shape(const PrefixArgs& a, uint32_t workgroups, hipStream_t s) {
-  hipLaunchKernelGGL((prefix_split_kernel<T, D, W, MT, D == 128 ? 4 : 8>), dim3(workgroups), dim3(64 * W), 0, s, a);
+  constexpr int NS = D == 128 ? 4 : 8;
+  if (MT == 2 && a.row_blocks > 1)
+    hipLaunchKernelGGL((prefix_split_kernel<T, D, W, MT, NS, MT == 2>), dim3(workgroups), dim3(64 * W), 0, s, a);
+  else
+    hipLaunchKernelGGL((prefix_split_kernel<T, D, W, MT, NS, false>), dim3(workgroups), dim3(64 * W), 0, s, a);
   if (int64_t(a.q_heads) * a.batch <= kFewRows)
     hipLaunchKernelGGL((prefix_combine_kernel<T, D, W, kJoinWaves>), dim3(a.q_heads, a.batch),
                        dim3(64 * kJoinWaves), 0, s, a);
