@@ -342,6 +342,32 @@ def test_a_captured_training_step_replays() -> None:
 
 
 @pytest.mark.gpu
+def test_gradients_where_hooks_move_what_is_saved() -> None:
+    """A copy to the host and back is dense, whatever the views' strides were."""
+    joint = _make((3, 7, 6 * 64 + 40), torch.bfloat16, 61)
+    weights, freq = _weights(64, torch.bfloat16, 62), rotary_frequencies(32, device="cuda")[0]
+    pos = torch.arange(7, device="cuda").expand(3, 7)
+    dq, dk = _make((3, 4, 7, 64), torch.bfloat16, 63), _make((3, 2, 7, 64), torch.bfloat16, 64)
+
+    def gradients():
+        leaves = [joint[..., :4 * 64].view(3, 7, 4, 64).transpose(1, 2),
+                  joint[..., 4 * 64:6 * 64].view(3, 7, 2, 64).transpose(1, 2), *weights]
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        return torch.autograd.grad(qk_norm_rotary(*leaves, pos, freq), leaves, (dq, dk))
+
+    want = gradients()
+    with torch.autograd.graph.save_on_cpu():
+        got = gradients()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+    def whole(t):  # strides of the last dimension other than 1
+        return t.movedim(0, -1).contiguous().movedim(-1, 0) if t.ndim == 4 else t
+
+    with torch.autograd.graph.saved_tensors_hooks(whole, lambda t: t), pytest.raises(ValueError, match="contiguous"):
+        gradients()
+
+
+@pytest.mark.gpu
 def test_forward_mode_is_refused_not_dropped() -> None:
     from torch.autograd import forward_ad
 

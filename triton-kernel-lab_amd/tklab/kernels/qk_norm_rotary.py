@@ -59,17 +59,14 @@ def qk_norm_rotary(
         ``(q, k)`` with the inputs' shapes and memory order: statistics and rotation in float32,
         angles in float64, rounded once to the dtype. Differentiable in ``q``, ``k`` and both
         weights, in reverse mode only; the weights' gradients are summed in float32 in a fixed
-        order.
+        order. As with every autograd function, a backward pass is captured into a graph from leaves
+        of which no eager graph is alive.
 
     Raises:
         ValueError: on an unsupported shape, dtype, layout or device.
         RuntimeError: on a forward-mode tangent.
     """
-    plan = _plan(q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
-                 q_weight.shape, q_weight.stride(), q_weight.dtype, q_weight.get_device(),
-                 k_weight.shape, k_weight.stride(), k_weight.dtype, k_weight.get_device(),
-                 positions.shape, positions.stride(), positions.dtype, positions.get_device(),
-                 frequencies.shape, frequencies.stride(), frequencies.dtype, frequencies.get_device())
+    plan = _plan_of(q, k, q_weight, k_weight, positions, frequencies)
     validate_epsilon(eps)
     if not 2.0**-126 <= eps < 2.0**127:
         raise ValueError("eps must be a normal float32")
@@ -89,7 +86,7 @@ class _QkNormRotaryFunction(torch.autograd.Function):
         """Norm and turn."""
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
-        ctx.how = how, plan
+        ctx.how = how
         return _forward(q, k, q_weight, k_weight, positions, frequencies, how, plan)
 
     @staticmethod
@@ -102,7 +99,9 @@ class _QkNormRotaryFunction(torch.autograd.Function):
         sides = [s for s in sides if s[3] is not None and (need[s[0]] or need[s[0] + 2])]
         grads: list[torch.Tensor | None] = [None] * 8
         if sides:
-            results = _backward(sides, positions, frequencies, *ctx.how)
+            # Hooks on saved tensors may give them back with other strides.
+            plan = _plan_of(q, k, q_weight, k_weight, positions, frequencies)
+            results = _backward(sides, positions, frequencies, ctx.how, plan)
             for (which, *_), (dx, dw) in zip(sides, results):
                 grads[which] = dx if need[which] else None
                 grads[which + 2] = dw if need[which + 2] else None
@@ -195,6 +194,15 @@ def _like(x: torch.Tensor) -> torch.Tensor:
 def _strides(strides: tuple[int, ...]):
     """Table of ``{batch, head, token}`` strides."""
     return _hip.int64_table((0, strides[1], strides[0]) if len(strides) == 3 else tuple(strides[:3]))
+
+
+def _plan_of(q, k, q_weight, k_weight, positions, frequencies):
+    """:func:`_plan` of these tensors."""
+    return _plan(q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
+                 q_weight.shape, q_weight.stride(), q_weight.dtype, q_weight.get_device(),
+                 k_weight.shape, k_weight.stride(), k_weight.dtype, k_weight.get_device(),
+                 positions.shape, positions.stride(), positions.dtype, positions.get_device(),
+                 frequencies.shape, frequencies.stride(), frequencies.dtype, frequencies.get_device())
 
 
 @lru_cache(maxsize=1024)
