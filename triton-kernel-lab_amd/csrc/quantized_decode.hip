@@ -21,6 +21,13 @@
 // what the rounding left, as a second product: HBM leaves the matrix units the time (89.1 -> 89.7 us at
 // B32 L16384 ragged), and results are as near to float64's as float32 arithmetic's, 1.7e-3 of their
 // size in bfloat16 instead of 2.4e-3. Sums are float32.
+//
+// What bounds it (D128 Hkv8, both kernels): HBM. B32 Hq32 e4m3, ragged up to 16384 (508 MB) 90 us, 5.6 TB/s,
+// the last runs to end among it; of 8192 equal keys (554 MB) 95 us, 5.8; B2 Hq64 L131072 int8 (554 MB)
+// 90 us, 6.2. B1 L2000: 5.8 + 3.7 us, latencies one after the other.
+// Measured and not kept: ordinary loads in place of non-temporal ones (15 % more), a ring of 3 or 6 stages,
+// two rounds of workgroups, runs that may span sequences (ragged 95.5 -> 92.4 us, but equal 95 -> 101 and
+// B8 Hkv1 15.9 -> 20.2), a search of the least run length that fits (ragged 96 -> 93, equal 95.6 -> 102).
 #include "attention_dma.hpp"
 #include "decode_runs.hpp"
 #include "eight_bit.hpp"

@@ -55,9 +55,8 @@ def prefix_decode(
     """
     if scale is not None and not abs(scale) < 2.0**126:
         raise ValueError("scale must be finite and below 2**126")
-    q_shape = q.shape
     (batch, q_heads, head_dim), kv_heads, prefix_len, max_len, device, slots, tables = _plan(
-        q_shape, q.stride(), q.dtype, q.get_device(),
+        q.shape, q.stride(), q.dtype, q.get_device(),
         k_prefix.shape, k_prefix.stride(), k_prefix.dtype, k_prefix.get_device(),
         v_prefix.shape, v_prefix.stride(), v_prefix.dtype, v_prefix.get_device(),
         k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device(),
@@ -68,7 +67,7 @@ def prefix_decode(
     k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     if (q_ptr | kp_ptr | vp_ptr | k_ptr | v_ptr) & 15:
         _hip.check_aligned(q=q_ptr, k_prefix=kp_ptr, v_prefix=vp_ptr, k_cache=k_ptr, v_cache=v_ptr)
-    out = q.new_empty(q_shape)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = None
     if return_lse:
         lse = q.new_empty((batch, q_heads), dtype=torch.float32)

@@ -52,15 +52,14 @@ def quantized_decode(
     """
     if scale is not None and not abs(scale) < 2.0**126:
         raise ValueError("scale must be finite and below 2**126")
-    q_shape = q.shape
     (batch, q_heads, head_dim), kv_heads, max_len, device, kind, slots, tables = _plan(
-        q_shape, q.stride(), q.dtype, q.get_device(), *cache_meta(k_cache, v_cache, scales),
+        q.shape, q.stride(), q.dtype, q.get_device(), *cache_meta(k_cache, v_cache, scales),
         None if cache_seqlens is None else lengths_meta(cache_seqlens))
     q_ptr, k_ptr, v_ptr, s_ptr = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr()
     if (q_ptr | k_ptr | v_ptr) & 15 or s_ptr & 7:
         _hip.check_aligned(q=q_ptr, k_cache=k_ptr, v_cache=v_ptr)
         raise ValueError("pairs of scales must be 8-byte aligned")
-    out = q.new_empty(q_shape)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = workspace = None
     if return_lse:
         lse = q.new_empty((batch, q_heads), dtype=torch.float32)
