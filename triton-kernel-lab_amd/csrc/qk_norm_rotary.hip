@@ -3,8 +3,9 @@
 // R the rotation of rotary.hip over the first rotary_dim features. x is read and y written once;
 // everything between is float32 in registers. Rows and lanes: qk_norm_rotary.hpp.
 //
-// Bound by HBM: 2 x 8192 tokens of 32 query and 8 KV heads, D128, bf16 (336 MB) 61 us, 5.5 TB/s; 3 x 1000
-// tokens of 16 and 4 heads of 96 features, 48 of them turned, fp16 (23 MB) 12 us; one token 3.3 us.
+// Bound by HBM: 2 x 8192 tokens of 32 query and 8 KV heads, D128, bf16 (336 MB) 61 us, 5.5 TB/s (65 in
+// neighbouring pairs), of which the angles' arithmetic costs 3; 3 x 1000 tokens of 16 and 4 heads of 96
+// features, 48 of them turned, fp16 (23 MB) 10 us; one token 3.3 us.
 #include "qk_norm_rotary.hpp"
 
 namespace tk_qk_norm {
@@ -155,7 +156,10 @@ int plan(int dtype, const void* const pointers[2][4], const Tables tables[2], co
   a.rotated_units = interleaved && vec > 1 ? int(rotary_dim) / vec : half / (interleaved ? 1 : vec);
   a.units = a.rotated_units + int(head_dim - rotary_dim) / vec;
   a.lanes_log2 = 0;
-  while ((1 << a.lanes_log2) < a.units && a.lanes_log2 < 6) ++a.lanes_log2;
+  // Full vectors of the interleaved layout, which hold half the features of a unit of two, go two to a
+  // lane (D128 with one: forward 71 us, backward 120; with two 65 and 104).
+  const int per_lane = interleaved && vec * size == 16 ? 2 : 1;
+  while ((per_lane << a.lanes_log2) < a.units && a.lanes_log2 < 6) ++a.lanes_log2;
   units_per_lane = (a.units + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
   a.positions = positions;
   a.frequencies = frequencies;
@@ -208,7 +212,7 @@ template <typename T, int VEC, int NU>
 static void launch(const Args& a, bool interleaved, dim3 grid, size_t lds, hipStream_t s) {
   if (interleaved)
     hipLaunchKernelGGL((qk_norm_rotary_kernel<T, VEC, NU, true>), grid, dim3(kThreads), lds, s, a);
-  else
+  else if constexpr (VEC * NU < 16)  // (two units of 8 are of the interleaved layout)
     hipLaunchKernelGGL((qk_norm_rotary_kernel<T, VEC, NU, false>), grid, dim3(kThreads), lds, s, a);
 }
 

@@ -9,7 +9,9 @@
 // sums; a second kernel adds those rows in a fixed order. Results do not depend on timing.
 //
 // Bound by HBM: 2 x 8192 tokens of 32 query and 8 KV heads, D128, bf16 (503 MB) 100 us with the second
-// kernel's 4, 5 TB/s; 3 x 1000 tokens of 16 and 4 heads of 96 features, fp16 (35 MB) 20 + 4 us.
+// kernel's 4, 5 TB/s (104 in neighbouring pairs); 3 x 1000 tokens of 16 and 4 heads of 96 features, fp16
+// (35 MB) 20 + 4 us. Measured and not kept: four workgroups per CU in 128 registers, which spill (135 us),
+// runs twice as long (28 % more, the last round half empty) or half as long (6 % more, the angles' phases).
 #include "qk_norm_rotary.hpp"
 
 namespace tk_qk_norm {
@@ -161,7 +163,7 @@ static void launch(const Args& a, bool interleaved, hipStream_t s) {
   const dim3 grid(a.side[0].groups + a.side[1].groups);
   if (interleaved)
     hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, VEC, NU, true>), grid, dim3(kThreads), lds, s, a);
-  else
+  else if constexpr (VEC * NU < 16)  // (two units of 8 are of the interleaved layout)
     hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, VEC, NU, false>), grid, dim3(kThreads), lds, s, a);
 }
 
