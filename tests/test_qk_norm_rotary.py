@@ -342,6 +342,21 @@ def test_a_captured_training_step_replays() -> None:
 
 
 @pytest.mark.gpu
+def test_gradients_of_gradients_are_refused() -> None:
+    q, k = _make((5, 4, 64), torch.float32, 71), _make((5, 2, 64), torch.float32, 72)
+    leaves = [t.requires_grad_() for t in (q, k, *_weights(64, torch.float32, 73))]
+    freq, pos = rotary_frequencies(64, device="cuda")[0], torch.arange(5, device="cuda")
+    dq, dk = _make(q.shape, torch.float32, 74), _make(k.shape, torch.float32, 75)
+    want = torch.autograd.grad(qk_norm_rotary(*leaves, pos, freq), leaves, (dq, dk))
+    out = qk_norm_rotary(*leaves, pos, freq)
+    got = torch.autograd.grad(out, leaves, (dq.requires_grad_(), dk), create_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    for x in got:
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            x.sum().backward()
+
+
+@pytest.mark.gpu
 def test_gradients_where_hooks_move_what_is_saved() -> None:
     """A copy to the host and back is dense, whatever the views' strides were."""
     joint = _make((3, 7, 6 * 64 + 40), torch.bfloat16, 61)

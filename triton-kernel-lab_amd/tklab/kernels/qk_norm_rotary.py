@@ -90,22 +90,35 @@ class _QkNormRotaryFunction(torch.autograd.Function):
         return _forward(q, k, q_weight, k_weight, positions, frequencies, how, plan)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, dq_out, dk_out):
         """Gradients of the sides whose output was given one."""
-        q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        sides = [(0, q, q_weight, dq_out), (1, k, k_weight, dk_out)]
-        sides = [s for s in sides if s[3] is not None and (need[s[0]] or need[s[0] + 2])]
-        grads: list[torch.Tensor | None] = [None] * 8
-        if sides:
-            # Hooks on saved tensors may give them back with other strides.
-            plan = _plan_of(q, k, q_weight, k_weight, positions, frequencies)
-            results = _backward(sides, positions, frequencies, ctx.how, plan)
-            for (which, *_), (dx, dw) in zip(sides, results):
-                grads[which] = dx if need[which] else None
-                grads[which + 2] = dw if need[which + 2] else None
-        return tuple(grads)
+        if torch.is_grad_enabled():  # create_graph: the result is marked as not differentiable again
+            return _once_differentiable(ctx, dq_out, dk_out)
+        return _gradients(ctx, dq_out, dk_out)
+
+
+def _gradients(ctx: Any, dq_out, dk_out):
+    """Of all inputs, None where there is none or none is needed."""
+    q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
+    needs_q, needs_k, needs_q_weight, needs_k_weight, *_ = ctx.needs_input_grad
+    # Hooks on saved tensors may give them back with other strides.
+    plan = _plan_of(q, k, q_weight, k_weight, positions, frequencies)
+    _, sizes, q_strides, k_strides, *_ = plan
+    q_side = k_side = None
+    dq = dk = dq_weight = dk_weight = None
+    if dq_out is not None and (needs_q or needs_q_weight):
+        q_side = q, q_weight, dq_out, *q_strides, sizes[2]
+    if dk_out is not None and (needs_k or needs_k_weight):
+        k_side = k, k_weight, dk_out, *k_strides, sizes[3]
+    if q_side is not None:
+        dq, dq_weight, dk, dk_weight = _backward(q_side, k_side, positions, frequencies, ctx.how, plan)
+    elif k_side is not None:
+        dk, dk_weight, *_ = _backward(k_side, None, positions, frequencies, ctx.how, plan)
+    return (dq if needs_q else None, dk if needs_k else None, dq_weight if needs_q_weight else None,
+            dk_weight if needs_k_weight else None, None, None, None, None)
+
+
+_once_differentiable = once_differentiable(_gradients)
 
 
 def _forward(q, k, q_weight, k_weight, positions, frequencies, how, plan):
@@ -137,50 +150,53 @@ def _forward(q, k, q_weight, k_weight, positions, frequencies, how, plan):
     return q_out, k_out
 
 
-def _backward(sides, positions, frequencies, how, plan):
-    """(dx, dweight) of each side (which, x, weight, dy), one or two of them."""
-    device, sizes, *tables_of, position_strides, wide = plan
-    pointers, tables, weights, grads, held = [], [], [], [], []
-    for which, x, weight, dy in sides:
-        if dy.stride(-1) != 1:  # a broadcast gradient has stride 0
-            dy = dy.contiguous()
-        dx, dw = _like(x), torch.empty_like(weight)
-        x_strides, out_strides = tables_of[which]
-        pointers += (x.data_ptr(), dy.data_ptr(), dx.data_ptr())
-        tables += (x_strides, _strides(dy.stride()), out_strides)
-        weights.append(weight.data_ptr())
-        grads.append((dx, dw))
-        held.append(dy)  # until the call below: a copy's memory would be handed out again
-    pad = () if len(sides) == 2 else (None,)
-    batch, tokens, q_heads, kv_heads, *dims = sizes
-    heads = (q_heads, kv_heads)
-    partials = torch.empty((_PARTIAL_ROWS, dims[0]), dtype=torch.float32, device=positions.device)
+def _backward(first, second, positions, frequencies, how, plan):
+    """(dx, dweight) of one side or of both, each (x, weight, dy, strides, strides of dx, heads)."""
+    device, (batch, tokens, _, _, *dims), _, _, position_strides, wide = plan
+    x, weight, dy, strides, out_strides, heads = first
+    dx, dweight = _like(x), torch.empty_like(weight)
+    if dy.stride(-1) != 1:  # a broadcast gradient has stride 0
+        dy = dy.contiguous()
+    tables = (strides, _strides(dy.stride()), out_strides)
+    pointers = (x.data_ptr(), dy.data_ptr(), dx.data_ptr())
+    if second is None:
+        dx2 = dweight2 = None
+        more_pointers = more_tables = (None, None, None)
+        weights = (weight.data_ptr(), None, dweight.data_ptr(), None)
+        heads2 = 0
+    else:
+        x2, weight2, dy2, strides2, out_strides2, heads2 = second
+        dx2, dweight2 = _like(x2), torch.empty_like(weight2)
+        if dy2.stride(-1) != 1:
+            dy2 = dy2.contiguous()
+        more_tables = (strides2, _strides(dy2.stride()), out_strides2)
+        more_pointers = (x2.data_ptr(), dy2.data_ptr(), dx2.data_ptr())
+        weights = (weight.data_ptr(), weight2.data_ptr(), dweight.data_ptr(), dweight2.data_ptr())
+    # Float32, as elements of x's type.
+    partials = x.new_empty(_PARTIAL_ROWS * dims[0] * 4 // x.element_size())
     _hip.call_on(
         device,
         "tk_qk_norm_rotary_bwd",
-        _hip.DTYPE_CODES[sides[0][1].dtype],
+        _hip.DTYPE_CODES[x.dtype],
         *pointers,
-        *(pad * 3),
+        *more_pointers,
         *weights,
-        *pad,
-        *(dw.data_ptr() for _, dw in grads),
-        *pad,
         partials.data_ptr(),
         positions.data_ptr(),
         frequencies.data_ptr(),
         batch,
         tokens,
-        heads[sides[0][0]],
-        0 if pad else kv_heads,
+        heads,
+        heads2,
         *dims,
         *tables,
-        *(pad * 3),
+        *more_tables,
         position_strides,
         *how,
         wide,
         _hip.stream_on(device),
     )
-    return grads
+    return dx, dweight, dx2, dweight2
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
