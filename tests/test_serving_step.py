@@ -167,3 +167,34 @@ def test_a_captured_step_replays() -> None:
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(n, at)
     assert at.tolist() == [5, 6, 7, 8, 160]
+
+
+def test_two_batches_on_two_streams_at_once() -> None:
+    """Steps of two batches, sent for in turns: each call's workspace is its own."""
+    gen = torch.Generator("cuda").manual_seed(7)
+    batches = []
+    for heads, length in ((8, 3000), (32, 900)):
+        cache = [torch.randint(-100, 101, (BATCH, KV, length, DIM), generator=gen, device="cuda", dtype=torch.int8)
+                 for _ in "kv"]
+        scales = torch.rand(BATCH, KV, length, 2, generator=gen, device="cuda") * 0.02
+        prefix = [torch.randn(KV, 4 * length, DIM, generator=gen, device="cuda").to(DTYPE) for _ in "kv"]
+        own = [torch.randn(BATCH, KV, length, DIM, generator=gen, device="cuda").to(DTYPE) for _ in "kv"]
+        lens = torch.randint(1, length + 1, (BATCH,), generator=gen, device="cuda", dtype=torch.int32)
+        queries = [torch.randn(BATCH, heads, DIM, generator=gen, device="cuda").to(DTYPE) for _ in range(8)]
+        batches.append((queries, (*cache, scales, lens), (*prefix, *own, lens)))
+
+    def step(batch, i):
+        queries, cache, shared = batch
+        return (*quantized_decode(queries[i], *cache, return_lse=True), *prefix_decode(queries[i], *shared, return_lse=True))
+
+    want = [[step(batch, i) for i in range(8)] for batch in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    got = [[], []]
+    for i in range(8):
+        for batch, stream, into in zip(batches, streams, got):
+            with torch.cuda.stream(stream):
+                into.append(step(batch, i))
+    torch.cuda.synchronize()
+    for one, other in zip(got, want):
+        assert all(torch.equal(x, y) for a, b in zip(one, other) for x, y in zip(a, b))

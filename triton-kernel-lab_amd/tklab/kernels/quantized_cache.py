@@ -43,7 +43,8 @@ def append_quantized(
 
     Args:
         k_cache, v_cache: ``[batch, kv_heads, max_len, head_dim]`` float8_e4m3fn or int8, written in
-            place; head_dim a multiple of 16, at most 1024; rows 16-byte aligned.
+            place; head_dim a multiple of 16, at most 1024; rows 16-byte aligned; they may not overlap
+            one another.
         scales: float32 ``[batch, kv_heads, max_len, 2]``, written in place; pairs 8-byte aligned.
         cache_seqlens: int32 ``[batch]`` context lengths, clamped to ``[0, max_len]``.
         k, v: ``[batch, kv_heads, tokens, head_dim]`` float16, bfloat16 or float32, any strides whose
