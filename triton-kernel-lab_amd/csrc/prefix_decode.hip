@@ -43,7 +43,8 @@
 // exponentials of both row tiles behind one test of the maximum, which leaves no registers (180 us).
 // Against the 133 us: 32 rows of a wave on 32x32x16 products, half the matrix instructions at a lower clock
 // (133.7; equal lengths 191 for 195, but the prefix alone 90 for 86 and 256 sequences behind 16384 keys
-// 145 for 138).
+// 145 for 138); DMA and reads of keys issued among the output products, a higher priority for the prefix's
+// waves (no difference) or for the others (152).
 #include "attention_dma.hpp"
 #include "decode_runs.hpp"
 #include "tk_common.hpp"
