@@ -298,3 +298,101 @@ def test_slots_of_sizes_that_are_not_taken() -> None:
     for sizes in [(0, 8, 4, 2000, 128), (1, 8, 4, 2000, 96), (1, 8, -4, 2000, 128), (70000, 8, 4, 2000, 128),
                   (1, 8, 9000, 2000, 128), (1, 8, 4, 2 ** 31, 128), (60000, 1, 4, 2 ** 30, 128)]:
         assert _hip.query("tk_quantized_decode_slots", *sizes) == -1
+
+
+# ------------------------------------------------------------------ weights of very different sizes
+
+
+def _near(q, codes_k, codes_v, scales, factor):
+    """What one KV head's rows are in float64, and how far off a result may be whose weights go through
+    the second product as a bfloat16 and the bfloat16 of what that leaves.
+
+    Each of the two is off by at most 2^-8 of what it rounds, so both together by 2^-16 of a weight times
+    its scale, whatever the scales of other keys; the other terms are this module's.
+    """
+    s = scales.double()
+    keys, values = codes_k.double() * s[:, :1], codes_v.double() * s[:, 1:]
+    x, dim, n = q.double(), q.shape[-1], s.shape[0]
+    scores = x @ keys.t() * factor
+    delta = (dim + 8) * 2.0 ** -24 * (x.abs() @ keys.abs().t() * abs(factor)).amax(1, keepdim=True)
+    delta = delta + 2.0 ** -22 + 2.0 ** -23 * (scores.abs().amax(1, keepdim=True) * 1.45 + 8)
+    p = scores.softmax(1)
+    want, size = p @ values, p @ values.abs()
+    bound = 2.0 ** -16 * size + (2 * delta + (n + 64) * 2.0 ** -24) * (size + want.abs())
+    info = torch.finfo(q.dtype)
+    return want, bound + info.eps / 2 * (want.abs() + bound) + info.tiny * info.eps
+
+
+def _check_near(q, k, v, scales, some):
+    """Some (sequence, KV head)."""
+    out = quantized_decode(q, k, v, scales)
+    group = q.shape[1] // k.shape[1]
+    for b, g in some:
+        rows = slice(g * group, (g + 1) * group)
+        want, bound = _near(q[b, rows], k[b, g], v[b, g], scales[b, g], q.shape[-1] ** -0.5)
+        off = (out[b, rows].double() - want).abs()
+        assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("larger", [0, 5, 13, 20, 30])
+@pytest.mark.parametrize("above", [0, 14])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", HALF)
+def test_keys_beside_a_large_value_without_weight(dtype, kind, above, larger) -> None:
+    """One key whose value is 2^larger times the others' and whose weight is negligible, before or behind
+    them; and, `above` nats over the others, a key without a value. So many sequences that each is one run."""
+    q, k, v, scales = _problem(16, 128, 64, 1000, 64, dtype, kind, 20, spread=0)
+    # The first feature alone makes the difference: 8 times 1/8 times the key's.
+    q[..., 0] = 8
+    scales[..., 1] *= 64  # (results of normal float16 numbers)
+    k.view(torch.uint8)[..., 0] = 0
+    k.view(torch.uint8)[:, :, [3, 700, 40], :] = 0
+    one = torch.ones((), device="cuda").to(kind)
+    scales[:, :, [3, 700], 0], scales[:, :, 40, 0] = -40.0, float(above)
+    k.view(torch.uint8)[:, :, [3, 700, 40], 0] = one.view(torch.uint8)
+    scales[:8, :, 3, 1] *= 2.0 ** larger
+    scales[8:, :, 700, 1] *= 2.0 ** larger
+    v.view(torch.uint8)[:, :, 40] = 0
+    _check_near(q, k, v, scales, [(0, 0), (1, 63), (8, 5), (15, 31)])
+
+
+def _few_keys(dtype, kind, device):
+    """Values of both signs under weights of some size each: results below the sizes that were summed."""
+    gen = torch.Generator(device).manual_seed(21)
+    q = (0.3 * torch.randn(4, 8, 64, generator=gen, device=device)).to(dtype)
+    codes = [(50 * torch.randn(4, 2, 5, 64, generator=gen, device=device)).round().clamp(-120, 120).to(kind) for _ in "kv"]
+    return q, *codes, torch.rand(4, 2, 5, 2, generator=gen, device=device) * 0.01 + 0.01
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", HALF)
+def test_weights_keep_what_their_rounding_left(dtype, kind) -> None:
+    _check_near(*_few_keys(dtype, kind, "cuda"), [(b, g) for b in range(4) for g in range(2)])
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_the_bound_is_passed_by_weights_rounded_once(dtype) -> None:
+    """The same problem with weights of one rounding, on the CPU: what the bound has to notice."""
+    q, k, v, scales = _few_keys(dtype, torch.int8, "cpu")
+
+    def worst(parts):
+        most = 0.0
+        for b in range(4):
+            for g in range(2):
+                x, s = q[b, 4 * g: 4 * g + 4], scales[b, g]
+                want, bound = _near(x, k[b, g], v[b, g], s, 64 ** -0.5)
+                scores = x.double() @ (k[b, g].double() * s[:, :1]).t() * 64 ** -0.5
+                p = torch.exp(scores - scores.amax(1, keepdim=True))
+                weights = p * s[:, 1]
+                rounded = sum(parts(weights.float()))
+                got = ((rounded @ v[b, g].double()) / p.sum(1, keepdim=True)).to(dtype)
+                most = max(most, float(((got.double() - want).abs() / bound).max()))
+        return most
+
+    def pair(w):
+        first = w.bfloat16().float()
+        return first.double(), (w - first).bfloat16().double()
+
+    assert worst(lambda w: [w.to(dtype).double()]) > 1 and worst(pair) <= 1

@@ -6,21 +6,25 @@
 //
 // Split kernel: one wave per (run of 32-key tiles, KV head, block of 16 MT heads), both products on
 // v_mfma_f32_16x16x32 as in the 16-bit decode:
-//   S^T (16 keys x 16 heads) = K . Q^T. A lane's 16 bytes of a key are features 64 c + 16 quad .. +15:
+//   S^T (16 keys x 16 heads) = K . Q^T in q's type. A lane's 16 bytes of a key are features 64 c + 16 quad .. +15:
 //     two operands, with Q^T's features in the same order.
-//   O^T (16 dims x 16 heads) += V^T . P^T. P^T comes from the score registers, V^T from
+//   O^T (16 dims x 16 heads) += V^T . P^T in bfloat16. P^T comes from the score registers, V^T from
 //     ds_read_b64_tr_b8 (in each 16-lane group, lanes 2 j and 2 j + 1 read 16 bytes of row j, lane i
 //     receives column i of rows 0 .. 7): rows 4 quad .. +3 and 16 + 4 quad .. +3, the keys whose
 //     scores the lane holds.
 // K, V and the scales reach LDS by non-temporal buffer->LDS DMA into a ring of tiles.
 //
 // Weights. The running maximum m moves only when a tile's exceeds it by more than 8, so p <= 2^8.
-// p vs, divided by a running power of two above every |vs| met so far, is rounded to the storage dtype
-// for the second product: so no scale leaves that dtype's range, whatever the values' size (in float16
-// what falls below 2^-24 of the unit is lost, as in the 16-bit decode). The rounded part is followed by
-// what the rounding left, as a second product: HBM leaves the matrix units the time (89.1 -> 89.7 us at
-// B32 L16384 ragged), and results are as near to float64's as float32 arithmetic's, 1.7e-3 of their
-// size in bfloat16 instead of 2.4e-3. Sums are float32.
+// p vs, divided by a running power of two above every |vs| met so far so that no scale overflows, is
+// rounded to bfloat16 for the second product, and what that left to bfloat16 once more as a product of
+// its own: together off by at most 2^-16 of the weight, however small the weight is and whatever the other
+// keys' scales are. float16 cannot hold them: what falls below 2^-24 of the unit is nothing there (runs of
+// 1000 keys, one of them without a value and 14 nats above the rest, one with a value 32 times the others'
+// and no weight: results off by 20 to 44 %, now by 2.3e-4). HBM leaves the matrix units the time for the
+// second product: 89.1 -> 89.7 us at B32 L16384 ragged, and bfloat16 results are off by 1.65e-3 of their
+// size, as float32 arithmetic's are, instead of 2.4e-3; float16's by 2.1e-4, as those. Widening int8 codes
+// to bfloat16 costs float16 queries at D64 4 % (B32 L16384 110 -> 114 us), the others nothing. Sums are
+// float32.
 //
 // What bounds it (D128 Hkv8, both kernels): HBM. B32 Hq32 e4m3, ragged up to 16384 (508 MB) 90 us, 5.6 TB/s,
 // the last runs to end among it; of 8192 equal keys (554 MB) 95 us, 5.8; B2 Hq64 L131072 int8 (554 MB)
@@ -88,14 +92,9 @@ __device__ __forceinline__ i32x4 widen8(int lo, int hi) {
                widen2<T, kType, false>(hi), widen2<T, kType, true>(hi)};
 }
 
-// The low or high half of a register as float32.
-template <typename T>
+// The low or high bfloat16 of a register as float32.
 __device__ __forceinline__ float half_of(int x, int high) {
-  const uint16_t bits = uint16_t(uint32_t(x) >> (high ? 16 : 0));
-  if constexpr (__is_same(T, __bf16))
-    return __uint_as_float(uint32_t(bits) << 16);
-  else
-    return tk::to_f32(__builtin_bit_cast(_Float16, bits));
+  return __uint_as_float(high ? uint32_t(x) & 0xFFFF0000u : uint32_t(x) << 16);
 }
 
 template <int OFF>
@@ -403,24 +402,24 @@ __global__ __launch_bounds__(64, 1) void quantized_split_kernel(DecodeArgs a) {
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[i][r] *= vs[i][r];
-      pf[m][0] = tk_attn::acc_frag2<T>(p[0], p[1]);
+      pf[m][0] = tk_attn::acc_frag2<__bf16>(p[0], p[1]);
       f32x4 rest[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) rest[i][r] = p[i][r] - half_of<T>(pf[m][0][2 * i + r / 2], r % 2);
-      pf[m][1] = tk_attn::acc_frag2<T>(rest[0], rest[1]);
+        for (int r = 0; r < 4; ++r) rest[i][r] = p[i][r] - half_of(pf[m][0][2 * i + r / 2], r % 2);
+      pf[m][1] = tk_attn::acc_frag2<__bf16>(rest[0], rest[1]);
     }
     tk_attn::wait_lgkm<0>();
 #pragma unroll
     for (int c = 0; c < OC; ++c) asm volatile("" : "+v"(vc[c]));
 #pragma unroll
     for (int c = 0; c < OC; ++c) {
-      const i32x4 vf = widen8<T, kType>(vc[c][0], vc[c][1]);
+      const i32x4 vf = widen8<__bf16, kType>(vc[c][0], vc[c][1]);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) o[m][c] = tk_attn::Mma16<T>::run(vf, pf[m][e], o[m][c]);
+        for (int e = 0; e < 2; ++e) o[m][c] = tk_attn::Mma16<__bf16>::run(vf, pf[m][e], o[m][c]);
     }
   }
   // The tiles issued past the end still write (zeros) into the ring.

@@ -4,9 +4,9 @@
 reads KV head ``h // (q_heads // kv_heads)`` (``docs/research/gqa_decode_model.md``, "Semantic GQA
 mapping"), and the arithmetic is the reference attention forward's for one query row
 (``flash_attention.py:90-117, 248-264``) on keys and values ``code * scale``: the scales multiply
-scores and weights in float32, codes are exact in the query's dtype, and a weight times its value's
-scale goes through the second product as two numbers of that dtype, its rounding and what that left.
-Base-2 LSE. Inference only: there is no autograd.
+scores and weights in float32, codes are exact in float16 and bfloat16, and a weight times its value's
+scale goes through the second product as two bfloat16 numbers, its rounding and what that left: off by
+at most 2^-16 of itself, whatever the other keys' scales and weights. Base-2 LSE. Inference only: there is no autograd.
 """
 
 from __future__ import annotations
