@@ -332,3 +332,49 @@ def test_lengths_of_another_batch_are_refused() -> None:
                   dict(batch=4, lengths=4, dtype=torch.int64), dict(batch=4, lengths=4, device=1)):
         with pytest.raises(ValueError, match="cache_seqlens must be"):
             plan(**wrong)
+
+
+# ------------------------------------------------------------------ weights of very different sizes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [1, 2, 4, 8])
+@pytest.mark.parametrize("dtype", HALF)
+def test_keys_far_below_keys_without_values(dtype, heads) -> None:
+    """Every 512th key has no value and is 17 nats above the others, which are all there is to a result:
+    over runs of a thousand keys of the prefix and of the own caches, in each of the workgroups' shapes.
+
+    This module's tolerance, but for float16's subnormals: a weight is held in units of at most 2^-7 of its
+    run's largest, so one below 2^-14 of such a unit is off by 2^-32 of the largest weight at most.
+    """
+    batch, kv, dim = 16, 64, 64
+    q, kp, vp, k, v = _problem(batch, heads * kv, kv, 8192, 1024, dim, dtype, 30)
+    q[..., 0] = 8
+    for keys, values in ((kp, vp), (k, v)):
+        keys[..., 0] = 0
+        keys[..., 40::512, :] = 0
+        keys[..., 40::512, 0] = 17
+        values.copy_(values.abs() * 1024)  # of one sign, and results of normal float16 numbers
+        values[..., 40::512, :] = 0
+    out, lse = prefix_decode(q, kp, vp, k, v, return_lse=True)
+    half, info = torch.finfo(dtype).eps / 2, torch.finfo(dtype)
+    for b, g in ((0, 0), (7, 21), (15, 63)):
+        rows = slice(g * heads, (g + 1) * heads)
+        keys, values = torch.cat((kp[g], k[b, g])).double(), torch.cat((vp[g], v[b, g])).double()
+        x = q[b, rows].double()
+        scores = x @ keys.t() * dim ** -0.5
+        delta = (dim + 4) * 2.0 ** -24 * (x.abs() @ keys.abs().t() * dim ** -0.5).amax(1, keepdim=True)
+        delta = delta + 2.0 ** -22 + 2.0 ** -23 * (scores.abs().amax(1, keepdim=True) * 1.45 + 8)
+        log = torch.logsumexp(scores, 1, keepdim=True)
+        p = torch.exp(scores - log)
+        want, spread = p @ values, p @ values.abs()
+        count = (keys.shape[0] + 64) * 2.0 ** -24
+        bound = half * spread + (2 * delta + count) * (spread + want.abs())
+        if dtype == torch.float16:
+            bound = bound + 2.0 ** -32 * p.amax(1, keepdim=True) * values.abs().sum(0)
+        bound = bound + half * (want.abs() + bound) + info.tiny * info.eps
+        off = (out[b, rows].double() - want).abs()
+        assert bool((off <= bound).all()), float((off / bound).max())
+        lse_off = (lse[b, rows].double() - log[:, 0] / math.log(2)).abs()
+        lse_bound = (delta[:, 0] + count) * 1.45 + 2.0 ** -22 * (log[:, 0].abs() * 1.45 + 1)
+        assert bool((lse_off <= lse_bound).all()), float((lse_off / lse_bound).max())

@@ -167,10 +167,12 @@ struct JoinScratch {
   float top[kJoinWaves], sum[kJoinWaves];
 };
 
-// slot(i): index of part i of `parts`, i of which part_ml holds (reference maximum, sum) and part_o D
-// unnormalized floats. Writes the row of the output and, where `lse` is not null, its base-2 LSE; no
-// weight at all gives 0 and -inf. WAVES of the workgroup's waves, `wave` among them, join the row.
-template <typename T, int D, int WAVES, typename Slot>
+// slot(i): index of part i of `parts`, i of which part_ml holds (reference of the exponentials, their sum)
+// and part_o D unnormalized floats. Writes the row of the output and, where `lse` is not null, its base-2
+// LSE; no weight at all gives 0 and -inf. References lie kLift below maxima: without it the sum's logarithm
+// is the smaller and the LSE's rounding with it (7.7e-8 of it for 4.5e-8). WAVES of the workgroup's waves,
+// `wave` among them, join the row.
+template <typename T, int D, int WAVES, int kLift = 0, typename Slot>
 __device__ __forceinline__ void join_parts(const float* part_o, const float2* part_ml, int parts, Slot slot, T* out,
                                            float* lse, int wave, JoinScratch<D>& shared) {
   using tk_attn::f32x4;
@@ -226,7 +228,7 @@ __device__ __forceinline__ void join_parts(const float* part_o, const float2* pa
 #pragma unroll
   for (int i = 0; i < 4; ++i) row[i] = sum == 0.f ? 0.f : acc[i] / sum;
   tk::store_vec<T, 4>(out + 4 * d, row);
-  if (lane == 0 && lse != nullptr) *lse = sum == 0.f ? -INFINITY : top + log2f(sum);
+  if (lane == 0 && lse != nullptr) *lse = sum == 0.f ? -INFINITY : top + kLift + log2f(sum * (1.f / (1 << kLift)));
 }
 
 }  // namespace tk_runs

@@ -23,9 +23,12 @@
 // that run at once, with a prefix tile priced against an own one; the prefix's runs are a share long and
 // come first, own ones half a share, so that none that starts late ends late.
 //
-// Softmax statistics and sums are float32, P is rounded to the storage dtype for the second product (as
-// in every attention of this library; bfloat16 results are 2.3e-3 from float64's instead of 1.7e-3), O
-// once at the end.
+// Softmax statistics and sums are float32, P is rounded to the storage dtype for the second product, as
+// in every attention of this library: bfloat16 results are 2.3e-3 from float64's instead of 1.7e-3, float16
+// ones 2.9e-4 instead of 2.1e-4. (What the rounding leaves as a second product would have to be in both
+// parts and in every shape, or a sequence's accuracy would depend on its batch: 11.0 -> 11.5 us for a few
+// sequences, 41.7 -> 43.3 at 16, and 16 matrix instructions more beside a tile's 32 in the prefix part of
+// many rows, which issue bounds.) O is rounded once at the end.
 //
 // Rows past a workgroup's 128 make further row blocks, which read the same keys at about the same time:
 // they run on one XCD, and the prefix's loads are then ordinary ones, so that its L2 keeps a tile for all
@@ -192,7 +195,7 @@ struct Rows {
   static constexpr int HB = 4;  // output chunks per batch of V reads
   i32x4 qf[MT][DC];
   f32x4 o[MT][OC];
-  float top[MT], sum[MT];  // reference maximum of row row16, this lane's share of its sum
+  float top[MT], sum[MT];  // reference of row row16's exponentials, this lane's share of their sum
   uint32_t ka[DC], va[OC];
 
   __device__ __forceinline__ void start(int row16, int quad) {
@@ -257,9 +260,13 @@ struct Rows {
     }
   }
 
-  // P = exp2(scale s - top) into pf. The reference maximum moves only when the tile's exceeds it by
-  // more than 8 (base 2), so p <= 2^8 and o and sum are rescaled in few tiles: a lane whose
-  // exponentials sum to at most 2^8 has none above it, and then no maximum is formed.
+  // P = exp2(scale s - top) into pf. The reference moves only when the tile's maximum exceeds it by
+  // more than kMost (base 2), and then to kLift below that, so p <= 2^kMost and o and sum are rescaled in
+  // few tiles: a lane whose exponentials sum to at most 2^kMost has none above it, and then no maximum is
+  // formed. In float16 P is kept near that type's upper end: below 2^-14 it is off by up to 2^-25, with the
+  // lift 2^-32 of the run's largest (where valueless keys are 17 or 20 nats above the others, results were
+  // off by 3.8 % and 88 % without it and are by 1.7e-4 and 6e-4, at no cost). bfloat16 has float32's range.
+  static constexpr int kLift = __is_same(T, __bf16) ? 0 : 7, kMost = kLift + 8;
   __device__ __forceinline__ void weigh(const f32x4 (&s)[2], float scale, int m, f32x4 (&p)[2], float& part) const {
     part = 0.f;
 #pragma unroll
@@ -272,14 +279,14 @@ struct Rows {
   }
   __device__ __forceinline__ void settle(const f32x4 (&s)[2], float scale, int m, f32x4 (&p)[2], float part,
                                          i32x4& pf) {
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(part <= 256.f)) != 0, 0)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(part <= float(1 << kMost))) != 0, 0)) {
       float high = s[0][0];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) high = fmaxf(high, s[i][r]);
       high = tk_attn::max_over_column(high) * scale;
-      const float next = high > top[m] + 8.f ? high : top[m];
+      const float next = high > top[m] + kMost ? high - kLift : top[m];
       const float alpha = __builtin_amdgcn_exp2f(top[m] - next);
       top[m] = next;
       sum[m] *= alpha;
@@ -674,7 +681,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void prefix_combine_kernel(PrefixA
   const int64_t prefix_step = int64_t(a.kv_heads) * a.rows, own_step = int64_t(a.kv_heads) * a.group;
   const int64_t prefix0 = int64_t(kvh) * a.rows + int64_t(b) * a.group + g;
   const int64_t own0 = int64_t(a.most_runs) * prefix_step + (int64_t(flat0) * a.kv_heads + kvh) * a.group + g;
-  join_parts<T, D, WAVES>(a.part_o, a.part_ml, deal.prefix_runs + splits,
+  join_parts<T, D, WAVES, Rows<T, D, 1>::kLift>(a.part_o, a.part_ml, deal.prefix_runs + splits,
                           [&](int i) {
                             return i < deal.prefix_runs ? prefix0 + i * prefix_step
                                                         : own0 + (i - deal.prefix_runs) * own_step;

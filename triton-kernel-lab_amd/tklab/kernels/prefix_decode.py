@@ -5,7 +5,8 @@ reads them once for every sequence; :func:`prefix_decode` takes them as tensors 
 dimension, reads them once for the whole batch, and attends over each sequence's own cache in the same
 launch. Head mapping and arithmetic are ``gqa_decode``'s (``docs/research/gqa_decode_model.md``,
 "Semantic GQA mapping"; ``flash_attention.py:90-117, 248-264``): scores scaled by ``scale * log2(e)``, P
-rounded to the storage dtype before the PV product, base-2 LSE. Inference only: there is no autograd.
+rounded to the storage dtype before the PV product (in float16 a weight below 2^-21 of the largest is off
+by up to 2^-32 of that), base-2 LSE. Inference only: there is no autograd.
 """
 
 from __future__ import annotations
