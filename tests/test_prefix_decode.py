@@ -378,3 +378,15 @@ def test_keys_far_below_keys_without_values(dtype, heads) -> None:
         lse_off = (lse[b, rows].double() - log[:, 0] / math.log(2)).abs()
         lse_bound = (delta[:, 0] + count) * 1.45 + 2.0 ** -22 * (log[:, 0].abs() * 1.45 + 1)
         assert bool((lse_off <= lse_bound).all()), float((lse_off / lse_bound).max())
+
+
+def test_more_work_than_a_share_counts_is_refused() -> None:
+    """Tiles of a workgroup's share are counted in 32 bits: views that repeat positions or heads reach
+    sizes at which that would overflow (a prefix of 2^30 keys and 32600 heads), calls of many minutes."""
+    from tklab import _hip
+
+    for sizes in [(128, 32600, 1, 2 ** 30, 32, 64), (1, 65535, 1, 2 ** 30, 32, 64), (31, 2040, 1, 32, 2 ** 30, 64),
+                  (30, 65535, 1, 33, 2 ** 30, 128), (65535, 16, 64, 2 ** 30, 32, 64)]:
+        assert _hip.query("tk_prefix_decode_slots", *sizes) == -1
+    for sizes in [(128, 8, 4, 2 ** 30, 32, 64), (31, 8, 4, 32, 2 ** 30, 128), (1, 4096, 1, 2 ** 30, 32, 64)]:
+        assert _hip.query("tk_prefix_decode_slots", *sizes) > 0

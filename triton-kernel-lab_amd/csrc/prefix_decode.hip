@@ -764,7 +764,7 @@ Plan make_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_le
 }
 
 // Why a problem of these (positive) sizes is not taken, or null. The grid holds at most 2^22
-// workgroups, and tiles and partial results are counted in 32 bits.
+// workgroups, and tiles, partial results and a share's tiles (make_deal) are counted in 32 bits.
 const char* unsupported(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len, int64_t max_len,
                         int64_t head_dim) {
   if (head_dim != 64 && head_dim != 128) return "head_dim must be 64 or 128";
@@ -775,6 +775,10 @@ const char* unsupported(int64_t batch, int64_t kv_heads, int64_t group, int64_t 
   if (batch * tk::cdiv(max_len, kTileKeys) > INT32_MAX / 2 || p.workgroups > (1 << 22) ||
       p.most_runs * kv_heads * batch * group + p.most_own * kv_heads * group > INT32_MAX)
     return "problem too large";
+  const Shape shape = shape_for(batch * group);
+  const double prefix_work = double(tk::cdiv(prefix_len, kTileKeys)) * double(kv_heads * p.row_blocks);
+  const double own_work = double(batch * tk::cdiv(max_len, kTileKeys)) * double(kv_heads) / own_waves(shape.waves);
+  if (prefix_work + own_work * 16 / shape.price > double(kWorkgroups) * (1 << 30)) return "problem too large";
   return nullptr;
 }
 
