@@ -108,13 +108,6 @@ struct Row {
     }
   };
 
-  static __device__ __forceinline__ void load_weight(const void* weight, const Layout& at,
-                                                     float (&w)[NU][N]) {
-    Raw raw;
-    raw.load(static_cast<const T*>(weight), at);
-    raw.expand(at, w);
-  }
-
   // Non-temporal stores: they leave the caches to the tensors that are read again (B2 N8192 Hq32 Hkv8 D128:
   // a forward followed by its backward 162 us, 173 with ordinary stores; each among its like 61 and 100, 59
   // and 96 with ordinary ones).

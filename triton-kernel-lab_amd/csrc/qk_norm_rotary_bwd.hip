@@ -131,7 +131,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rotary_bwd_kernel(Args a) {
 }
 
 // Sums of the partial rows: 8 features by 128 slices of the rows a workgroup, so that a thread adds a
-// handful of rows (32 features by 32 slices: 9.9 us at 1023 rows, the loads one behind the other).
+// handful of rows (32 features by 32 slices: 9.9 us, the loads one behind the other, where the partial rows
+// were 1023; now they are kGroups at most).
 constexpr int kCols = 8, kSlices = 128;
 template <typename T>
 __global__ __launch_bounds__(kCols* kSlices) void qk_norm_weight_kernel(Args a) {
