@@ -4,8 +4,8 @@
 // A key's scale multiplies its score and a value's its weight, so codes are only widened (exact in
 // both 16-bit types) and no row is ever multiplied out.
 //
-// Split kernel: one wave per (run of 32-key tiles, KV head, block of 16 MT heads), both products on
-// v_mfma_f32_16x16x32 as in the 16-bit decode:
+// Split kernel: one wave per (run of 32-key tiles, KV head, block of 16 MT heads; groups above 32 heads read
+// the cache once for every 32), both products on v_mfma_f32_16x16x32 as in the 16-bit decode:
 //   S^T (16 keys x 16 heads) = K . Q^T in q's type. A lane's 16 bytes of a key are features 64 c + 16 quad .. +15:
 //     two operands, with Q^T's features in the same order.
 //   O^T (16 dims x 16 heads) += V^T . P^T in bfloat16. P^T comes from the score registers, V^T from
